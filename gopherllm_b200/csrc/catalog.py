@@ -4,13 +4,13 @@ from __future__ import annotations
 from typing import Iterable, Iterator, Tuple
 
 # libraries that do not depend on a model's sizes
-GENERAL = ("rowwise.cu", "qkv_cache.cu", "attention_generic.cu", "attention_mixed.cu", "latent.cu", "recurrent.cu", "memory_chunks.cu", "selective_scan.cu",
+GENERAL = ("rowwise.cu", "qkv_cache.cu", "attention_generic.cu", "attention_spans_f32.cu", "cache_evict.cu", "attention_mixed.cu", "latent.cu", "recurrent.cu", "memory_chunks.cu", "selective_scan.cu",
            "gated_unit.cu", "streams.cu", "moe.cu", "gemm_simt.cu", "gemm_skinny.cu", "gemm_stream.cu",
            "gemm_tcgen05.cu", "sampling.cu")
 
 # libraries compiled once per head size (GL_HEAD_DIM)
 PER_HEAD_DIM: Tuple[str, ...] = ("attention_decode.cu", "attention_prefill.cu", "attention_prefill_tc.cu",
-                                  "decode_layer.cu")
+                                  "decode_layer.cu", "attention_spans.cu")
 # libraries compiled once per (key size, value size): GL_HEAD_DIM and, where it differs, GL_VALUE_DIM
 PER_PAIR_DIMS: Tuple[str, ...] = ("attention_mixed_tc.cu",)
 # libraries that take only some head sizes

@@ -12,6 +12,7 @@ import os
 from ctypes import POINTER, Structure, byref, c_float, c_int, c_void_p
 from typing import Optional
 
+import numpy as np
 import torch
 
 from .csrc import build, catalog
@@ -829,6 +830,291 @@ def attention(q, out, k_cache, v_cache, ctx, pages, num_heads: int, num_kv_heads
         return
     attention_generic(q, out, k_cache, v_cache, ctx.seq_qstart, ctx.seq_qlen, ctx.seq_ctx, pages,
                       num_heads, num_kv_heads, head_dim, ctx.max_qlen, window)
+
+
+# ---------------------------------------------------------------------------
+# A cache that sequences share, and that forgets.
+class PrefixPlan:
+    """Which sequences of a batch have their first pages in common, and how their attention is shared out among blocks:
+    made by ``prefix_plan`` for the batch's composition and kept as long as that stays (the sequences' own positions
+    may grow).  ``ints`` on the device: the sequences group by group, the items of the shared pages, and for every sequence the
+    pages it shares and the slots their results take."""
+
+    def __init__(self, layout: "PrefixLayout", ints: torch.Tensor):
+        self.layout, self.ints = layout, ints
+
+
+class PrefixLayout:
+    """The host's part of a ``PrefixPlan``: ``ints`` (numpy int32: what the device needs) and sizes."""
+
+    def __init__(self, groups, batch: int, num_heads: int, num_kv_heads: int, head_dim: int, dtype, own: int, sms: int):
+        if batch < 1 or num_heads < 1 or num_kv_heads < 1 or num_heads % num_kv_heads:
+            raise KernelError(f"prefix_plan: {batch} sequences of {num_heads} heads on {num_kv_heads} key/value heads")
+        if own < 1:
+            raise KernelError("prefix_plan: every sequence has a position of its own at least, the one its token is at")
+        _check_span_heads("prefix_plan", dtype, head_dim)
+        self.batch, self.num_heads, self.num_kv_heads, self.head_dim, self.dtype = batch, num_heads, num_kv_heads, head_dim, dtype
+        group = num_heads // num_kv_heads
+        seen: set = set()
+        checked = []
+        for members, shared in groups:
+            members, shared = [int(b) for b in members], int(shared)
+            if not members or any(not 0 <= b < batch for b in members) or len(set(members)) < len(members) or seen & set(members):
+                raise KernelError(f"prefix_plan: a group's members are sequences 0..{batch - 1}, each in one group at most, not {members[:8]}")
+            if shared < PAGE or shared % PAGE:
+                raise KernelError(f"prefix_plan: sequences share whole pages of {PAGE} positions, not {shared}")
+            seen.update(members)
+            checked.append((members, shared // PAGE))
+        most = max((len(m) * group for m, _ in checked), default=1)
+        self.rows = min(most, span_rows(dtype, head_dim))         # rows of an item
+        tiles = [-(-len(m) * group // self.rows) for m, _ in checked]
+        # blocks walk equal stretches of pages, short enough to fill the machine a few times over
+        total = sum(t * p for t, (_, p) in zip(tiles, checked)) * num_kv_heads
+        stretch = max(2, -(-total // (PREFIX_BLOCKS_PER_SM * sms)))
+        order, items, shared_of = [], [], [[0, 0] for _ in range(batch)]
+        slots = 0
+        for (members, pages), n_tiles in zip(checked, tiles):
+            n = -(-pages // stretch)
+            per = -(-pages // n)
+            n = -(-pages // per)
+            slots = max(slots, n)
+            for tile in range(n_tiles):
+                first = tile * self.rows
+                rows = min(self.rows, len(members) * group - first)
+                items += [[len(order), first, rows, i * per, min(pages, (i + 1) * per), i] for i in range(n)]
+            for b in members:
+                shared_of[b] = [pages, n]
+            order += members
+        self.max_shared = max((p for _, p in checked), default=0)
+        own_pages = -(-own // PAGE)
+        self.chunks = span_chunks(dtype, head_dim, group)
+        self.splits = span_splits(batch, num_kv_heads * self.chunks, own_pages, sms)
+        self.slots, self.n_items = slots + self.splits, len(items)
+        flat = [v for it in items for v in it]
+        self.items_at, self.shared_at = len(order), len(order) + len(flat)
+        self.ints = np.array(order + flat + [v for s in shared_of for v in s], dtype=np.int32)
+
+
+PREFIX_BLOCKS_PER_SM = 4
+
+
+def _check_span_heads(what: str, dtype, head_dim: int) -> None:
+    if dtype == torch.bfloat16:
+        if head_dim % 16 or not 16 <= head_dim <= 256:
+            raise KernelError(f"{what}: bfloat16 heads of 16..256 in steps of 16, not {head_dim}")
+    elif dtype == torch.float32:
+        if not 1 <= head_dim <= 256:
+            raise KernelError(f"{what}: heads of 1..256, not {head_dim}")
+    else:
+        raise KernelError(f"{what}: element type {dtype} is not supported (float32 and bfloat16 are)")
+
+
+def span_rows(dtype, head_dim: int) -> int:
+    """Rows of queries one block takes over a span of the cache at most."""
+    return 8 if dtype == torch.float32 else 32 if head_dim <= 128 else 16
+
+
+def span_chunks(dtype, head_dim: int, group: int) -> int:
+    """Blocks that share a key/value head's ``group`` query heads over a span."""
+    n = -(-group // span_rows(dtype, head_dim))
+    return -(-group // -(-group // n))
+
+
+def span_splits(batch: int, heads: int, pages: int, sms: int) -> int:
+    """Spans a sequence's own pages are cut into: enough blocks for two on every SM, at most eight pages a block."""
+    return max(1, min(pages, max(-(-2 * sms // max(1, batch * heads)), -(-pages // 8))))
+
+
+def prefix_plan(groups, batch: int, num_heads: int, num_kv_heads: int, head_dim: int, dtype, own: int, device) -> PrefixPlan:
+    """The plan for ``attention_prefix``.  ``groups``: (sequences, shared positions) pairs; the first ``shared positions`` (whole
+    pages) of these sequences of the batch lie on the same pages.  A sequence of no group shares nothing.  ``own``: about the
+    most positions a sequence will have behind its shared ones (its page count decides how the work is cut, never what comes out)."""
+    device = torch.device(device)
+    layout = PrefixLayout(groups, batch, num_heads, num_kv_heads, head_dim, dtype, own, sm_count(device))
+    return PrefixPlan(layout, torch.from_numpy(layout.ints).to(device))
+
+
+class _SpanArgs(Structure):
+    _fields_ = [(n, c_void_p) for n in ("q", "out", "k_cache", "v_cache", "seq_row", "seq_qlen", "seq_ctx", "pages", "order", "items",
+                                        "seq_shared", "part_o", "part_ml", "scores", "weights")] + \
+               [(n, c_int) for n in ("B", "nH", "nKV", "max_pages", "n_pages", "n_items", "splits", "slots", "chunks", "reach")]
+
+
+class _SpanF32Args(Structure):
+    _fields_ = _SpanArgs._fields_ + [("hd", c_int), ("last", c_int)]
+
+
+class _RunArgs(Structure):
+    _fields_ = [(n, c_void_p) for n in ("q", "k_cache", "seq_row", "seq_qlen", "seq_ctx", "pages", "ml", "weights")] + \
+               [(n, c_int) for n in ("B", "nH", "nKV", "max_pages", "n_pages", "reach", "last")]
+
+
+def _one_device(what: str, *tensors) -> None:
+    """The tensors of a call lie on the device that is current: the launch goes to its stream."""
+    here = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.device.index != here:
+            raise KernelError(f"{what}: a tensor on {t.device} beside cuda:{here}, the device that is current")
+
+
+def _need_span(what: str, q, out, k_cache, v_cache, seq_ctx, pages, num_heads, num_kv_heads, head_dim) -> int:
+    _check_span_heads(what, q.dtype if isinstance(q, torch.Tensor) else None, head_dim)
+    if num_heads < 1 or num_kv_heads < 1 or num_heads % num_kv_heads:
+        raise KernelError(f"{what}: {num_heads} heads are not a multiple of {num_kv_heads} key/value heads")
+    _need(q, "q")
+    if q.dim() != 2 or q.shape[1] != num_heads * head_dim:
+        raise KernelError(f"{what}: q must be [tokens, {num_heads * head_dim}], is {tuple(q.shape)}")
+    _need(out, "out", q.dtype, q.shape)
+    _need(k_cache, "k_cache", q.dtype)
+    _need(v_cache, "v_cache", q.dtype, k_cache.shape)
+    if k_cache.dim() != 4 or tuple(k_cache.shape[1:]) != (num_kv_heads, PAGE, head_dim):
+        raise KernelError(f"cache pages must be [*, {num_kv_heads}, {PAGE}, {head_dim}], are {tuple(k_cache.shape)}")
+    _need(seq_ctx, "seq_ctx", torch.int32)
+    _need(pages, "pages", torch.int32)
+    B = seq_ctx.numel()
+    if seq_ctx.dim() != 1 or pages.dim() != 2 or pages.shape[0] != B:
+        raise KernelError(f"{what}: pages {tuple(pages.shape)} do not go with {B} sequences")
+    if B > 65535:
+        raise KernelError(f"{what}: {B} sequences are more than a launch takes (65535)")
+    _one_device(what, q, out, k_cache, v_cache, seq_ctx, pages)
+    return B
+
+
+def attention_prefix(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, seq_ctx: torch.Tensor,
+                     pages: torch.Tensor, plan: PrefixPlan, num_heads: int, num_kv_heads: int, head_dim: int) -> None:
+    """Attention of one token a sequence (row b of ``q``, scaled, is sequence b) over the paged cache, the keys and values on
+    shared pages read once for all sequences that ``plan`` says share them:
+    out[b, h] = sum_j softmax_j(q[b, h] . k[j]) v[j], j = 0..seq_ctx[b].  What ``plan`` says is what ``pages`` holds: a group's
+    members have the same ids in their first columns.  ``seq_ctx``, positions cached before this step, is read on the device:
+    one call captured in a graph serves later steps.  bfloat16 (heads of 16..256 in steps of 16) or float32 (heads up to 256)."""
+    B = _need_span("attention_prefix", q, out, k_cache, v_cache, seq_ctx, pages, num_heads, num_kv_heads, head_dim)
+    lay = plan.layout
+    if (lay.batch, lay.num_heads, lay.num_kv_heads, lay.head_dim, lay.dtype) != (B, num_heads, num_kv_heads, head_dim, q.dtype) or q.shape[0] != B:
+        raise KernelError(f"attention_prefix: a plan for {lay.batch} sequences, {lay.num_heads}/{lay.num_kv_heads} heads of {lay.head_dim} ({lay.dtype}) "
+                          f"does not go with {B} sequences, {q.shape[0]} rows, {num_heads}/{num_kv_heads} heads of {head_dim} ({q.dtype})")
+    if pages.shape[1] < lay.max_shared:
+        raise KernelError(f"attention_prefix: {lay.max_shared} shared pages in a table of {pages.shape[1]}")
+    _need(plan.ints, "plan", torch.int32)
+    _one_device("attention_prefix", plan.ints)
+    n = B * num_heads * lay.slots
+    part = empty((n * (head_dim + 2),), torch.float32, q.device)
+    base, at = plan.ints.data_ptr(), part.data_ptr()
+    fields = (q.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), None, None, seq_ctx.data_ptr(), pages.data_ptr(),
+              base, base + 4 * lay.items_at, base + 4 * lay.shared_at, at, at + 4 * n * head_dim, None, None,
+              B, num_heads, num_kv_heads, pages.shape[1], k_cache.shape[0], lay.n_items, lay.splits, lay.slots, lay.chunks, 0)
+    launches = 3 if lay.n_items else 2
+    if q.dtype == torch.float32:
+        a = _SpanF32Args(*fields, head_dim, 0)
+        _check(_launch(_lib("attention_spans_f32.cu").gl_attention_prefix_f32, byref(a), c_int(lay.rows), _stream()), "attention_prefix", launches)
+    else:
+        a = _SpanArgs(*fields)
+        fn = _lib("attention_spans.cu", catalog.head_dim_defines(head_dim)).gl_attention_prefix
+        _check(_launch(fn, byref(a), c_int(lay.rows), _stream()), "attention_prefix", launches)
+
+
+def attention_weighed(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, weights: torch.Tensor,
+                      seq_qstart: torch.Tensor, seq_qlen: torch.Tensor, seq_ctx: torch.Tensor, pages: torch.Tensor, num_heads: int,
+                      num_kv_heads: int, head_dim: int, max_qlen: int, max_len: int, last: int = 0) -> None:
+    """Causal attention of this step's runs of tokens over the cache (their own keys included), keeping the weight that every
+    cached position has been given.  ``weights`` [pages, key/value heads, PAGE] float32 lies beside the cache under the same page
+    ids; with p the softmax weights of query i and head h,
+    weights[j] <- (weights[j] if j < seq_ctx[b] else 0) + sum of p[i, h, j] over the run's queries i and the query heads h
+    of the key/value head: a position that is new in this step starts from nothing.  ``last`` n > 0: only a run's last n
+    queries are counted.  Places behind a sequence's last position stay as they are, a sequence without tokens leaves everything
+    as it is.  ``max_qlen``, ``max_len``: the longest run, and the longest sequence after the step."""
+    B = _need_span("attention_weighed", q, out, k_cache, v_cache, seq_ctx, pages, num_heads, num_kv_heads, head_dim)
+    _need(weights, "weights", torch.float32, k_cache.shape[:3])
+    _need(seq_qstart, "seq_qstart", torch.int32, (B,))
+    _need(seq_qlen, "seq_qlen", torch.int32, (B,))
+    _one_device("attention_weighed", weights, seq_qstart, seq_qlen)
+    if last < 0 or max_qlen < 0 or max_len < max_qlen or max_len > pages.shape[1] * PAGE:
+        raise KernelError(f"attention_weighed: runs of up to {max_qlen} tokens, sequences of up to {max_len} positions in tables of "
+                          f"{pages.shape[1]} pages, the last {last} queries counted")
+    if B == 0 or max_qlen == 0:
+        return
+    group, n_pages = num_heads // num_kv_heads, k_cache.shape[0]
+    f32 = q.dtype == torch.float32
+    lib = _lib("attention_spans_f32.cu") if f32 else _lib("attention_spans.cu", catalog.head_dim_defines(head_dim))
+    if max_qlen == 1:
+        chunks = span_chunks(q.dtype, head_dim, group)
+        splits = span_splits(B, num_kv_heads * chunks, -(-max_len // PAGE), sm_count(q.device))
+        n = B * num_heads * splits
+        part = empty((n * (head_dim + 2) + B * num_heads * max_len,), torch.float32, q.device)
+        at = part.data_ptr()
+        fields = (q.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), seq_qstart.data_ptr(), seq_qlen.data_ptr(),
+                  seq_ctx.data_ptr(), pages.data_ptr(), None, None, None, at, at + 4 * n * head_dim, at + 4 * n * (head_dim + 2),
+                  weights.data_ptr(), B, num_heads, num_kv_heads, pages.shape[1], n_pages, 0, splits, splits, chunks, max_len)
+        if f32:
+            a = _SpanF32Args(*fields, head_dim, 0)
+            _check(_launch(lib.gl_attention_weighed_f32, byref(a), _stream()), "attention_weighed", 3)
+        else:
+            a = _SpanArgs(*fields)
+            _check(_launch(lib.gl_attention_weighed, byref(a), _stream()), "attention_weighed", 3)
+        return
+    ml = empty((q.shape[0], num_heads, 2), torch.float32, q.device)
+    if f32:
+        a = _SpanF32Args(q.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), seq_qstart.data_ptr(), seq_qlen.data_ptr(),
+                         seq_ctx.data_ptr(), pages.data_ptr(), None, None, None, None, ml.data_ptr(), None, weights.data_ptr(),
+                         B, num_heads, num_kv_heads, pages.shape[1], n_pages, 0, 1, 1, 1, max_len, head_dim, last)
+        _check(_launch(lib.gl_attention_weighed_runs_f32, byref(a), c_int(max_qlen), _stream()), "attention_weighed", 2)
+        return
+    run = attention_prefill_tc if USE_TCGEN05 and head_dim <= TC_ATTENTION_MAX_HEAD_DIM else attention_prefill
+    run(q, out, k_cache, v_cache, seq_qstart, seq_qlen, seq_ctx, pages, num_heads, num_kv_heads, head_dim, max_qlen)
+    a = _RunArgs(q.data_ptr(), k_cache.data_ptr(), seq_qstart.data_ptr(), seq_qlen.data_ptr(), seq_ctx.data_ptr(), pages.data_ptr(),
+                 ml.data_ptr(), weights.data_ptr(), B, num_heads, num_kv_heads, pages.shape[1], n_pages, max_len, last)
+    _check(_launch(lib.gl_attention_weigh_runs, byref(a), c_int(max_qlen), _stream()), "attention_weighed", 2)
+
+
+class _EvictArgs(Structure):
+    _fields_ = [(n, c_void_p) for n in ("k_cache", "v_cache", "weights", "seq_len", "pages", "to", "kept")] + \
+               [(n, c_int) for n in ("layers", "B", "nKV", "n_pages", "max_pages", "to_pages", "keep", "recent", "first", "k_bytes", "v_bytes")]
+
+
+def cache_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, weights: torch.Tensor, seq_len: torch.Tensor, pages: torch.Tensor, keep: int,
+                recent: int = 0, first: int = 0, to_pages: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Cuts sequences longer than ``keep`` positions down to that many, layer by layer and key/value head by head: the ``first``
+    and the ``recent`` last positions stay and, of those between, the ones with the largest ``weights`` (equal ones: the lower
+    position; a NaN counts as less than any number).  What stays moves, in order, to positions 0..keep - 1 of the
+    sequence's own pages, or with ``to_pages`` [B, n] of those (none of which any of ``pages`` may be; the sequence's own
+    pages then stay as they are, and a sequence of up to ``keep`` positions is copied whole).  Keys, values
+    [(layers,) pages, key/value heads, PAGE, head size] and weights [(layers,) pages, key/value heads, PAGE] move together;
+    places behind the ones that are kept stay as they are.  ``seq_len`` [B]: positions cached.  In place no two sequences may share a page.
+    Returns the positions kept, int32 [(layers,) B, key/value heads, keep], behind a shorter sequence's -1."""
+    _need(k_cache, "k_cache")
+    _need(v_cache, "v_cache", k_cache.dtype)
+    dtype_code(k_cache.dtype)
+    if k_cache.dim() not in (4, 5) or k_cache.shape[-2] != PAGE or v_cache.shape[:-1] != k_cache.shape[:-1]:
+        raise KernelError(f"cache_evict: keys {tuple(k_cache.shape)} and values {tuple(v_cache.shape)} are not [(layers,) pages, heads, {PAGE}, size]")
+    _need(weights, "weights", torch.float32, k_cache.shape[:-1])
+    _need(seq_len, "seq_len", torch.int32)
+    _need(pages, "pages", torch.int32)
+    B = seq_len.numel()
+    if seq_len.dim() != 1 or pages.dim() != 2 or pages.shape[0] != B:
+        raise KernelError(f"cache_evict: pages {tuple(pages.shape)} do not go with {B} sequences")
+    if keep < 1 or first < 0 or recent < 0 or first + recent > keep:
+        raise KernelError(f"cache_evict: the first {first} and the last {recent} positions do not go into {keep}")
+    _one_device("cache_evict", k_cache, v_cache, weights, seq_len, pages, to_pages)
+    if to_pages is not None:
+        _need(to_pages, "to_pages", torch.int32)
+        if to_pages.dim() != 2 or to_pages.shape[0] != B or to_pages.shape[1] * PAGE < min(keep, pages.shape[1] * PAGE):
+            raise KernelError(f"cache_evict: pages {tuple(to_pages.shape)} do not hold {keep} positions of {B} sequences")
+        if to_pages.data_ptr() == pages.data_ptr():
+            raise KernelError("cache_evict: to_pages is the table of the sequences' own pages; leave it out to work in place")
+    layers = k_cache.shape[0] if k_cache.dim() == 5 else 1
+    n_pages, heads = k_cache.shape[-4], k_cache.shape[-3]
+    es = k_cache.element_size()
+    if max(k_cache.shape[-1], v_cache.shape[-1]) * es > 4096 or min(k_cache.shape[-1], v_cache.shape[-1]) < 1:
+        raise KernelError(f"cache_evict: heads of {k_cache.shape[-1]} and {v_cache.shape[-1]} are outside 1..{4096 // es}")
+    if heads > 65535 or B * layers > 65535:
+        raise KernelError(f"cache_evict: {layers} layers of {B} sequences, {heads} heads are more than a launch takes")
+    kept = empty((*k_cache.shape[:-4], B, heads, keep), torch.int32, k_cache.device)
+    to = pages if to_pages is None else to_pages
+    if B == 0 or layers == 0 or n_pages == 0 or pages.shape[1] == 0:
+        return kept.fill_(-1)
+    a = _EvictArgs(k_cache.data_ptr(), v_cache.data_ptr(), weights.data_ptr(), seq_len.data_ptr(), pages.data_ptr(), to.data_ptr(), kept.data_ptr(),
+                   layers, B, heads, n_pages, pages.shape[1], to.shape[1], keep, recent, first, k_cache.shape[-1] * es, v_cache.shape[-1] * es)
+    _check(_launch(_lib("cache_evict.cu").gl_cache_evict, byref(a), c_int(sm_count(k_cache.device)), _stream()), "cache_evict", 2)
+    return kept
 
 
 class _DecodeLayerArgs(Structure):
