@@ -15,6 +15,7 @@ from typing import Callable, List, Optional, Sequence
 
 import torch
 
+from . import ops
 from .cache.sequence_cache import SequenceCache
 from .config import load_config, read_config_json
 from .config.registry import Architecture
@@ -72,6 +73,15 @@ class Model:
     def close_sequence(self, slot: int) -> None:
         self.engine.close(slot)
 
+    def fork_sequence(self, slot: int, positions: Optional[int] = None) -> int:
+        """A new sequence that begins as the first ``positions`` (default: all) of an open one.  Their whole pages are shared, held
+        once and, in steps of one token a sequence, read once for all sequences of the batch that share them."""
+        return self.engine.fork(slot, positions)
+
+    def evict(self, slots, keep: int, recent: int = 0, first: int = 0) -> None:
+        """See Engine.evict (a model loaded with ``weigh=True``)."""
+        self.engine.evict(slots, keep, recent, first)
+
     def step(self, runs, want=None) -> torch.Tensor:
         """See Engine.step."""
         return self.engine.step(runs, want)
@@ -81,7 +91,10 @@ class Model:
         lists).  Options: max_tokens, temperature, top_p, top_k, min_p,
         repeat_penalty, seed, stop_tokens, should_stop, on_token (called with
         (request index, token) for every token as it is emitted; returning
-        False cancels).  Returns a GenerationResult, or a list of them."""
+        False cancels); share_prefix: prompts of a batch that begin alike are run once
+        as far as they do, and their sequences share those pages; cache_keep, cache_recent, cache_first: a
+        sequence that has come to hold a page more than cache_keep positions is cut down to them
+        (see Engine.evict; needs ``weigh=True`` when loading).  Returns a GenerationResult, or a list of them."""
         from .engine.generate import GenerationOptions, generate
         single = len(prompts) > 0 and not isinstance(prompts[0], (list, tuple))
         opts = options.pop("options", None) or GenerationOptions.from_kwargs(self.spec, **options)
@@ -110,13 +123,25 @@ def _cache_sizes(spec, max_tokens: Optional[int]):
     return max_tokens, min(spec.max_positions, pages * 64)
 
 
+def _build_cache(model: DecoderModel, max_tokens: int, positions: int, cdt, device, max_slots, weigh: bool) -> SequenceCache:
+    if weigh:
+        for e in model.spec.schedule:
+            if not getattr(getattr(model.blocks[e.layer], "mixer", None), "forgets", False) or e.cache is None or not e.writes:
+                raise ValueError(f"layer {e.layer}: weigh=True is for models whose layers all keep whole-sequence attention's keys and values "
+                                 f"in cache entries of their own")
+            if not ops.span_heads_fit(cdt, model.blocks[e.layer].mixer.spec.head_dim):
+                raise ValueError(f"layer {e.layer}: weigh=True takes heads of 16 to 256 in steps of 16 in bfloat16, of up to 256 in 32 bits")
+    return SequenceCache(model.cache_requests(), max_tokens, positions, cdt, device, max_slots=max_slots, weigh=weigh,
+                         last_position=model.spec.max_positions if weigh else None)
+
+
 def build_model(arch: Architecture, config) -> DecoderModel:
     return DecoderModel(arch.build_spec(config))
 
 
 def load(path: str, dtype="bfloat16", max_tokens: Optional[int] = None, device="cuda:0",
          max_slots: Optional[int] = None, log: Optional[Callable[[str], None]] = None,
-         keep_stored: Optional[bool] = None) -> Model:
+         keep_stored: Optional[bool] = None, weigh: bool = False) -> Model:
     """Open a model folder (config.json + model.safetensors).
 
     dtype: "bfloat16" (the serving kernels) or "float32" (everything in true
@@ -129,6 +154,9 @@ def load(path: str, dtype="bfloat16", max_tokens: Optional[int] = None, device="
     inside a 16-bit checkpoint stays 32-bit.  keep_stored=True keeps every matrix
     that is not stored as bfloat16 in 32-bit (exact, and slow: such products run on
     CUDA cores); keep_stored=False rounds every matrix.
+    weigh: the cache keeps, beside every position's keys and values, the attention weight it has been
+    given (4 bytes a layer and key/value head), so that sequences can be cut down to what weighs most
+    (``Model.evict``, ``generate(cache_keep=...)``); for models that are whole-sequence attention throughout.
     """
     device = _require_cuda(device)
     cdt = compute_dtype(dtype)
@@ -147,8 +175,7 @@ def load(path: str, dtype="bfloat16", max_tokens: Optional[int] = None, device="
         model.load(tensors)
         del tensors
         max_tokens, positions = _cache_sizes(model.spec, max_tokens)
-        cache = SequenceCache(model.cache_requests(), max_tokens, positions,
-                              cdt, device, max_slots=max_slots)
+        cache = _build_cache(model, max_tokens, positions, cdt, device, max_slots, weigh)
         engine = Engine(model, cache, cdt, device)
     info = LoadInfo(path=os.path.abspath(path), architecture=arch.name,
                     dtype="bfloat16" if cdt == torch.bfloat16 else "float32",
@@ -165,7 +192,7 @@ def _draw_workers() -> int:
 
 
 def load_random(config, seed: int = 0, dtype="bfloat16", max_tokens: Optional[int] = None,
-                device="cuda:0", max_slots: Optional[int] = None, layers: Optional[int] = None) -> Model:
+                device="cuda:0", max_slots: Optional[int] = None, layers: Optional[int] = None, weigh: bool = False) -> Model:
     """A model with seeded random weights built in memory: tensor for tensor what
     ``write_random_model(folder, config, seed)`` writes and ``load(folder, dtype)`` then holds (the
     tensors are drawn on the CPU from the same per-tensor generators, several at a time, and rounded
@@ -194,8 +221,7 @@ def load_random(config, seed: int = 0, dtype="bfloat16", max_tokens: Optional[in
         model.load(tensors)
         del tensors
         max_tokens, positions = _cache_sizes(model.spec, max_tokens)
-        cache = SequenceCache(model.cache_requests(), max_tokens, positions,
-                              cdt, device, max_slots=max_slots)
+        cache = _build_cache(model, max_tokens, positions, cdt, device, max_slots, weigh)
         engine = Engine(model, cache, cdt, device)
     info = LoadInfo(path=f"random:{seed}", architecture=arch.name,
                     dtype="bfloat16" if cdt == torch.bfloat16 else "float32",

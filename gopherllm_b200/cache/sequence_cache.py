@@ -42,6 +42,7 @@ class KVView:
     k: torch.Tensor
     v: torch.Tensor
     writes: bool = True
+    weights: Optional[torch.Tensor] = None      # [pages, kv_heads, PAGE] float32: what attention gave each position, if the cache keeps it
 
 
 @dataclass
@@ -59,6 +60,8 @@ class _Group:
         self.pool = IdPool(n_pages, f"page of cache group {gid}")
         self.keys: Optional[torch.Tensor] = None        # [entries, pages, kv_heads, PAGE, head_dim]
         self.values: Optional[torch.Tensor] = None      # [entries, pages, kv_heads, PAGE, value_dim]
+        self.weights: Optional[torch.Tensor] = None     # [entries, pages, kv_heads, PAGE] float32
+        self.more: Dict[int, int] = {}                  # page -> sequences that hold it besides the first
 
 
 class SequenceCache:
@@ -66,13 +69,21 @@ class SequenceCache:
     mixer made of several (its view is then the tuple of their views).
 
     max_tokens: positions all live sequences may hold together, each sequence
-    rounded up to a whole page.  max_positions: the longest a sequence may get.
+    rounded up to a whole page.  max_positions: the most positions of a sequence the cache holds.
+
+    Sequences may share pages (``fork``): a shared page is full and is never written again.  With ``weigh`` every page has,
+    beside its keys and values, the softmax weight its positions have been given so far; a sequence can then be cut down to
+    the positions that weigh most (``shrink`` records it).  Its next token's position stays what it was, so
+    a sequence that has been cut may come to lie at positions up to ``last_position`` (default: max_positions).
     """
 
     def __init__(self, requests: Sequence, max_tokens: int, max_positions: int,
-                 dtype: torch.dtype, device, max_slots: Optional[int] = None, allocate: bool = True):
+                 dtype: torch.dtype, device, max_slots: Optional[int] = None, allocate: bool = True,
+                 weigh: bool = False, last_position: Optional[int] = None):
         self.dtype, self.device = dtype, device
         self.max_positions = int(max_positions)
+        self.last_position = max(self.max_positions, int(last_position or 0))
+        self.weigh = bool(weigh)
         self.n_pages = max(1, -(-int(max_tokens) // PAGE))
         self.max_pages_per_seq = max(1, -(-self.max_positions // PAGE))
         self.max_slots = int(max_slots) if max_slots else min(self.n_pages, 1024)
@@ -117,15 +128,18 @@ class SequenceCache:
                 if not r.values_in_keys:
                     g.values = torch.empty((len(g.entries), self.n_pages, r.value_heads or r.num_kv_heads, PAGE,
                                             r.value_dim or r.head_dim), dtype=dtype, device=device)
+                if self.weigh:
+                    g.weights = torch.empty((len(g.entries), self.n_pages, r.num_kv_heads, PAGE), dtype=torch.float32, device=device)
         # per-slot bookkeeping
         self._length = [0] * self.max_slots
+        self._forgotten = [0] * self.max_slots                 # positions a sequence has lost to ``shrink``
         self._pages: List[List[List[int]]] = [[[] for _ in self.groups] for _ in range(self.max_slots)]
         # per slot and group: pages before this index have been released (groups with a window or chunks only)
         self._first_page: List[List[int]] = [[0 for _ in self.groups] for _ in range(self.max_slots)]
 
     # -- sizes ------------------------------------------------------------
     def bytes(self) -> int:
-        n = sum(t.numel() * t.element_size() for g in self.groups for t in (g.keys, g.values) if t is not None)
+        n = sum(t.numel() * t.element_size() for g in self.groups for t in (g.keys, g.values, g.weights) if t is not None)
         return n + sum(s.numel() * 4 for s in self._states if s is not None)
 
     def bytes_per_position(self) -> int:
@@ -146,14 +160,15 @@ class SequenceCache:
         if kind == "kv":
             g = self.groups[a]
             # (a group whose values lie in its key rows hands out the keys twice)
-            return KVView(group=a, k=g.keys[b], v=g.values[b] if g.values is not None else g.keys[b], writes=writes)
+            return KVView(group=a, k=g.keys[b], v=g.values[b] if g.values is not None else g.keys[b], writes=writes,
+                          weights=g.weights[b] if g.weights is not None else None)
         return StateView(rows=self._states[a], writes=writes)
 
     # -- sequences --------------------------------------------------------
     def open(self) -> int:
         """Take a slot for a new sequence of length 0; its state rows are zeroed."""
         slot = self.slots.take()
-        self._length[slot] = 0
+        self._length[slot] = self._forgotten[slot] = 0
         for s in self._states:
             if s is not None:
                 s[slot].zero_()
@@ -181,6 +196,11 @@ class SequenceCache:
         self._held(slot)
         return self._length[slot]
 
+    def position(self, slot: int) -> int:
+        """The position of the sequence's next token: the positions it holds and those it has lost."""
+        self._held(slot)
+        return self._length[slot] + self._forgotten[slot]
+
     def _held(self, slot: int) -> None:
         if not self.slots.is_held(slot):
             raise ValueError(f"slot {slot} is not in use")
@@ -198,6 +218,8 @@ class SequenceCache:
             if new_len > self.max_positions:
                 raise CacheFull(f"sequence in slot {slot} would reach {new_len} positions, "
                                 f"the cache holds {self.max_positions} per sequence")
+            if new_len + self._forgotten[slot] > self.last_position:
+                raise CacheFull(f"sequence in slot {slot} would reach position {new_len + self._forgotten[slot]}, the model has {self.last_position}")
             if new_len < self._length[slot]:
                 raise ValueError(f"slot {slot}: cannot shrink from {self._length[slot]} to {new_len}")
             need += self.pages_needed(slot, new_len)
@@ -227,7 +249,7 @@ class SequenceCache:
                 first_seen = new_len - new_len % chunk if chunk > 0 else max(0, new_len - w + 1)
                 keep_from = min(first_seen // PAGE, len(pg))
                 for i in range(self._first_page[slot][g.gid], keep_from):
-                    g.pool.give(pg[i])
+                    self._give(g, pg[i])
                     pg[i] = RELEASED
                 if keep_from > self._first_page[slot][g.gid]:
                     self._first_page[slot][g.gid] = keep_from
@@ -238,11 +260,114 @@ class SequenceCache:
         for g in self.groups:
             for p in self._pages[slot][g.gid]:
                 if p != RELEASED:
-                    g.pool.give(p)
+                    self._give(g, p)
             self._pages[slot][g.gid] = []
             self._first_page[slot][g.gid] = 0
-        self._length[slot] = 0
+        self._length[slot] = self._forgotten[slot] = 0
         self.slots.give(slot)
+
+    @staticmethod
+    def _give(g: _Group, page: int) -> None:
+        """One sequence less holds the page; the last one gives it back."""
+        n = g.more.get(page, 0)
+        if n > 1:
+            g.more[page] = n - 1
+        elif n == 1:
+            del g.more[page]
+        else:
+            g.pool.give(page)
+
+    # -- sequences that share pages ------------------------------------------
+    def fork(self, slot: int, positions: Optional[int] = None) -> int:
+        """A new sequence that begins as the first ``positions`` (default: all) of the one in ``slot``.  Their whole pages are
+        shared, a page that is begun is copied; both sequences go on independently.  With state, a window or chunks only the
+        whole sequence can be continued: what it was before is no longer held."""
+        self._held(slot)
+        n = self._length[slot] if positions is None else int(positions)
+        if not 0 <= n <= self._length[slot]:
+            raise ValueError(f"slot {slot}: {n} of {self._length[slot]} positions cannot be continued")
+        if n < self._length[slot] and (self._forgotten[slot] or any(s is not None for s in self._states)
+                                       or any(g.req.window > 0 or g.req.chunk > 0 for g in self.groups)):
+            raise ValueError(f"slot {slot}: what the sequence was at {n} of its {self._length[slot]} positions is no longer held")
+        whole, begun = n // PAGE, 1 if n % PAGE else 0
+        for g in self.groups:
+            if begun > g.pool.free_count:
+                raise CacheFull(f"one more page of {PAGE} positions wanted, none of {g.pool.n} free in cache group {g.gid}")
+        new = self.slots.take()
+        for s in self._states:
+            if s is not None:
+                s[new].copy_(s[slot])
+        for g in self.groups:
+            old = self._pages[slot][g.gid]
+            pages = old[:whole]
+            for p in pages:
+                if p != RELEASED:
+                    g.more[p] = g.more.get(p, 0) + 1
+            if begun:
+                pages.append(g.pool.take())
+                for t in (g.keys, g.values, g.weights):
+                    if t is not None:
+                        t[:, pages[-1]].copy_(t[:, old[whole]])
+            self._pages[new][g.gid] = pages
+            self._first_page[new][g.gid] = self._first_page[slot][g.gid]
+        self._length[new], self._forgotten[new] = n, self._forgotten[slot]
+        return new
+
+    def shares_pages(self, slot: int) -> bool:
+        return any(p in g.more for g in self.groups for p in self._pages[slot][g.gid])
+
+    def shared_prefixes(self, slots: Sequence[int]) -> List[Tuple[List[int], int]]:
+        """(members, positions) for the sequences among ``slots`` that begin on the same pages: indices into ``slots``, and how many
+        positions lie on pages that all of them have in common.  A page is the same in every group of entries or in none (a
+        group with a window may have given it back)."""
+        g = next((g for g in self.groups if g.req.window <= 0 and g.req.chunk <= 0), None)
+        if g is None or not g.more:
+            return []
+        by_first: Dict[int, List[int]] = {}
+        for i, slot in enumerate(slots):
+            pg = self._pages[slot][g.gid]
+            if pg and pg[0] in g.more:
+                by_first.setdefault(pg[0], []).append(i)
+        out = []
+        for members in by_first.values():
+            if len(members) < 2:
+                continue
+            lists = [self._pages[slots[i]][g.gid] for i in members]
+            n, least = 1, min(self._length[slots[i]] // PAGE for i in members)
+            while n < least and lists[0][n] in g.more:
+                n += 1
+            for pg in lists[1:]:
+                while pg[:n] != lists[0][:n]:                  # (the common head: at least the first page)
+                    n = next(j for j in range(n) if pg[j] != lists[0][j])
+            out.append((members, n * PAGE))
+        return out
+
+    # -- sequences that are cut down ---------------------------------------------
+    def fresh_pages(self, wants: Sequence[Tuple[int, int]]) -> Dict[int, List[List[int]]]:
+        """Pages outside every sequence for what will be kept of these: wants = [(slot, positions)]; slot -> pages by group.
+        All or none."""
+        need = sum(-(-n // PAGE) for _, n in wants)
+        for g in self.groups:
+            if need > g.pool.free_count:
+                raise CacheFull(f"{need} more pages of {PAGE} positions wanted, {g.pool.free_count} of {g.pool.n} free in cache group {g.gid}")
+        return {slot: [g.pool.take_many(-(-n // PAGE)) for g in self.groups] for slot, n in wants}
+
+    def shrink(self, slot: int, keep: int, onto: Optional[List[List[int]]] = None) -> None:
+        """Record that of the sequence ``keep`` positions stay, now at the head of its pages, or on the pages ``onto``."""
+        self._held(slot)
+        if not 0 < keep <= self._length[slot]:
+            raise ValueError(f"slot {slot}: {keep} of {self._length[slot]} positions cannot stay")
+        if onto is None and self.shares_pages(slot):
+            raise ValueError(f"slot {slot} shares pages with another sequence: what stays must move to pages of its own")
+        n = -(-keep // PAGE)
+        for g in self.groups:
+            pg = self._pages[slot][g.gid]
+            gone, stay = (pg[n:], pg[:n]) if onto is None else (pg, onto[g.gid])
+            self._pages[slot][g.gid] = list(stay)
+            for p in gone:
+                self._give(g, p)
+        self._forgotten[slot] += self._length[slot] - keep
+        self._length[slot] = keep
 
     def page_rows(self, group: int, slots: Sequence[int], out: Optional[np.ndarray] = None) -> np.ndarray:
         """[len(slots), max_pages_per_seq] int32 page ids (the unused tail and pages released before a
@@ -266,7 +391,7 @@ class SequenceCache:
         """Positions reserved by live sequences, each rounded up to whole pages."""
         if not self.groups:
             return sum(self._length[s] for s in self.live_slots())
-        return sum(len(self._pages[s][0]) for s in self.live_slots()) * PAGE
+        return (sum(len(self._pages[s][0]) for s in self.live_slots()) - sum(self.groups[0].more.values())) * PAGE
 
     def check(self) -> None:
         """Invariants: no page lost, none owned twice, free slots own nothing."""
@@ -274,6 +399,8 @@ class SequenceCache:
         for g in self.groups:
             g.pool.check()
             owned: List[int] = []
+            for p, n in g.more.items():
+                assert n > 0 and g.pool.is_held(p), f"page {p} of group {g.gid} is shared by nobody"
             for s in range(self.max_slots):
                 pg = self._pages[s][g.gid]
                 if not self.slots.is_held(s):
@@ -282,5 +409,8 @@ class SequenceCache:
                 assert all(p == RELEASED for p in pg[:k]) and all(p != RELEASED for p in pg[k:]), \
                     f"slot {s}: released pages of group {g.gid} do not form the head of its list"
                 owned.extend(pg[k:])
-            assert len(owned) == len(set(owned)), f"a page of group {g.gid} is owned twice"
-            assert len(owned) == g.pool.held_count, f"pages of group {g.gid} are lost"
+            times: Dict[int, int] = {}
+            for p in owned:
+                times[p] = times.get(p, 0) + 1
+            assert {p: n - 1 for p, n in times.items() if n > 1} == g.more, f"a page of group {g.gid} is owned twice"
+            assert len(times) == g.pool.held_count, f"pages of group {g.gid} are lost"

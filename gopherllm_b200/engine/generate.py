@@ -29,13 +29,22 @@ class GenerationOptions:
     its context, runtime.go:1131), on_token(request index, token): called for every
     emitted token as it is known; returning False cancels the generation with what
     was generated so far (the reference's streaming callback, runtime.go:793-815,
-    1024, which gets text; this library is token-level)."""
+    1024, which gets text; this library is token-level).
+
+    share_prefix: prompts of a batch that begin alike are run once as far as they do (whole pages), and
+    their sequences share those pages.  cache_keep n > 0: a sequence that has come to hold a page more than n
+    positions is cut down to n, the cache_first first, the cache_recent last and those between that
+    attention has given the most weight (an engine whose cache keeps weights)."""
     max_tokens: int = 256
     sampler: SamplerConfig = field(default_factory=SamplerConfig)
     seed: int = 0
     stop_tokens: Tuple[int, ...] = ()
     should_stop: Optional[Callable[[], bool]] = None
     on_token: Optional[Callable[[int, int], Optional[bool]]] = None
+    share_prefix: bool = False
+    cache_keep: int = 0
+    cache_recent: int = 0
+    cache_first: int = 0
 
     @classmethod
     def from_kwargs(cls, spec=None, **kw) -> "GenerationOptions":
@@ -50,7 +59,8 @@ class GenerationOptions:
             stops = tuple(spec.stop_tokens) if spec is not None else ()
         o = cls(max_tokens=kw.pop("max_tokens", 256), sampler=s, seed=kw.pop("seed", 0),
                 stop_tokens=tuple(int(t) for t in stops), should_stop=kw.pop("should_stop", None),
-                on_token=kw.pop("on_token", None))
+                on_token=kw.pop("on_token", None), share_prefix=bool(kw.pop("share_prefix", False)), cache_keep=kw.pop("cache_keep", 0),
+                cache_recent=kw.pop("cache_recent", 0), cache_first=kw.pop("cache_first", 0))
         if kw:
             raise TypeError(f"unknown generation options: {', '.join(sorted(kw))}")
         return o
@@ -58,6 +68,9 @@ class GenerationOptions:
     def validate(self) -> None:
         if not isinstance(self.max_tokens, int) or self.max_tokens <= 0:
             raise ValueError("max_tokens must be greater than 0")
+        if not isinstance(self.cache_keep, int) or self.cache_keep < 0 or self.cache_recent < 0 or self.cache_first < 0 \
+                or self.cache_recent + self.cache_first > self.cache_keep:
+            raise ValueError(f"the first {self.cache_first} and the last {self.cache_recent} positions do not go into {self.cache_keep}")
         self.sampler.validate()
 
 
@@ -91,13 +104,36 @@ class GenerationCanceled(RuntimeError):
 # ---------------------------------------------------------------------------
 # decisions (no device involved)
 # ---------------------------------------------------------------------------
-def pages_for(prompt_len: int, max_tokens: int, max_positions: int) -> int:
-    """Pages a request can come to hold: its prompt plus every token it may feed."""
-    return -(-min(prompt_len + max_tokens, max_positions) // PAGE)
+def pages_for(prompt_len: int, max_tokens: int, max_positions: int, keep: int = 0, shares: bool = False) -> int:
+    """Pages a request can come to hold: its prompt plus every token it may feed; with ``keep`` its prompt, and later no
+    more than a page beyond that many positions.  What is kept of a sequence that ``shares`` pages moves to others."""
+    most = min(prompt_len + max_tokens, max_positions)
+    if keep > 0:
+        most = min(most, max(prompt_len, keep + PAGE)) + (keep if shares else 0)
+    return -(-most // PAGE) + (1 if keep > 0 and shares else 0)
+
+
+def begin_alike(prompts: Sequence[Sequence[int]]) -> List[Tuple[List[int], int]]:
+    """(members, tokens) for prompts that share their first page of tokens or more: how many whole pages of tokens all members
+    have in common, short of any member's last token (which is run by each, for its logits)."""
+    by_first: dict = {}
+    for i, p in enumerate(prompts):
+        if len(p) > PAGE:
+            by_first.setdefault(tuple(p[:PAGE]), []).append(i)
+    out = []
+    for members in by_first.values():
+        if len(members) < 2:
+            continue
+        least, most = min(prompts[i] for i in members), max(prompts[i] for i in members)      # (all others lie between them)
+        n, end = 0, min(len(prompts[i]) for i in members) - 1
+        while n < end and least[n] == most[n]:
+            n += 1
+        out.append((members, n // PAGE * PAGE))
+    return out
 
 
 def plan_batches(prompt_lens: Sequence[int], max_tokens: int, max_positions: int,
-                 page_budget: int, slot_budget: int) -> List[List[int]]:
+                 page_budget: int, slot_budget: int, keep: int = 0, shares: bool = False) -> List[List[int]]:
     """Cut requests, in order, into batches whose worst-case page need fits the cache."""
     batches: List[List[int]] = []
     cur: List[int] = []
@@ -108,7 +144,7 @@ def plan_batches(prompt_lens: Sequence[int], max_tokens: int, max_positions: int
         if n >= max_positions:
             # the reference rejects len(tokens) >= MaxSeqLen before any forward (runtime.go:866-868)
             raise ValueError(f"request {i}: prompt of {n} tokens does not fit {max_positions} positions")
-        need = pages_for(n, max_tokens, max_positions)
+        need = pages_for(n, max_tokens, max_positions, keep, shares)
         if need > page_budget:
             raise ValueError(f"request {i} needs {need * PAGE} cached positions, the cache holds {page_budget * PAGE}")
         if cur and (used + need > page_budget or len(cur) >= slot_budget):
@@ -159,7 +195,9 @@ def generate(engine, prompts: Sequence[Sequence[int]], options: GenerationOption
     cache = engine.cache
     seed = options.seed if options.seed != 0 else time.time_ns()
     batches = plan_batches([len(p) for p in prompts], options.max_tokens, spec.max_positions,
-                           cache.n_pages, cache.max_slots)
+                           cache.n_pages, cache.max_slots, options.cache_keep, options.share_prefix)
+    if options.cache_keep and not getattr(cache, "weigh", False):
+        raise ValueError("cache_keep needs a cache that keeps the weight of its positions (load the model with weigh=True)")
     results: List[Optional[GenerationResult]] = [None] * len(prompts)
     prepare = getattr(engine, "prepare_decode", None)
     # kernels that gave up a bounded wait leave a status word: read where the host waits anyway, so that
@@ -173,12 +211,25 @@ def generate(engine, prompts: Sequence[Sequence[int]], options: GenerationOption
                   for i in batch]
         sampler = DeviceSampler(options.sampler, [request_seed(seed, i) for i in batch],
                                 [prompts[i] for i in batch], spec.vocab, engine.device)
-        slots = [engine.open() for _ in batch]
+        slots: List[Optional[int]] = [None] * len(batch)
         stats = [GenerationStats(prompt_tokens=len(prompts[i])) for i in batch]
         live = list(range(len(batch)))
         canceled = False
         try:
-            logits = engine.step([(slots[r], states[r].prompt) for r in live])
+            skip = [0] * len(batch)                 # tokens of a prompt that lie on shared pages already
+            if options.share_prefix:
+                for members, n in begin_alike([s.prompt for s in states]):
+                    # the first member runs the common tokens, the others go on from there
+                    slots[members[0]] = engine.open()
+                    engine.step([(slots[members[0]], states[members[0]].prompt[:n])], [[]])
+                    for r in members:
+                        skip[r] = n
+                        if slots[r] is None:
+                            slots[r] = engine.fork(slots[members[0]])
+            for r in live:
+                if slots[r] is None:
+                    slots[r] = engine.open()
+            logits = engine.step([(slots[r], states[r].prompt[skip[r]:]) for r in live])
             rows_dev = None
             first = True
             t_prefill_end = None
@@ -193,6 +244,10 @@ def generate(engine, prompts: Sequence[Sequence[int]], options: GenerationOption
                 # a stop token, the step has merely fed one token too many to a sequence that is closed,
                 # and the rows of the others stand (a row does not depend on its neighbours).
                 ahead, ahead_logits, sampled = None, None, None
+                # (a sequence that has grown a page beyond what it may keep is cut before its next step)
+                due = options.cache_keep and [slots[r] for r in live if cache.length(slots[r]) >= options.cache_keep + PAGE]
+                if due:
+                    engine.evict(due, options.cache_keep, options.cache_recent, options.cache_first)
                 if prepare is not None and all(states[r].may_continue() for r in live):
                     ahead = prepare([slots[r] for r in live])
                     if fetch is not None:

@@ -17,6 +17,7 @@ import numpy as np
 import torch
 
 from ..cache.sequence_cache import PAGE, SequenceCache
+from ..ops import span_heads_fit
 from .model import DecoderModel
 
 
@@ -32,6 +33,9 @@ class StepContext:
     after the step), total_len (positions of all sequences after the step), query_keys
     (pairs of a token of the step and a position it may see), is_decode (every run is one token), act_dtype, device,
     scratch (per-step memo shared by the parts, e.g. position tables).
+    tok_place[T]: where the token's key and value lie among the sequence's cached ones; tok_pos unless the sequence has been cut.
+    prefix: plans for pages that the step's sequences share, by heads (query heads, key/value heads, head size); empty if they
+    share none or too little.
     """
 
     def __init__(self, device, act_dtype):
@@ -44,10 +48,13 @@ class StepContext:
         self.n_tokens = self.n_seqs = self.n_want = 0
         self.max_qlen = self.max_len = self.total_len = self.query_keys = 0
         self.is_decode = False
+        self.tok_place = None
+        self.prefix: Dict[tuple, object] = {}
         self.next_block = None           # the block of the run behind the current one (models of several residual streams)
         self.side_stream = None          # a second stream blocks may fork onto (decode steps only)
 
 
+SHARED_POSITIONS = 1024              # positions that reading shared pages once must spare a step before it is worth its own kernels
 GRAPH_F32_RUN_BYTES = 128 << 20      # weights of a model for each run of its schedule, up to which 32-bit decode steps are captured
 
 
@@ -58,8 +65,9 @@ def _pad4(n: int) -> int:
 class _Layout:
     """Offsets of the step's arrays inside one int32 buffer (each 16-byte aligned)."""
 
-    def __init__(self, T: int, B: int, M: int, groups: int, max_pages: int):
+    def __init__(self, T: int, B: int, M: int, groups: int, max_pages: int, places: bool = False, prefix: Sequence = ()):
         self.T, self.B, self.M, self.groups, self.max_pages = T, B, M, groups, max_pages
+        self.places, self.prefix = places, tuple(prefix)       # a place for every token; plans (ops.PrefixLayout) for shared pages
         o = 0
         self.off: Dict[str, Tuple[int, int]] = {}
         for name, n in (("tokens", T), ("tok_seq", T), ("tok_pos", T), ("seq_slot", B),
@@ -69,10 +77,16 @@ class _Layout:
         for g in range(groups):
             self.off[f"pages{g}"] = (o, B * max_pages)
             o += _pad4(B * max_pages)
+        if places:
+            self.off["tok_place"] = (o, T)
+            o += _pad4(T)
+        for i, plan in enumerate(self.prefix):
+            self.off[f"prefix{i}"] = (o, plan.ints.size)
+            o += _pad4(plan.ints.size)
         self.size = max(o, 4)
 
     def key(self):
-        return (self.T, self.B, self.M, self.groups, self.max_pages)
+        return (self.T, self.B, self.M, self.groups, self.max_pages, *(p.key() for p in self.prefix))
 
 
 class Engine:
@@ -94,6 +108,10 @@ class Engine:
         self._graphs: Dict[tuple, object] = {}             # insertion order = least recently used first
         self.graph_limit = 64                                # captured steps kept (each holds its logits and descriptor)
         self._graph_pool = None
+        # heads of the mixers that read shared pages once for all who share them
+        heads = {b.mixer.shared_heads for b in getattr(model, "blocks", ()) if getattr(getattr(b, "mixer", None), "shared_heads", None)}
+        self.shared_heads = sorted(h for h in heads if span_heads_fit(act_dtype, h[2]))
+        self.share_prefixes = True
         self.overlap_branches = True                         # decode steps run parallel branches on two streams
         self._side_stream = None
         self._copy_stream = None
@@ -111,6 +129,42 @@ class Engine:
 
     def close(self, slot: int) -> None:
         self.cache.close(slot)
+
+    def fork(self, slot: int, positions: Optional[int] = None) -> int:
+        """See SequenceCache.fork."""
+        return self.cache.fork(slot, positions)
+
+    @torch.no_grad()
+    def evict(self, slots: Sequence[int], keep: int, recent: int = 0, first: int = 0) -> None:
+        """Cut these sequences down to ``keep`` positions where they hold more: in every layer and key/value head the ``first``
+        and the ``recent`` last ones stay and, of those between, the ones that attention has given the most weight so far
+        (see ops.cache_evict).  The pages this frees go back to the cache; the next token's position is what it was."""
+        from .. import ops
+        cache = self.cache
+        if not cache.weigh:
+            raise ValueError("this model's cache does not keep the weight of its positions (load it with weigh=True)")
+        slots = [int(s) for s in slots]
+        if len(set(slots)) != len(slots):
+            raise ValueError("a sequence appears twice among those to cut")
+        if keep < 1 or recent < 0 or first < 0 or first + recent > keep:
+            raise ValueError(f"the first {first} and the last {recent} positions do not go into {keep}")
+        long = [s for s in slots if cache.length(s) > keep]
+        shared = [s for s in long if cache.shares_pages(s)]
+        alone = [s for s in long if s not in set(shared)]
+        fresh = cache.fresh_pages([(s, keep) for s in shared])
+        i32 = lambda v: torch.from_numpy(np.ascontiguousarray(v, dtype=np.int32)).to(self.device)  # noqa: E731
+        with torch.cuda.device(self.device):
+            for part, moved in ((alone, False), (shared, True)):
+                if not part:
+                    continue
+                length = i32([cache.length(s) for s in part])
+                used = max(-(-cache.length(s) // PAGE) for s in part)
+                for g in cache.groups:
+                    pages = i32(cache.page_rows(g.gid, part)[:, :used])
+                    to = i32([fresh[s][g.gid] for s in part]) if moved else None
+                    ops.cache_evict(g.keys, g.values, g.weights, length, pages, keep, recent, first, to)
+        for s in long:
+            cache.shrink(s, keep, fresh.get(s))
 
     def check_device(self) -> None:
         """Raise KernelError if a kernel gave up a bounded wait since the last check (its results, and
@@ -134,6 +188,7 @@ class Engine:
         if min(qlens) < 1:
             raise ValueError("every sequence of a step brings at least one token")
         ctxs = [cache.length(s) for s in slots]
+        firsts = [cache.position(s) for s in slots]
         T, B = sum(qlens), len(runs)
         if want is None:
             want = [[q - 1] for q in qlens]
@@ -152,7 +207,8 @@ class Engine:
             raise ValueError(f"token id outside [0, {self.vocab})")
         # every check that can refuse the step comes before this line: a refused step holds nothing
         cache.reserve([(s, c + q) for s, c, q in zip(slots, ctxs, qlens)])
-        lay = _Layout(T, B, len(rows), len(cache.groups), cache.max_pages_per_seq)
+        prefix = self._prefix_layouts(slots, ctxs) if max(qlens) == 1 else ()
+        lay = _Layout(T, B, len(rows), len(cache.groups), cache.max_pages_per_seq, firsts != ctxs and max(qlens) > 1, prefix)
         buf = np.zeros(lay.size, dtype=np.int32)
 
         def put(name, values):
@@ -161,7 +217,11 @@ class Engine:
 
         put("tokens", toks)
         put("tok_seq", np.repeat(np.arange(B), qlens))
-        put("tok_pos", np.concatenate([np.arange(c, c + q) for c, q in zip(ctxs, qlens)]))
+        put("tok_pos", np.concatenate([np.arange(c, c + q) for c, q in zip(firsts, qlens)]))
+        if lay.places:
+            put("tok_place", np.concatenate([np.arange(c, c + q) for c, q in zip(ctxs, qlens)]))
+        for i, plan in enumerate(lay.prefix):
+            put(f"prefix{i}", plan.ints)
         put("seq_slot", slots)
         put("seq_qstart", np.concatenate([[0], np.cumsum(qlens)[:-1]]))
         put("seq_qlen", qlens)
@@ -175,6 +235,24 @@ class Engine:
                     max_qlen=max(qlens), is_decode=max(qlens) == 1,
                     query_keys=sum(q * c + q * (q + 1) // 2 for c, q in zip(ctxs, qlens)))
         return lay, buf, meta
+
+    def _prefix_layouts(self, slots, ctxs):
+        """Plans for the pages that these sequences share, one for each kind of heads; none where reading them once spares too
+        little: a step's attention then takes the sequences one by one, from the same pages."""
+        if not self.shared_heads or not self.share_prefixes or self.cache.weigh:
+            return ()
+        from .. import ops
+        groups = self.cache.shared_prefixes(slots)
+        spared = sum((len(members) - 1) * n for members, n in groups)
+        if not groups or spared < SHARED_POSITIONS:
+            return ()
+        shared = [0] * len(slots)
+        for members, n in groups:
+            for b in members:
+                shared[b] = n
+        # (sized for a bucket of lengths, as captured steps are)
+        own = self._length_bucket(max(c + 1 - s for c, s in zip(ctxs, shared)))
+        return tuple(ops.PrefixLayout(groups, len(slots), *heads, self.act_dtype, own, ops.sm_count(self.device)) for heads in self.shared_heads)
 
     def _stage(self, buf: np.ndarray) -> torch.Tensor:
         """The descriptor in pinned host memory, ready for an asynchronous copy."""
@@ -205,6 +283,16 @@ class Engine:
         for g in range(lay.groups):
             o, n = lay.off[f"pages{g}"]
             ctx.pages.append(dev[o:o + n].view(lay.B, lay.max_pages))
+        # (one token a sequence: its place is what the sequence held before; captured steps move that along themselves)
+        ctx.tok_place = ctx.seq_ctx if meta["is_decode"] else ctx.tok_pos
+        if lay.places:
+            o, n = lay.off["tok_place"]
+            ctx.tok_place = dev[o:o + n]
+        if lay.prefix:
+            from .. import ops
+            for i, plan in enumerate(lay.prefix):
+                o, n = lay.off[f"prefix{i}"]
+                ctx.prefix[plan.num_heads, plan.num_kv_heads, plan.head_dim] = ops.PrefixPlan(plan, dev[o:o + n])
         ctx.n_tokens, ctx.n_seqs, ctx.n_want = lay.T, lay.B, lay.M
         ctx.max_qlen, ctx.is_decode = meta["max_qlen"], meta["is_decode"]
         ctx.max_len = max(meta["new_lens"])

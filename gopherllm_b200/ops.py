@@ -894,6 +894,11 @@ class PrefixLayout:
         self.items_at, self.shared_at = len(order), len(order) + len(flat)
         self.ints = np.array(order + flat + [v for s in shared_of for v in s], dtype=np.int32)
 
+    def key(self) -> tuple:
+        """What a captured call depends on besides ``ints``, which it reads on the device."""
+        return (self.batch, self.num_heads, self.num_kv_heads, self.head_dim, self.dtype, self.rows, self.n_items, self.splits, self.slots,
+                self.items_at, self.shared_at)
+
 
 PREFIX_BLOCKS_PER_SM = 4
 
@@ -907,6 +912,15 @@ def _check_span_heads(what: str, dtype, head_dim: int) -> None:
             raise KernelError(f"{what}: heads of 1..256, not {head_dim}")
     else:
         raise KernelError(f"{what}: element type {dtype} is not supported (float32 and bfloat16 are)")
+
+
+def span_heads_fit(dtype, head_dim: int) -> bool:
+    """Whether attention over spans (shared pages, weighed positions) takes heads of this type and size."""
+    try:
+        _check_span_heads("", dtype, head_dim)
+    except KernelError:
+        return False
+    return True
 
 
 def span_rows(dtype, head_dim: int) -> int:

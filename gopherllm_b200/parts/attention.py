@@ -25,6 +25,16 @@ class Attention(Mixer):
     capturable = True
     launches_only = True
 
+    @property
+    def forgets(self) -> bool:
+        """Its cache can be weighed and cut down: whole-sequence attention."""
+        return self.spec.window <= 0
+
+    @property
+    def shared_heads(self):
+        """(query heads, key/value heads, head size) of attention that may read shared pages once for all who share them."""
+        return (self.spec.num_heads, self.spec.num_kv_heads, self.spec.head_dim) if self.spec.window <= 0 else None
+
     def __init__(self, spec: MixerSpec):
         if spec.num_heads % spec.num_kv_heads:
             raise ValueError("num_heads must be a multiple of num_kv_heads")
@@ -107,7 +117,7 @@ class Attention(Mixer):
         return [("qkv", self.w_qkv, self.b_qkv, None), ("out", self.w_out, self.b_out, None)]
 
     def decode_fusable(self, ctx, cache):
-        if not ctx.is_decode or cache is None or self.v_from_k or self.gate:
+        if not ctx.is_decode or cache is None or self.v_from_k or self.gate or cache.weights is not None or self._prefix(ctx) is not None:
             return None
         s = self.spec
         tables = self.position.tables(ctx)
@@ -117,6 +127,10 @@ class Attention(Mixer):
                     window=s.window, cos=cos, sin=sin, interleaved=s.position.interleaved,
                     head_norm=self.q_norm is not None, k=cache.k, v=cache.v, pages=ctx.pages[cache.group],
                     writes=cache.writes)
+
+    def _prefix(self, ctx):
+        """The step's plan for pages that its sequences share, if it has one for these heads."""
+        return ctx.prefix.get(self.shared_heads) if ctx.prefix else None
 
     def until_last(self, xn, ctx, cache, first=None):
         """Everything but the output projection: the attention output [T, heads * head size] with the
@@ -130,7 +144,9 @@ class Attention(Mixer):
         group = s.num_heads // s.num_kv_heads
         gate_off = (s.num_heads + (1 if self.v_from_k else 2) * s.num_kv_heads) * s.head_dim if self.gate else -1
         span = ctx.max_len if s.window <= 0 else min(ctx.max_len, s.window + ops.PAGE)      # positions a token's keys can lie on
-        if (ctx.is_decode and self.q_norm is not None and self.q_norm.rms and not s.qk_norm.bias
+        prefix = self._prefix(ctx)
+        alone = prefix is None and cache.weights is None         # neither shared pages nor weights: attention may take the projection's rows
+        if (alone and ctx.is_decode and self.q_norm is not None and self.q_norm.rms and not s.qk_norm.bias
                 and ops.decode_takes_head(qkv.dtype, cache.k.dtype, s.head_dim, qkv.shape[1],
                                           s.position.interleaved or cos is None)):
             # one token a sequence: head norm, rotation, cache write, attention and gate in one kernel
@@ -141,7 +157,7 @@ class Attention(Mixer):
                                       splits, self.q_norm.weight, self.k_norm.weight, s.qk_norm.eps, s.window, cos, sin,
                                       s.q_scale, cache.writes, self.v_from_k, gate_off)
             return o, self.w_out, self.b_out
-        if (ctx.is_decode and not self.v_from_k and not self.gate and group <= ops.DECODE_MAX_GROUP
+        if (alone and ctx.is_decode and not self.v_from_k and not self.gate and group <= ops.DECODE_MAX_GROUP
                 and ops.decode_takes_qkv(qkv.dtype, cache.k.dtype, s.head_dim, 0 if cos is None else cos.shape[1],
                                          s.position.interleaved, self.q_norm is not None)):
             # one token a sequence: attention reads the projection's output itself (rotation, query scale
@@ -158,11 +174,20 @@ class Attention(Mixer):
         if self.q_norm is not None:
             qn, kn = (self.q_norm.weight, self.q_norm.bias), (self.k_norm.weight, self.k_norm.bias)
             eps, rms = s.qk_norm.eps, self.q_norm.rms
-        ops.qkv_to_cache(qkv, q, cache.k, cache.v, ctx.tok_seq, ctx.tok_pos, pages,
+        ops.qkv_to_cache(qkv, q, cache.k, cache.v, ctx.tok_seq, ctx.tok_place, pages,
                          s.num_heads, s.num_kv_heads, s.head_dim, s.q_scale, cos, sin,
                          interleaved=s.position.interleaved, q_norm=qn, k_norm=kn,
                          norm_eps=eps, norm_rms=rms, write_kv=cache.writes, v_from_k=self.v_from_k)
         o = ops.empty(q.shape, q.dtype, q.device)
+        if not alone:
+            if cache.weights is not None:
+                ops.attention_weighed(q, o, cache.k, cache.v, cache.weights, ctx.seq_qstart, ctx.seq_qlen, ctx.seq_ctx, pages,
+                                      s.num_heads, s.num_kv_heads, s.head_dim, ctx.max_qlen, ctx.max_len)
+            else:
+                ops.attention_prefix(q, o, cache.k, cache.v, ctx.seq_ctx, pages, prefix, s.num_heads, s.num_kv_heads, s.head_dim)
+            if self.gate:
+                ops.sigmoid_gate(o, qkv, gate_off)
+            return o, self.w_out, self.b_out
         ops.attention(q, o, cache.k, cache.v, ctx, pages, s.num_heads, s.num_kv_heads,
                       s.head_dim, window=s.window, gate=qkv if self.gate else None, gate_off=gate_off)
         return o, self.w_out, self.b_out

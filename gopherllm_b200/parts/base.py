@@ -133,6 +133,13 @@ class Mixer(Part):
     # that kind; a block whose parts all offer the fused form may run its decode step as one kernel.
     decode_fusable = None
 
+    # Whether the cache entry this mixer writes can be weighed (cache.weights) and cut down to what weighs most; it must then place
+    # its keys by ctx.tok_place and see a sequence's positions by their number in the cache alone.
+    forgets = False
+
+    # Optional: (query heads, key/value heads, head size) of a mixer that reads ctx.prefix, the step's plan for shared pages.
+    shared_heads = None
+
     # A mixer that sets this accepts callables among ``add``: it calls them just before its last
     # product and adds what they return.  A block uses that to let another branch run beside the
     # mixer on a second stream and join only where its result is needed.

@@ -1,0 +1,200 @@
+"""Sequences that share pages, sequences that are cut down: the cache's books, and what the generation loop decides (no device needed)."""
+import random
+
+import pytest
+import torch
+
+from gopherllm_b200.cache.pool import CacheFull
+from gopherllm_b200.cache.sequence_cache import PAGE, SequenceCache
+from gopherllm_b200.engine.generate import GenerationOptions, begin_alike, pages_for, plan_batches
+from gopherllm_b200.parts.base import KVRequest, StateRequest
+
+
+def make(pages=20, reqs=(KVRequest(2, 16), KVRequest(2, 16)), slots=6, allocate=False, positions=640, weigh=False, last=None):
+    return SequenceCache(list(reqs), pages * PAGE, positions, torch.float32, "cpu", max_slots=slots, allocate=allocate, weigh=weigh, last_position=last)
+
+
+def grow(c, slot, n):
+    c.reserve([(slot, n)])
+    c.commit(slot, n)
+
+
+def test_fork_shares_whole_pages_and_copies_the_one_begun():
+    c = make(allocate=True, weigh=True)
+    a = c.open()
+    grow(c, a, 150)
+    g = c.groups[0]
+    for t in (g.keys, g.values, g.weights):
+        t.copy_(torch.arange(t.numel(), dtype=torch.float32).view(t.shape))
+    b = c.fork(a)
+    pa, pb = c._pages[a][0], c._pages[b][0]
+    assert pa[:2] == pb[:2] and pa[2] != pb[2] and c.length(b) == 150
+    for t in (g.keys, g.values, g.weights):
+        assert torch.equal(t[:, pa[2]], t[:, pb[2]])
+    c.check()
+    assert c.tokens_held() == 4 * PAGE and g.pool.held_count == 4 and c.shares_pages(a) and c.shares_pages(b)
+    grow(c, b, 300)
+    assert c._pages[a][0] == pa and len(c._pages[b][0]) == 5
+    d = c.fork(b, 64)
+    assert c._pages[d][0] == pa[:1] and c.groups[0].more == {pa[0]: 2, pa[1]: 1}
+    c.close(a)
+    c.check()
+    assert c.groups[0].more == {pa[0]: 1}
+    c.close(b)
+    c.check()
+    assert c.groups[0].pool.held_count == 1 and not c.shares_pages(d)
+    c.close(d)
+    c.check()
+    assert c.groups[0].pool.held_count == 0
+
+
+def test_shared_prefixes():
+    c = make(pages=60, slots=12)
+    a = c.open()
+    grow(c, a, 400)
+    b, d = c.fork(a), c.fork(a, 200)
+    other = c.open()
+    grow(c, other, 70)
+    e = c.fork(other, 64)
+    lone = c.open()
+    grow(c, lone, 10)
+    grow(c, b, 500)
+    assert c.shared_prefixes([a, b]) == [([0, 1], 384)]
+    assert c.shared_prefixes([d, lone, b, a]) == [([0, 2, 3], 192)]
+    assert c.shared_prefixes([e, a, other, b]) == [([0, 2], 64), ([1, 3], 384)]
+    assert c.shared_prefixes([a, lone]) == [] and c.shared_prefixes([lone]) == []
+    f = c.fork(b)                                     # shares more with b than with a
+    assert c.shared_prefixes([b, f]) == [([0, 1], 448)] and c.shared_prefixes([f, a, b]) == [([0, 1, 2], 384)]
+
+
+def test_forks_that_are_refused():
+    c = make(pages=5)
+    a = c.open()
+    grow(c, a, 200)
+    for n in (-1, 201):
+        with pytest.raises(ValueError):
+            c.fork(a, n)
+    with pytest.raises(ValueError):
+        c.fork(5)
+    with pytest.raises(CacheFull):
+        b = c.fork(a)                                 # takes the last page ...
+        c.fork(a)                                     # ... and there is none for another's begun page
+    c.check()
+    c.close(b)
+    s = make(reqs=(KVRequest(2, 16), StateRequest((3,))), allocate=True)
+    a = s.open()
+    grow(s, a, 100)
+    s._states[0][a] = 7.0
+    with pytest.raises(ValueError, match="no longer held"):
+        s.fork(a, 64)                                 # the state has moved on
+    assert s._states[0][s.fork(a)].tolist() == [7.0] * 3
+    w = make(reqs=(KVRequest(2, 16, window=100),))
+    a = w.open()
+    grow(w, a, 400)
+    with pytest.raises(ValueError, match="no longer held"):
+        w.fork(a, 64)
+    b = w.fork(a)                                     # pages given back before the window stay given back
+    w.check()
+    grow(w, a, 600)
+    w.check()
+    assert w.shared_prefixes([a, b]) == []            # (a window's pages are not read as a prefix)
+    w.close(a)
+    w.check()
+    w.close(b)
+    w.check()
+    assert w.groups[0].pool.held_count == 0
+
+
+def test_shrink():
+    c = make(weigh=True, last=2000)
+    a = c.open()
+    grow(c, a, 300)
+    c.shrink(a, 100)
+    c.check()
+    assert c.length(a) == 100 and c.position(a) == 300 and len(c._pages[a][0]) == 2
+    grow(c, a, 130)
+    assert c.position(a) == 330
+    b = c.fork(a)
+    assert c.position(b) == 330
+    with pytest.raises(ValueError, match="no longer held"):
+        c.fork(a, 64)
+    with pytest.raises(ValueError, match="of its own"):
+        c.shrink(b, 64)
+    onto = c.fresh_pages([(b, 70)])
+    c.shrink(b, 70, onto[b])
+    c.check()
+    assert c.length(b) == 70 and c.position(b) == 330 and not c.shares_pages(a)
+    for n in (0, 71):
+        with pytest.raises(ValueError):
+            c.shrink(b, n)
+    with pytest.raises(CacheFull):
+        c.fresh_pages([(a, 64 * 30)])
+    c.close(a)
+    c.close(b)
+    c.check()
+    d = c.open()
+    assert c.position(d) == 0
+    with pytest.raises(CacheFull, match="the cache holds"):
+        c.reserve([(d, 641)])
+    small = make(weigh=True, last=700)
+    a = small.open()
+    grow(small, a, 600)
+    small.shrink(a, 64)
+    small.reserve([(a, 164)])
+    with pytest.raises(CacheFull, match="position"):
+        small.reserve([(a, 165)])
+
+
+@pytest.mark.parametrize("seed", range(20))
+def test_books_under_random_use(seed):
+    rng = random.Random(seed)
+    c = make(pages=40, slots=8, reqs=(KVRequest(1, 8), KVRequest(1, 16)), positions=600, weigh=True, last=5000)
+    for _ in range(200):
+        live = c.live_slots()
+        try:
+            what = rng.random()
+            if not live or what < 0.2:
+                c.open()
+            elif what < 0.4:
+                s = rng.choice(live)
+                c.fork(s, None if c._forgotten[s] else rng.choice((None, rng.randint(0, c.length(s)))))
+            elif what < 0.7:
+                s = rng.choice(live)
+                grow(c, s, c.length(s) + rng.randint(1, 150))
+            elif what < 0.85:
+                s = rng.choice(live)
+                if c.length(s) > 1:
+                    keep = rng.randint(1, c.length(s))
+                    c.shrink(s, keep, c.fresh_pages([(s, keep)])[s] if c.shares_pages(s) else None)
+            else:
+                c.close(rng.choice(live))
+        except CacheFull:
+            pass
+        c.check()
+        live = c.live_slots()
+        for members, n in c.shared_prefixes(live):
+            heads = {tuple(c._pages[live[i]][0][:n // PAGE]) for i in members}
+            assert n >= PAGE and len(heads) == 1 and all(c.length(live[i]) >= n for i in members)
+    for s in c.live_slots():
+        c.close(s)
+    c.check()
+    assert all(g.pool.held_count == 0 and not g.more for g in c.groups)
+
+
+def test_begin_alike():
+    a = list(range(1000))
+    assert begin_alike([a[:300], a[:100] + [5] * 300, a[:130]]) == [([0, 1, 2], 64)]
+    assert begin_alike([a[:300], a[:300]]) == [([0, 1], 256)]
+    assert begin_alike([a[:257], a[:257]]) == [([0, 1], 256)] and begin_alike([a[:256], a[:257]]) == [([0, 1], 192)]
+    assert begin_alike([a[:64], a[:64]]) == [] and begin_alike([a[:65], a[:66]]) == [([0, 1], 64)]
+    assert begin_alike([a[:90], [7] * 90, a[:80], [7] * 200, [8] * 70]) == [([0, 2], 64), ([1, 3], 64)]
+
+
+def test_pages_and_options_of_a_sequence_that_is_cut():
+    assert pages_for(1000, 5000, 2048) == 32 and pages_for(1000, 5000, 20480, keep=512) == 16 and pages_for(100, 5000, 20480, keep=512) == 9
+    assert pages_for(100, 20, 20480, keep=512) == 2 and pages_for(1000, 5000, 20480, keep=512, shares=True) == 25
+    assert plan_batches([100, 100], 5000, 20480, page_budget=18, slot_budget=8, keep=512) == [[0, 1]]
+    GenerationOptions(cache_keep=10, cache_recent=6, cache_first=4).validate()
+    for kw in (dict(cache_keep=-1), dict(cache_keep=10, cache_recent=11), dict(cache_recent=1), dict(cache_keep=4, cache_first=-1), dict(cache_keep=4.0)):
+        with pytest.raises(ValueError):
+            GenerationOptions(**kw).validate()
