@@ -10,6 +10,7 @@
 // sequence has of its own is spans of its own.  (2) Attention that keeps the weight every cached position is given: the
 // scores are written down beside the spans' results, and the pass that puts the spans together turns them into weights.
 //
+// Shared pages with many rows run on the 5th-generation tensor cores (the second half of this file); all else as follows.
 // A block takes one span for up to 8 NT rows.  It streams the span's pages through shared memory with cp.async; inside a page
 // each of its four warps owns 16 of the 64 keys: scores are an mma.sync chain with the keys as the 16-row operand and the rows as
 // columns, maximum, sum and rescaling are 32-bit, the weights turn into the other operand of the second product by a transposing
@@ -17,6 +18,10 @@
 // end of the span.  Weights are rounded to bfloat16 for the second product (its operand's type); the sums take them unrounded.
 #include "common.cuh"
 #include "decode_common.cuh"
+#include "tma.cuh"
+#include "tcgen05.cuh"
+#include <cooperative_groups.h>
+namespace cg = cooperative_groups;
 
 #ifndef GL_HEAD_DIM
 #error "compile with -DGL_HEAD_DIM=<head size>: this file is built once per head size a model uses, and knows none itself"
@@ -29,7 +34,9 @@ static_assert(GL_HEAD_DIM % 16 == 0 && GL_HEAD_DIM >= 16 && GL_HEAD_DIM <= 256, 
 #define SP_CHUNKS (SP_HD / 8)                       // 16-byte pieces of a row
 #define SP_ROW (SP_HD * 2 + 16)                     // padded row in bytes: conflict-free ldmatrix
 #define SP_TILE (GL_PAGE * SP_ROW)                  // one page of keys (or values) of one head
+#ifndef SP_STAGES
 #define SP_STAGES 2                                 // pages of keys and values in flight
+#endif
 #define SP_MAX_NT (SP_HD <= 128 ? 4 : 2)            // columns of 8 rows: the accumulators of more do not fit the registers
 #define SP_LOG2E 1.4426950408889634f
 
@@ -50,6 +57,7 @@ struct SpanArgs {
     float* scores;                // [B, nH, reach] or null
     float* weights;               // [pages, nKV, GL_PAGE] or null
     int B, nH, nKV, max_pages, n_pages, n_items, splits, slots, chunks, reach;
+    int early, held;              // set by the launchers: see the kernel
 };
 
 __device__ __forceinline__ void sp_cp16(unsigned dst, const void* src, int bytes) {
@@ -87,6 +95,18 @@ __device__ __forceinline__ float sp_exp2(float x) {
 // result with maximum m_i takes in one with maximum m >= m_i (nothing seen yet: both -inf):
 __device__ __forceinline__ float sp_factor(float m_i, float m) { return m_i == m ? 1.0f : sp_exp2(m_i - m); }
 
+// loads that stay behind the wait before them (what another kernel wrote meanwhile)
+__device__ __forceinline__ float2 sp_read(const float2* p) {
+    float2 v;
+    asm volatile("ld.global.cg.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "l"(p) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 sp_read(const float4* p) {
+    float4 v;
+    asm volatile("ld.global.cg.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p) : "memory");
+    return v;
+}
+
 template <int NT>
 __host__ __device__ constexpr int sp_fixed_bytes() {       // queries, then per row: sequence, head, last position seen
     return 8 * NT * SP_ROW + 8 * NT * 12;
@@ -94,26 +114,35 @@ __host__ __device__ constexpr int sp_fixed_bytes() {       // queries, then per 
 template <int NT>
 __host__ __device__ constexpr size_t sp_smem() {
     const size_t pages = 2 * SP_STAGES * (size_t)SP_TILE;
-    const size_t merge = sizeof(float) * (4 * 8 * NT * 2 + 4 * (size_t)SP_HD * 8 * NT);       // over the pages, when they are done
+    const size_t merge = sizeof(float) * (4 * 8 * NT * 2 + 5 * (size_t)SP_HD * 8 * NT + 8 * NT * 2);       // over the pages, when they are done
     return (pages > merge ? pages : merge) + sp_fixed_bytes<NT>();
 }
 
-// SHARED: blockIdx.x is an item of the plan; else blockIdx = (split, key/value head and its share of the query heads, sequence).
-template <int NT, bool SHARED>
+// What a block does: a stretch of shared pages for the rows of an item of the plan (blockIdx.x: the item), or a split of a
+// sequence's own pages for the query heads of a key/value head (blockIdx = split, head and its share of the query heads, sequence),
+// whose result is written down for the joining kernel, or joined here: the splits are then the blocks of a cluster, meet in
+// distributed shared memory, take in what the shared pages gave and write the output.
+enum { SP_ITEM = 0, SP_SPLIT = 1, SP_JOIN = 2 };
+
+template <int NT, int MODE>
 __global__ void __launch_bounds__(SP_THREADS)
 attn_span_kernel(SpanArgs a) {
     extern __shared__ __align__(16) unsigned char smem[];
+    constexpr bool SHARED = MODE == SP_ITEM;
     constexpr size_t AREA = sp_smem<NT>() - sp_fixed_bytes<NT>();
     const unsigned sbase = ad_smem(smem);
     unsigned char* qs = smem + AREA;                               // [8 NT] rows of queries
     int* row_seq = (int*)(qs + 8 * NT * SP_ROW);                   // [8 NT]
     int* row_head = row_seq + 8 * NT;
     int* row_last = row_head + 8 * NT;
+    float* held = (float*)(smem + sp_smem<NT>());                  // [rows][a.held] scores of the split's keys, where they are kept
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int grp = lane >> 2, t = lane & 3;
     const int G = a.nH / a.nKV;
+    // A kernel over shared pages lets the next one start once everything before both is complete; that one (early) then walks the
+    // sequences' own pages beside it and waits for it only where it takes in its results.
+    if (!a.early) gl_grid_wait();
     gl_grid_launch_dependents();
-    gl_grid_wait();
 
     int g, rows, p_begin, p_end, slot, table;
     if (SHARED) {
@@ -212,7 +241,17 @@ attn_span_kernel(SpanArgs a) {
                 ad_mma(s[n], af, b0, b1);
             }
         }
-        if (!SHARED && a.scores) {
+        if (MODE == SP_JOIN && a.weights) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int r = n * 8 + 2 * t + (e & 1);
+                    const int i = (p - p_begin) * GL_PAGE + warp * 16 + grp + (e >> 1) * 8;
+                    if (r < rows && i < a.held) held[r * a.held + i] = s[n][e];
+                }
+        }
+        if (MODE == SP_SPLIT && a.scores) {
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -283,6 +322,8 @@ attn_span_kernel(SpanArgs a) {
     // the four warps' softmaxes meet over the pages' memory
     float* ml_w = (float*)smem;                            // [4][8 NT][2]
     float* o_w = ml_w + 4 * 8 * NT * 2;                    // [4][hd][8 NT]
+    float* fin_o = o_w + 4 * SP_HD * 8 * NT;               // [rows][hd] this split's result, for the cluster
+    float* fin_ml = fin_o + 8 * NT * SP_HD;                // [rows][2]
     __syncthreads();
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -312,115 +353,523 @@ attn_span_kernel(SpanArgs a) {
             ov = fmaf(f, o_w[((size_t)w * SP_HD + d) * (8 * NT) + r], ov);
             l = fmaf(f, ml_w[(w * 8 * NT + r) * 2 + 1], l);
         }
+        if (MODE == SP_JOIN) {
+            fin_o[i] = ov;
+            if (d == 0) { fin_ml[2 * r] = m; fin_ml[2 * r + 1] = l; }
+            continue;
+        }
         const size_t at = ((size_t)row_seq[r] * a.nH + row_head[r]) * a.slots + slot;
         a.part_o[at * SP_HD + d] = ov;
         if (d == 0) { a.part_ml[at * 2] = m; a.part_ml[at * 2 + 1] = l; }
     }
+    if (MODE != SP_JOIN) return;
+    // The blocks of the cluster put their results and what the shared pages gave together: every block the factors of all parts,
+    // a row a warp, then its share of the outputs, four at a time.
+    cg::cluster_group cluster = cg::this_cluster();
+    const int S = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+    const int b = table, n_pre = a.seq_shared ? a.seq_shared[2 * b + 1] : 0, parts = S + n_pre;
+    float* fac = held + (a.weights ? rows * a.held : 0);          // [rows][parts]: factor / sum
+    float* stat = ml_w;                                    // [rows][2]: maximum, 1 / sum (the warps' results are done with)
+    if (a.early) gl_grid_wait();
+    if (S > 1) cluster.sync();
+    else __syncthreads();
+    for (int r = warp; r < rows; r += SP_THREADS / 32) {
+        const float2* pre = (const float2*)a.part_ml + ((size_t)b * a.nH + row_head[r]) * a.slots - S;
+        auto part = [&](int k) { return k < S ? ((const float2*)(S > 1 ? cluster.map_shared_rank(fin_ml, k) : fin_ml))[r] : sp_read(pre + k); };
+        float m = -INFINITY, l = 0.f;
+        for (int k = lane; k < parts; k += 32) m = fmaxf(m, part(k).x);
+        m = gl_warp_max(m);
+        for (int k = lane; k < parts; k += 32) {
+            const float2 ml = part(k);
+            const float f = sp_factor(ml.x, m);
+            fac[r * parts + k] = f;
+            l = fmaf(f, ml.y, l);
+        }
+        l = gl_warp_sum(l);
+        const float inv = l == 0.f ? 0.f : 1.0f / l;
+        for (int k = lane; k < parts; k += 32) fac[r * parts + k] *= inv;
+        if (lane == 0) { stat[2 * r] = m; stat[2 * r + 1] = inv; }
+    }
+    __syncthreads();
+    for (int i = tid * S + rank; i < rows * (SP_HD / 4); i += SP_THREADS * S) {
+        const int r = i / (SP_HD / 4), c = i - r * (SP_HD / 4);
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+        auto add = [&](float f, const float4 v) {
+            sum.x = fmaf(f, v.x, sum.x); sum.y = fmaf(f, v.y, sum.y); sum.z = fmaf(f, v.z, sum.z); sum.w = fmaf(f, v.w, sum.w);
+        };
+        for (int k = 0; k < S; ++k) add(fac[r * parts + k], ((const float4*)(S > 1 ? cluster.map_shared_rank(fin_o, k) : fin_o))[i]);
+        const float4* pre = (const float4*)a.part_o + (((size_t)b * a.nH + row_head[r]) * a.slots) * (SP_HD / 4) + c;
+#pragma unroll 8
+        for (int k = 0; k < n_pre; ++k) add(fac[r * parts + S + k], sp_read(pre + (size_t)k * (SP_HD / 4)));
+        const __nv_bfloat162 lo = __floats2bfloat162_rn(sum.x, sum.y), hi = __floats2bfloat162_rn(sum.z, sum.w);
+        *(uint2*)(a.out + ((size_t)(a.seq_row ? a.seq_row[b] : b) * a.nH + row_head[r]) * SP_HD + 4 * c) = make_uint2(*(const unsigned*)&lo, *(const unsigned*)&hi);
+    }
+    if (a.weights) {                                       // this block's scores become weights
+        const int n = min(min((p_end - p_begin) * GL_PAGE, total - p_begin * GL_PAGE), a.held);
+        for (int i = tid; i < n; i += SP_THREADS) {
+            float given = 0.f;
+            for (int r = 0; r < rows; ++r) given = fmaf(sp_exp2(fmaf(held[r * a.held + i], SP_LOG2E, -stat[2 * r])), stat[2 * r + 1], given);
+            const int j = p_begin * GL_PAGE + i;
+            float* w = a.weights + ((size_t)gl_checked(pg[j / GL_PAGE], a.n_pages, GL_BAD_PAGE) * a.nKV + g) * GL_PAGE + j % GL_PAGE;
+            *w = j < total - 1 ? *w + given : given;
+        }
+    }
+    if (S > 1) cluster.sync();                             // a block's memory stays until its peers have read it
 }
 
-// The spans of a row put together: blockIdx = (head, sequence).
-__global__ void attn_span_join_kernel(SpanArgs a) {
-    gl_grid_launch_dependents();
+// The spans of a sequence put together: blockIdx = (share of the positions, key/value head, sequence).  The blocks of a head share its
+// output out by query heads; with scores written down each turns the scores of its positions into weights, added up over the
+// query heads.  A position new in this step starts from nothing, whatever its place held.
+#define SP_JOIN_THREADS 256
+__global__ void __launch_bounds__(SP_JOIN_THREADS)
+attn_span_join_kernel(SpanArgs a) {
+    extern __shared__ float ml_all[];                      // [G][2]: maximum, 1 / sum
+    const int b = blockIdx.z, g = blockIdx.y, G = a.nH / a.nKV, tid = threadIdx.x, lane = tid & 31;
     gl_grid_wait();
-    const int h = blockIdx.x, b = blockIdx.y;
+    gl_grid_launch_dependents();
     if (a.seq_qlen && a.seq_qlen[b] <= 0) return;
     const int n = (a.seq_shared ? a.seq_shared[2 * b + 1] : 0) + a.splits;
-    const size_t at = ((size_t)b * a.nH + h) * a.slots;
-    const float* ml = a.part_ml + at * 2;
-    float m = -INFINITY;
-    for (int s = 0; s < n; ++s) m = fmaxf(m, ml[2 * s]);
-    __nv_bfloat16* out = a.out + ((size_t)(a.seq_row ? a.seq_row[b] : b) * a.nH + h) * SP_HD;
-    for (int d = threadIdx.x; d < SP_HD; d += blockDim.x) {
-        float o = 0.f, l = 0.f;
-        for (int s = 0; s < n; ++s) {
-            const float f = sp_factor(ml[2 * s], m);
-            o = fmaf(f, a.part_o[(at + s) * SP_HD + d], o);
-            l = fmaf(f, ml[2 * s + 1], l);
-        }
-        out[d] = __float2bfloat16_rn(l == 0.f ? 0.f : o / l);
-    }
-}
-
-// The weights a row gave its positions, added up over the query heads of a key/value head: blockIdx = (page, key/value head, sequence).
-// A position new in this step starts from nothing, whatever its place held.
-__global__ void __launch_bounds__(GL_PAGE)
-attn_span_weigh_kernel(SpanArgs a) {
-    gl_grid_launch_dependents();
-    gl_grid_wait();
-    const int b = blockIdx.z, g = blockIdx.y, p = blockIdx.x, G = a.nH / a.nKV;
-    const int pos = a.seq_ctx[b], j = p * GL_PAGE + threadIdx.x;
-    if ((a.seq_qlen && a.seq_qlen[b] <= 0) || p > pos / GL_PAGE) return;
-    float given = 0.f;
-    for (int h = g * G; h < (g + 1) * G; ++h) {
-        const float* ml = a.part_ml + ((size_t)b * a.nH + h) * a.slots * 2;
+    for (int i = tid >> 5; i < G; i += SP_JOIN_THREADS / 32) {
+        const float* ml = a.part_ml + ((size_t)b * a.nH + g * G + i) * a.slots * 2;
         float m = -INFINITY, l = 0.f;
-        for (int s = 0; s < a.splits; ++s) m = fmaxf(m, ml[2 * s]);
-        for (int s = 0; s < a.splits; ++s) l = fmaf(sp_factor(ml[2 * s], m), ml[2 * s + 1], l);
-        if (j <= pos && j < a.reach) given += sp_exp2(fmaf(a.scores[((size_t)b * a.nH + h) * a.reach + j], SP_LOG2E, -m)) / l;
+        for (int s = lane; s < n; s += 32) m = fmaxf(m, ml[2 * s]);
+        m = gl_warp_max(m);
+        for (int s = lane; s < n; s += 32) l = fmaf(sp_factor(ml[2 * s], m), ml[2 * s + 1], l);
+        l = gl_warp_sum(l);
+        if (lane == 0) { ml_all[2 * i] = m; ml_all[2 * i + 1] = 1.0f / l; }
     }
-    if (j > pos || j >= a.reach) return;
-    float* w = a.weights + ((size_t)gl_checked(a.pages[(size_t)b * a.max_pages + p], a.n_pages, GL_BAD_PAGE) * a.nKV + g) * GL_PAGE + threadIdx.x;
-    *w = j < pos ? *w + given : given;
+    __syncthreads();
+    for (int i = blockIdx.x; i < G; i += gridDim.x) {
+        const size_t at = ((size_t)b * a.nH + g * G + i) * a.slots;
+        const float m = ml_all[2 * i], inv = ml_all[2 * i + 1];
+        for (int d = tid; d < SP_HD; d += SP_JOIN_THREADS) {
+            float o = 0.f;
+#pragma unroll 4
+            for (int s = 0; s < n; ++s) o = fmaf(sp_factor(a.part_ml[(at + s) * 2], m), a.part_o[(at + s) * SP_HD + d], o);
+            a.out[((size_t)(a.seq_row ? a.seq_row[b] : b) * a.nH + g * G + i) * SP_HD + d] = __float2bfloat16_rn(inv == INFINITY ? 0.f : o * inv);
+        }
+    }
+    if (!a.weights) return;
+    const int pos = a.seq_ctx[b], most = min(pos + 1, a.reach);
+    for (int j = blockIdx.x * SP_JOIN_THREADS + tid; j < most; j += gridDim.x * SP_JOIN_THREADS) {
+        const float* sc = a.scores + ((size_t)b * a.nH + g * G) * a.reach + j;
+        float given = 0.f;
+#pragma unroll 4
+        for (int i = 0; i < G; ++i) given = fmaf(sp_exp2(fmaf(sc[(size_t)i * a.reach], SP_LOG2E, -ml_all[2 * i])), ml_all[2 * i + 1], given);
+        float* w = a.weights + ((size_t)gl_checked(a.pages[(size_t)b * a.max_pages + j / GL_PAGE], a.n_pages, GL_BAD_PAGE) * a.nKV + g) * GL_PAGE + j % GL_PAGE;
+        *w = j < pos ? *w + given : given;
+    }
 }
 
-template <int NT, bool SHARED>
-static int launch_span(const SpanArgs& a, dim3 grid, cudaStream_t stream) {
+#define SP_HELD_BYTES (56 * 1024)                  // scores a block keeps in shared memory at most
+#define SP_FACTOR_BYTES (24 * 1024)                // factors of the parts of its rows
+
+template <int NT, int MODE>
+static int launch_span(const SpanArgs& a, dim3 grid, int cluster, cudaStream_t stream) {
     static bool allowed[64] = {};
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) { cudaGetLastError(); return GL_ERR_DRIVER; }
+    const size_t most = sp_smem<NT>() + (MODE == SP_JOIN ? SP_HELD_BYTES + SP_FACTOR_BYTES : 0);
     if (!allowed[dev]) {
-        if (cudaFuncSetAttribute(attn_span_kernel<NT, SHARED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sp_smem<NT>()) != cudaSuccess) {
+        if (cudaFuncSetAttribute(attn_span_kernel<NT, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most) != cudaSuccess) {
             cudaGetLastError();
             return GL_ERR_SMEM;
         }
         allowed[dev] = true;
     }
-    return gl_launch(attn_span_kernel<NT, SHARED>, grid, dim3(SP_THREADS), sp_smem<NT>(), stream, 1, a);
+    const size_t smem = sp_smem<NT>() + (MODE == SP_JOIN ? sizeof(float) * ((a.weights ? (size_t)a.held * (a.nH / a.nKV) : 0) + 8 * NT * (size_t)(a.slots + a.splits)) : 0);
+    if (smem > most) return GL_ERR_SMEM;
+    return gl_launch(attn_span_kernel<NT, MODE>, grid, dim3(SP_THREADS), smem, stream, cluster, a);
 }
 
-template <bool SHARED>
-static int launch_spans(const SpanArgs& a, int rows, dim3 grid, cudaStream_t stream) {
-    if (rows <= 8) return launch_span<1, SHARED>(a, grid, stream);
-    if (rows <= 16) return launch_span<2, SHARED>(a, grid, stream);
-    return launch_span<SP_MAX_NT, SHARED>(a, grid, stream);
+template <int MODE>
+static int launch_spans(const SpanArgs& a, int rows, dim3 grid, int cluster, cudaStream_t stream) {
+    if (rows <= 8) return launch_span<1, MODE>(a, grid, cluster, stream);
+    if (rows <= 16) return launch_span<2, MODE>(a, grid, cluster, stream);
+    return launch_span<SP_MAX_NT, MODE>(a, grid, cluster, stream);
 }
 
 static int span_checked(const SpanArgs& a) {
-    if (a.nH <= 0 || a.nKV <= 0 || a.nH % a.nKV || a.B > 65535 || a.splits < 1 || a.slots < a.splits || a.max_pages <= 0) return GL_ERR_SHAPE;
+    if (a.nH <= 0 || a.nKV <= 0 || a.nH % a.nKV || a.B > 65535 || a.splits < 1 || a.slots < 0 || a.max_pages <= 0) return GL_ERR_SHAPE;
     const int G = a.nH / a.nKV;
     if (a.chunks < 1 || a.chunks > G || (long long)a.nKV * a.chunks > 65535 || (G + a.chunks - 1) / a.chunks > 8 * SP_MAX_NT) return GL_ERR_SHAPE;
     if ((a.chunks - 1) * ((G + a.chunks - 1) / a.chunks) >= G) return GL_ERR_SHAPE;        // every share of the heads has one
     if (((uintptr_t)a.q | (uintptr_t)a.k_cache | (uintptr_t)a.v_cache) & 15) return GL_ERR_ALIGN;
-    if (!a.part_o || !a.part_ml) return GL_ERR_SHAPE;
-    return GL_OK;
+    return a.slots > 0 && (!a.part_o || !a.part_ml) ? GL_ERR_SHAPE : GL_OK;
 }
 
-GL_API int gl_attention_span_rows() { return 8 * SP_MAX_NT; }        // rows of q a span takes at most
-
-// rows: the most that one of the plan's items has
-GL_API int gl_attention_prefix(const SpanArgs* args, int rows, cudaStream_t stream) {
-    const SpanArgs& a = *args;
-    if (a.B <= 0) return GL_OK;
-    int rc = span_checked(a);
-    if (rc != GL_OK) return rc;
-    if (a.n_items < 0 || a.scores || a.weights || !a.seq_shared || (a.n_items > 0 && (!a.items || !a.order || rows < 1 || rows > 8 * SP_MAX_NT))) return GL_ERR_SHAPE;
-    if (a.n_items > 0 && (rc = launch_spans<true>(a, rows, dim3(a.n_items, a.nKV), stream)) != GL_OK) return rc;
+static int launch_join(const SpanArgs& a, cudaStream_t stream) {
     const int G = a.nH / a.nKV;
-    if ((rc = launch_spans<false>(a, (G + a.chunks - 1) / a.chunks, dim3(a.splits, a.nKV * a.chunks, a.B), stream)) != GL_OK) return rc;
-    return gl_launch(attn_span_join_kernel, dim3(a.nH, a.B), dim3(SP_HD >= 128 ? 128 : 64), 0, stream, 1, a);
+    // with weights: a block for a thousand positions, one for each query head at least
+    const int shares = a.weights ? (a.reach + 4 * SP_JOIN_THREADS - 1) / (4 * SP_JOIN_THREADS) : 1;
+    return gl_launch(attn_span_join_kernel, dim3(shares > G ? shares : G, a.nKV, a.B), dim3(SP_JOIN_THREADS), 2 * G * sizeof(float), stream, 1, a);
 }
 
-GL_API int gl_attention_weighed(const SpanArgs* args, cudaStream_t stream) {
-    const SpanArgs& a = *args;
+static int shared_tc(const SpanArgs& a, int rows, cudaStream_t stream);
+
+// rows: the most that one of the plan's items has; joined: a sequence's splits are a cluster that joins its results and the shared
+// pages' itself (part_o and part_ml have slots for the shared pages alone), else a second kernel does (and they have the splits' too)
+GL_API int gl_attention_prefix(const SpanArgs* args, int rows, int joined, cudaStream_t stream) {
+    SpanArgs a = *args;
     if (a.B <= 0) return GL_OK;
     int rc = span_checked(a);
     if (rc != GL_OK) return rc;
-    if (!a.scores || !a.weights || a.seq_shared || a.reach <= 0) return GL_ERR_SHAPE;
-    const int G = a.nH / a.nKV, n_pages = (a.reach + GL_PAGE - 1) / GL_PAGE;
-    if ((rc = launch_spans<false>(a, (G + a.chunks - 1) / a.chunks, dim3(a.splits, a.nKV * a.chunks, a.B), stream)) != GL_OK) return rc;
-    if ((rc = gl_launch(attn_span_join_kernel, dim3(a.nH, a.B), dim3(SP_HD >= 128 ? 128 : 64), 0, stream, 1, a)) != GL_OK) return rc;
-    return gl_launch(attn_span_weigh_kernel, dim3(n_pages, a.nKV, a.B), dim3(GL_PAGE), 0, stream, 1, a);
+    if (a.n_items < 0 || a.scores || a.weights || !a.seq_shared || (a.n_items > 0 && (!a.items || !a.order || rows < 1 || a.slots < 1))) return GL_ERR_SHAPE;
+    if (joined ? a.splits > 8 || 8 * SP_MAX_NT * (long long)(a.slots + a.splits) * (int)sizeof(float) > SP_FACTOR_BYTES : a.slots < a.splits) return GL_ERR_SHAPE;
+    const int G = a.nH / a.nKV;
+    a.early = a.held = 0;
+    if (a.n_items > 0) {
+        rc = rows > 8 * SP_MAX_NT ? shared_tc(a, rows, stream) : launch_spans<SP_ITEM>(a, rows, dim3(a.n_items, a.nKV), 1, stream);
+        if (rc != GL_OK) return rc;
+        a.early = joined && gl_pdl;
+    }
+    const dim3 grid(a.splits, a.nKV * a.chunks, a.B);
+    if (joined) return launch_spans<SP_JOIN>(a, (G + a.chunks - 1) / a.chunks, grid, a.splits, stream);
+    if ((rc = launch_spans<SP_SPLIT>(a, (G + a.chunks - 1) / a.chunks, grid, 1, stream)) != GL_OK) return rc;
+    return launch_join(a, stream);
 }
+
+// Without ``scores`` the splits are a cluster that joins its results and keeps its scores in shared memory, else a second kernel
+// joins the splits' partial results and reads the scores back.
+GL_API int gl_attention_weighed(const SpanArgs* args, cudaStream_t stream) {
+    SpanArgs a = *args;
+    if (a.B <= 0) return GL_OK;
+    int rc = span_checked(a);
+    if (rc != GL_OK) return rc;
+    if (!a.weights || a.seq_shared || a.reach <= 0) return GL_ERR_SHAPE;
+    const int G = a.nH / a.nKV;
+    const dim3 grid(a.splits, a.nKV * a.chunks, a.B);
+    a.early = a.held = 0;
+    if (!a.scores) {
+        // (a pitch of 4 more than whole pages: the eight keys of four rows that a warp stores lie in different banks)
+        a.held = ((a.reach + GL_PAGE - 1) / GL_PAGE + a.splits - 1) / a.splits * GL_PAGE + 4;
+        if (a.chunks > 1 || a.splits > 8 || a.slots > 0 || (long long)a.held * G * (int)sizeof(float) > SP_HELD_BYTES) return GL_ERR_SHAPE;
+        return launch_spans<SP_JOIN>(a, G, grid, a.splits, stream);
+    }
+    if (a.slots < a.splits) return GL_ERR_SHAPE;
+    if ((rc = launch_spans<SP_SPLIT>(a, (G + a.chunks - 1) / a.chunks, grid, 1, stream)) != GL_OK) return rc;
+    return launch_join(a, stream);
+}
+
+// ---------------------------------------------------------------------------
+// Shared pages with many rows, on the 5th-generation tensor cores: the same partial results as attn_span_kernel<SP_ITEM>.
+//
+// A block takes 128 or 256 rows of an item (members x query heads, whatever their places in q) as one or two tiles and walks
+// the item's pages.  One warp feeds key and value pages by TMA through two rings; each tile has a thread of its own that issues
+// tcgen05.mma: scores S = Q K^T (M 128, N 64) into one of two buffers in tensor memory, two pages ahead of the rows, and O += P V
+// (M 128, N = head size, the weights read from tensor memory where their scores were, the values MN-major as the cache holds
+// them).  Four warps a tile own a row a thread: no shuffles for maximum and sum.  The output in tensor memory is rescaled only
+// when a row's maximum has grown by 2^8.  All pages are seen whole, so there is no mask but for a caller whose sequences end inside.
+// Bound by the issue of the products (12 a page of 64 keys at a head size of 128) beside the powers, and by memory where one tile holds
+// all rows.  Waits are bounded; a block whose wait runs out records it, frees its tensor memory and returns.
+// ---------------------------------------------------------------------------
+#if SP_HD <= 128
+#define ST_BM 128
+#define ST_THREADS(NT) ((NT) * 160 + 32)
+#define ST_TMEM_COLS(NT) (256 * (NT))
+// pieces of the head size for queries and keys: widths 64, 64, 32, 16 as far as they fit
+struct StSeg { int off, width; };
+__host__ __device__ constexpr int st_nseg() { return (SP_HD / 64) + ((SP_HD % 64) >= 32 ? 1 : 0) + ((SP_HD % 32) >= 16 ? 1 : 0); }
+__host__ __device__ constexpr StSeg st_seg(int i) {
+    int off = 0, idx = 0;
+    for (int k = 0; k < SP_HD / 64; ++k) { if (idx == i) return StSeg{off, 64}; off += 64; ++idx; }
+    if ((SP_HD % 64) >= 32) { if (idx == i) return StSeg{off, 32}; off += 32; ++idx; }
+    if ((SP_HD % 32) >= 16) { if (idx == i) return StSeg{off, 16}; off += 16; ++idx; }
+    return StSeg{0, 0};
+}
+__host__ __device__ constexpr int st_seg_base(int i, int rows) {
+    int b = 0;
+    for (int k = 0; k < i; ++k) b += ((rows * st_seg(k).width * 2 + 1023) / 1024) * 1024;
+    return b;
+}
+#define ST_NSEG st_nseg()
+#define ST_Q_BYTES st_seg_base(ST_NSEG, ST_BM)
+#define ST_K_BYTES st_seg_base(ST_NSEG, GL_PAGE)
+#define ST_VATOMS ((SP_HD + 63) / 64)
+#define ST_VATOM_BYTES (GL_PAGE * 128)
+#define ST_V_BYTES (ST_VATOMS * ST_VATOM_BYTES)
+// pages in flight: with one tile no more than leaves room on the SM for a block that walks own pages beside it
+__host__ __device__ constexpr int st_stages(int nt) {
+    const int n = ((nt == 2 ? 224 * 1024 : 144 * 1024) - nt * ST_Q_BYTES) / (ST_K_BYTES + ST_V_BYTES);
+    return n > 8 ? 8 : n;
+}
+static_assert(st_stages(2) >= 3 && st_stages(1) >= 3, "shared memory holds too few pages");
+struct StMaps { CUtensorMap k[4], v; };
+
+template <int NT>
+__global__ void __launch_bounds__(ST_THREADS(NT), 1)
+shared_tc_kernel(SpanArgs a, const __grid_constant__ StMaps maps) {
+    extern __shared__ unsigned char smem_raw[];
+    __shared__ unsigned tmem_slot;
+    __shared__ volatile int failed;
+    unsigned char* smem = smem_raw + ((1024u - (gl_smem_u32(smem_raw) & 1023u)) & 1023u);
+    constexpr int STAGES = st_stages(NT), PRODUCER = 4 * NT;
+    const unsigned base = gl_smem_u32(smem);
+    const unsigned sQ = base, sK = sQ + NT * ST_Q_BYTES, sV = sK + STAGES * ST_K_BYTES, bars = sV + STAGES * ST_V_BYTES;
+    const unsigned bar_kf = bars, bar_ke = bar_kf + 8 * STAGES, bar_vf = bar_ke + 8 * STAGES, bar_ve = bar_vf + 8 * STAGES;
+    const unsigned bar_t = bar_ve + 8 * STAGES;            // per tile: scores full [2], weights full [2], product done, output full, queries there
+#define ST_SF(t, i) (bar_t + 64 * (t) + 8 * (i))
+#define ST_PF(t, i) (bar_t + 64 * (t) + 16 + 8 * (i))
+#define ST_PD(t) (bar_t + 64 * (t) + 32)
+#define ST_OF(t) (bar_t + 64 * (t) + 40)
+#define ST_QF(t) (bar_t + 64 * (t) + 48)
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        failed = 0;
+        for (int s = 0; s < STAGES; ++s) {
+            mbar_init(bar_kf + 8 * s, 1); mbar_init(bar_ke + 8 * s, NT);
+            mbar_init(bar_vf + 8 * s, 1); mbar_init(bar_ve + 8 * s, NT);
+        }
+        for (int t = 0; t < NT; ++t) {
+            for (int i = 0; i < 2; ++i) { mbar_init(ST_SF(t, i), 1); mbar_init(ST_PF(t, i), 4); }
+            mbar_init(ST_PD(t), 1); mbar_init(ST_OF(t), 1); mbar_init(ST_QF(t), 4);
+        }
+        mbar_fence_init();
+    }
+    if (warp == PRODUCER) tmem_alloc(gl_smem_u32(&tmem_slot), ST_TMEM_COLS(NT));
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const unsigned tmem = tmem_slot;
+    gl_grid_wait();                                        // (then the next kernel may start: all before both is complete)
+    gl_grid_launch_dependents();
+
+    const int* it = a.items + 6 * blockIdx.x;
+    const int g = blockIdx.y, first = it[1], rows_all = it[2], p_begin = it[3], n = it[4] - it[3], slot = it[5];
+    const int* members = a.order + it[0];
+    const int G = a.nH / a.nKV;
+    // tile t: score buffers at columns 256 t and 256 t + 64 (a page's weights overwrite the first 32 columns of its scores, two a
+    // column), output at 256 t + 128.  A second tile without rows takes no part.
+    const int tiles = rows_all > ST_BM ? 2 : 1;
+
+    if (warp == PRODUCER) {
+        if (lane == 0) {
+            const int* pg = a.pages + (size_t)members[0] * a.max_pages + p_begin;
+            for (int j = 0; j < n && !failed; ++j) {
+                const int st = j % STAGES;
+                const unsigned par = ((j / STAGES) - 1) & 1;
+                const int row = (gl_checked(pg[j], a.n_pages, GL_BAD_PAGE) * a.nKV + g) * GL_PAGE;
+                if (j >= STAGES && !mbar_wait(bar_ke + 8 * st, par)) { failed = 1; break; }
+                mbar_expect_tx(bar_kf + 8 * st, GL_PAGE * SP_HD * 2);
+#pragma unroll
+                for (int s = 0; s < ST_NSEG; ++s)
+                    tma_load_2d(sK + st * ST_K_BYTES + st_seg_base(s, GL_PAGE), &maps.k[s], st_seg(s).off, row, bar_kf + 8 * st);
+                if (j >= STAGES && !mbar_wait(bar_ve + 8 * st, par)) { failed = 1; break; }
+                mbar_expect_tx(bar_vf + 8 * st, ST_V_BYTES);                       // zero fill counts
+#pragma unroll
+                for (int c = 0; c < ST_VATOMS; ++c)
+                    tma_load_2d(sV + st * ST_V_BYTES + c * ST_VATOM_BYTES, &maps.v, 64 * c, row, bar_vf + 8 * st);
+            }
+        }
+    } else if (warp > PRODUCER) {
+        if (lane == 0) {
+            constexpr uint32_t idesc_s = umma_idesc_bf16(GL_PAGE, 0);
+            constexpr uint32_t idesc_o = umma_idesc_bf16(SP_HD, 1);
+            const int t = warp - PRODUCER - 1, nt = t < tiles ? n : 0;
+            auto issue_scores = [&](int j) {
+                const int st = j % STAGES;
+                bool begin = true;
+#pragma unroll
+                for (int s = 0; s < ST_NSEG; ++s) {
+                    const int rb = st_seg(s).width * 2;
+                    const uint64_t dq = umma_tile_desc(sQ + t * ST_Q_BYTES + st_seg_base(s, ST_BM), rb);
+                    const uint64_t dk = umma_tile_desc(sK + st * ST_K_BYTES + st_seg_base(s, GL_PAGE), rb);
+#pragma unroll
+                    for (int k = 0; k < st_seg(s).width / 16; ++k) {
+                        umma_bf16(tmem + 256 * t + 64 * (j & 1), dq + 2 * k, dk + 2 * k, idesc_s, begin ? 0u : 1u);
+                        begin = false;
+                    }
+                }
+                umma_commit(ST_SF(t, j & 1));
+                umma_commit(bar_ke + 8 * st);
+            };
+            bool ok = nt == 0 || mbar_wait(ST_QF(t), 0);
+            for (int j = 0; ok && j < 2 && j < nt; ++j) {
+                ok = mbar_wait(bar_kf + 8 * (j % STAGES), (j / STAGES) & 1);
+                if (ok) { tc_fence_after(); issue_scores(j); }
+            }
+            for (int j = 0; ok && j < nt && !failed; ++j) {
+                const int st = j % STAGES;
+                ok = mbar_wait(ST_PF(t, j & 1), (j >> 1) & 1) && mbar_wait(bar_vf + 8 * st, (j / STAGES) & 1);
+                if (!ok) break;
+                tc_fence_after();
+                const uint64_t dv = umma_smem_desc(sV + st * ST_V_BYTES, ST_VATOM_BYTES, 1024, 2);
+#pragma unroll
+                for (int k = 0; k < GL_PAGE / 16; ++k)
+                    umma_bf16_tmem_a(tmem + 256 * t + 128, tmem + 256 * t + 64 * (j & 1) + 8 * k, dv + (uint64_t)((16 * 128) >> 4) * k, idesc_o, (j | k) ? 1u : 0u);
+                umma_commit(ST_PD(t));
+                if (j == nt - 1) umma_commit(ST_OF(t));
+                umma_commit(bar_ve + 8 * st);
+                if (j + 2 < nt) {                          // over S_j and P_j, which the rows and the product above are done with
+                    ok = mbar_wait(bar_kf + 8 * ((j + 2) % STAGES), ((j + 2) / STAGES) & 1);
+                    if (!ok) break;
+                    tc_fence_after();
+                    issue_scores(j + 2);
+                }
+            }
+            // a tile without rows still hands every page back, once it has been loaded
+            for (int j = nt; ok && j < n && !failed; ++j) {
+                const int st = j % STAGES;
+                ok = mbar_wait(bar_kf + 8 * st, (j / STAGES) & 1);
+                if (ok) mbar_arrive(bar_ke + 8 * st);
+                ok = ok && mbar_wait(bar_vf + 8 * st, (j / STAGES) & 1);
+                if (ok) mbar_arrive(bar_ve + 8 * st);
+            }
+            if (!ok) failed = 1;
+        }
+    } else if ((warp >> 2) < tiles) {
+        const int t = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane, row = t * ST_BM + r;
+        const bool real = row < rows_all;
+        const int b = real ? members[(first + row) / G] : -1, h = g * G + (first + row) % G;
+        const int last = real ? a.seq_ctx[b] : 0x7fffffff;
+        {   // this row's query into the tile, in the order that the products read it (16-byte pieces turned by the row)
+            const uint4* src = (const uint4*)(a.q + ((size_t)(real ? b : 0) * a.nH + (real ? h : 0)) * SP_HD);
+#pragma unroll
+            for (int s = 0; s < ST_NSEG; ++s) {
+                const int rb = st_seg(s).width * 2, pieces = rb / 16;
+                unsigned char* dst = smem + t * ST_Q_BYTES + st_seg_base(s, ST_BM) + r * rb;
+                const int turn = ((r * rb) >> 7) & (pieces - 1);
+#pragma unroll
+                for (int c = 0; c < pieces; ++c)
+                    *(uint4*)(dst + ((c ^ turn) << 4)) = real ? src[st_seg(s).off / 8 + c] : make_uint4(0, 0, 0, 0);
+            }
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(ST_QF(t));
+        }
+        const unsigned lane_off = (unsigned)(quarter * 32) << 16;
+        const unsigned tS = tmem + 256 * t + lane_off, tO = tS + 128;
+        float m_run = -INFINITY, l_run = 0.f;              // (the maximum as a power of two, as of the last rescaling)
+        bool alive = true;
+        for (int j = 0; j < n; ++j) {
+            bool ok = mbar_wait(ST_SF(t, j & 1), (j >> 1) & 1);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) { failed = 1; alive = false; break; }
+            tc_fence_after();
+            float sc[GL_PAGE];
+            {
+                unsigned (&su)[GL_PAGE] = reinterpret_cast<unsigned (&)[GL_PAGE]>(sc);
+                tmem_ld32_issue(tS + 64 * (j & 1), *reinterpret_cast<unsigned (*)[32]>(&su[0]));
+                tmem_ld32_issue(tS + 64 * (j & 1) + 32, *reinterpret_cast<unsigned (*)[32]>(&su[32]));
+                tmem_ld_wait();
+            }
+            const int j0 = (p_begin + j) * GL_PAGE;
+            if (j0 + GL_PAGE - 1 > last) {
+#pragma unroll
+                for (int i = 0; i < GL_PAGE; ++i)
+                    if (j0 + i > last) sc[i] = -INFINITY;
+            }
+            float mx8[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) mx8[i] = sc[i];
+#pragma unroll
+            for (int i = 8; i < GL_PAGE; i += 8)
+#pragma unroll
+                for (int k = 0; k < 8; ++k) mx8[k] = fmaxf(mx8[k], sc[i + k]);
+            const float mx = fmaxf(fmaxf(fmaxf(mx8[0], mx8[1]), fmaxf(mx8[2], mx8[3])), fmaxf(fmaxf(mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7])));
+            const float m_new = fmaxf(m_run, mx * SP_LOG2E);
+            const bool rescale = __any_sync(0xffffffffu, m_new - m_run > 8.f);      // (-inf to finite: yes; -inf to -inf: no)
+            float corr = 1.f;
+            if (rescale && m_new != -INFINITY) {
+                corr = sp_exp2(m_run - m_new);
+                m_run = m_new;
+            }
+            const float mu = m_run == -INFINITY ? 0.f : m_run;
+            if (rescale && j >= 1) {
+                ok = mbar_wait(ST_PD(t), (j - 1) & 1);     // the products so far are complete
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) { failed = 1; alive = false; break; }
+                tc_fence_after();
+#pragma unroll
+                for (int c = 0; c < SP_HD; c += 16) {
+                    unsigned t16[16];
+                    tmem_ld16(tO + c, t16);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) t16[i] = __float_as_uint(__uint_as_float(t16[i]) * corr);
+                    tmem_st16(tO + c, t16);
+                }
+            }
+            float ps4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < GL_PAGE; c += 32) {
+                unsigned pk[16];
+#pragma unroll
+                for (int i = 0; i < 32; i += 4) {
+                    const float e0 = sp_exp2(fmaf(sc[c + i], SP_LOG2E, -mu)), e1 = sp_exp2(fmaf(sc[c + i + 1], SP_LOG2E, -mu));
+                    const float e2 = sp_exp2(fmaf(sc[c + i + 2], SP_LOG2E, -mu)), e3 = sp_exp2(fmaf(sc[c + i + 3], SP_LOG2E, -mu));
+                    ps4[0] += e0; ps4[1] += e1; ps4[2] += e2; ps4[3] += e3;
+                    __nv_bfloat162 p0 = __floats2bfloat162_rn(e0, e1), p1 = __floats2bfloat162_rn(e2, e3);
+                    pk[i / 2] = *(unsigned*)&p0; pk[i / 2 + 1] = *(unsigned*)&p1;
+                }
+                tmem_st16(tS + 64 * (j & 1) + c / 2, pk);
+            }
+            l_run = l_run * corr + ((ps4[0] + ps4[1]) + (ps4[2] + ps4[3]));
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(ST_PF(t, j & 1));
+        }
+        if (alive) {
+            bool ok = mbar_wait(ST_OF(t), 0);
+            ok = __all_sync(0xffffffffu, ok);
+            if (ok) {
+                tc_fence_after();
+                const size_t at = ((size_t)(real ? b : 0) * a.nH + h) * a.slots + slot;
+#pragma unroll
+                for (int c = 0; c < SP_HD; c += 16) {
+                    unsigned t16[16];
+                    tmem_ld16(tO + c, t16);
+                    if (real)
+#pragma unroll
+                        for (int i = 0; i < 16; i += 4)
+                            *(uint4*)(a.part_o + at * SP_HD + c + i) = make_uint4(t16[i], t16[i + 1], t16[i + 2], t16[i + 3]);
+                }
+                if (real) { a.part_ml[at * 2] = m_run; a.part_ml[at * 2 + 1] = l_run; }
+            } else {
+                failed = 1;
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == PRODUCER) {
+        tc_fence_after();
+        tmem_dealloc(tmem, ST_TMEM_COLS(NT));
+    }
+    if (threadIdx.x == 0 && failed) atomicExch(&gl_wait_failed, 1);
+}
+
+template <int NT>
+static int launch_shared_tc(const SpanArgs& a, const StMaps& maps, cudaStream_t stream) {
+    static bool allowed[64] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) { cudaGetLastError(); return GL_ERR_DRIVER; }
+    const size_t smem = NT * (size_t)ST_Q_BYTES + st_stages(NT) * ((size_t)ST_K_BYTES + ST_V_BYTES) + 32 * st_stages(NT) + 64 * NT + 1024;
+    if (!allowed[dev]) {
+        if (cudaFuncSetAttribute(shared_tc_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) {
+            cudaGetLastError();
+            return GL_ERR_SMEM;
+        }
+        allowed[dev] = true;
+    }
+    return gl_launch(shared_tc_kernel<NT>, dim3(a.n_items, a.nKV), dim3(ST_THREADS(NT)), smem, stream, 1, a, maps);
+}
+static int shared_tc(const SpanArgs& a, int rows, cudaStream_t stream) {
+    if (rows > 2 * ST_BM) return GL_ERR_SHAPE;
+    StMaps maps;
+    const uint64_t kv_rows = (uint64_t)a.n_pages * a.nKV * GL_PAGE;
+    if (kv_rows > 0x7fffffffULL) return GL_ERR_SHAPE;      // (a row's number is a coordinate)
+    for (int s = 0; s < ST_NSEG; ++s) {
+        const int rc = gl_cached_map(&maps.k[s], a.k_cache, kv_rows, SP_HD, GL_PAGE, st_seg(s).width, 2);
+        if (rc != GL_OK) return rc;
+    }
+    const int rc = gl_cached_map(&maps.v, a.v_cache, kv_rows, SP_HD, GL_PAGE, 64, 2);       // what a box has beyond the head size reads as zero
+    if (rc != GL_OK) return rc;
+    return rows > ST_BM ? launch_shared_tc<2>(a, maps, stream) : launch_shared_tc<1>(a, maps, stream);
+}
+#else
+static int shared_tc(const SpanArgs&, int, cudaStream_t) { return GL_ERR_SHAPE; }
+#endif
 
 // ---------------------------------------------------------------------------
 // Runs of several tokens: the weights their positions are given.  The attention itself is the prefill kernels'; what it does

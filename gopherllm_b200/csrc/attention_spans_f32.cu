@@ -9,6 +9,8 @@
 // Runs of several tokens take rows of consecutive queries; a second kernel then walks the cache page by page, multiplies its
 // keys with all the rows that see them and adds up e^(s - m) / l.  No sum depends on the order in which blocks run.
 #include "common.cuh"
+#include <cooperative_groups.h>
+namespace cg = cooperative_groups;
 
 #define SF_THREADS 128
 #define SF_MAX_HD 256
@@ -30,6 +32,7 @@ struct SpanF32Args {
     float* scores;                // [B, nH, reach] or null
     float* weights;               // [pages, nKV, GL_PAGE] or null
     int B, nH, nKV, max_pages, n_pages, n_items, splits, slots, chunks, reach, hd, last;
+    int early, held, joined;      // set by the launchers
 };
 
 enum { SF_OWN = 0, SF_SHARED = 1, SF_RUN = 2 };
@@ -261,48 +264,323 @@ span_f32_kernel(SpanF32Args a) {
     }
 }
 
-// The spans of a row put together: blockIdx = (head, sequence).
-__global__ void span_f32_join_kernel(SpanF32Args a) {
-    gl_grid_launch_dependents();
+// The spans of a sequence put together, as in attention_spans.cu: blockIdx = (share of the positions, key/value head, sequence).
+#define SF_JOIN_THREADS 256
+__global__ void __launch_bounds__(SF_JOIN_THREADS)
+span_f32_join_kernel(SpanF32Args a) {
+    extern __shared__ __align__(16) float sf[];                    // [G][2]: maximum, sum
+    const int b = blockIdx.z, g = blockIdx.y, G = a.nH / a.nKV, tid = threadIdx.x, lane = tid & 31;
     gl_grid_wait();
-    const int h = blockIdx.x, b = blockIdx.y;
+    gl_grid_launch_dependents();
     if (a.seq_qlen && a.seq_qlen[b] <= 0) return;
     const int n = (a.seq_shared ? a.seq_shared[2 * b + 1] : 0) + a.splits;
-    const size_t at = ((size_t)b * a.nH + h) * a.slots;
-    const float* ml = a.part_ml + at * 2;
-    float m = -INFINITY;
-    for (int s = 0; s < n; ++s) m = fmaxf(m, ml[2 * s]);
-    float* out = a.out + ((size_t)(a.seq_row ? a.seq_row[b] : b) * a.nH + h) * a.hd;
-    for (int d = threadIdx.x; d < a.hd; d += blockDim.x) {
-        float o = 0.f, l = 0.f;
-        for (int s = 0; s < n; ++s) {
-            const float f = sf_factor(ml[2 * s], m);
-            o = fmaf(f, a.part_o[(at + s) * a.hd + d], o);
-            l = fmaf(f, ml[2 * s + 1], l);
+    for (int i = tid >> 5; i < G; i += SF_JOIN_THREADS / 32) {
+        const float* ml = a.part_ml + ((size_t)b * a.nH + g * G + i) * a.slots * 2;
+        float m = -INFINITY, l = 0.f;
+        for (int s = lane; s < n; s += 32) m = fmaxf(m, ml[2 * s]);
+        m = gl_warp_max(m);
+        for (int s = lane; s < n; s += 32) l = fmaf(sf_factor(ml[2 * s], m), ml[2 * s + 1], l);
+        l = gl_warp_sum(l);
+        if (lane == 0) { sf[2 * i] = m; sf[2 * i + 1] = l; }
+    }
+    __syncthreads();
+    for (int i = blockIdx.x; i < G; i += gridDim.x) {
+        const size_t at = ((size_t)b * a.nH + g * G + i) * a.slots;
+        const float m = sf[2 * i], l = sf[2 * i + 1];
+        for (int d = tid; d < a.hd; d += SF_JOIN_THREADS) {
+            float o = 0.f;
+#pragma unroll 4
+            for (int s = 0; s < n; ++s) o = fmaf(sf_factor(a.part_ml[(at + s) * 2], m), a.part_o[(at + s) * a.hd + d], o);
+            a.out[((size_t)(a.seq_row ? a.seq_row[b] : b) * a.nH + g * G + i) * a.hd + d] = l == 0.f ? 0.f : o / l;
         }
-        out[d] = l == 0.f ? 0.f : o / l;
+    }
+    if (!a.weights) return;
+    const int pos = a.seq_ctx[b], most = min(pos + 1, a.reach);
+    for (int j = blockIdx.x * SF_JOIN_THREADS + tid; j < most; j += gridDim.x * SF_JOIN_THREADS) {
+        const float* sc = a.scores + ((size_t)b * a.nH + g * G) * a.reach + j;
+        float given = 0.f;
+#pragma unroll 4
+        for (int i = 0; i < G; ++i) given += expf(sc[(size_t)i * a.reach] - sf[2 * i]) / sf[2 * i + 1];
+        float* w = a.weights + ((size_t)gl_checked(a.pages[(size_t)b * a.max_pages + j / GL_PAGE], a.n_pages, GL_BAD_PAGE) * a.nKV + g) * GL_PAGE + j % GL_PAGE;
+        *w = j < pos ? *w + given : given;
     }
 }
 
-// One token a sequence: the scores written down become weights, added up over the query heads of a key/value head.
-__global__ void __launch_bounds__(GL_PAGE)
-span_f32_weigh_kernel(SpanF32Args a) {
-    gl_grid_launch_dependents();
-    gl_grid_wait();
-    const int b = blockIdx.z, g = blockIdx.y, p = blockIdx.x, G = a.nH / a.nKV;
-    const int pos = a.seq_ctx[b], j = p * GL_PAGE + threadIdx.x;
-    if ((a.seq_qlen && a.seq_qlen[b] <= 0) || p > pos / GL_PAGE) return;
-    float given = 0.f;
-    for (int h = g * G; h < (g + 1) * G; ++h) {
-        const float* ml = a.part_ml + ((size_t)b * a.nH + h) * a.slots * 2;
-        float m = -INFINITY, l = 0.f;
-        for (int s = 0; s < a.splits; ++s) m = fmaxf(m, ml[2 * s]);
-        for (int s = 0; s < a.splits; ++s) l = fmaf(sf_factor(ml[2 * s], m), ml[2 * s + 1], l);
-        if (j <= pos && j < a.reach) given += expf(a.scores[((size_t)b * a.nH + h) * a.reach + j] - m) / l;
+// ---------------------------------------------------------------------------
+// Heads of whole 16-byte pieces: keys and values go from the cache straight to registers.  Eight lanes take a key (a lane CP pieces of it),
+// so a warp takes four at a time and has 2 UN of their pieces' rows under way; no barrier stands between two keys.  With R rows
+// the eight lanes' shares of R products are added up and dealt out in one exchange, so that a lane ends with the whole score of
+// row ``lane mod R`` and takes its power alone.  Each of a warp's four groups of lanes has a softmax of its own; they meet at the end of
+// the span, then the warps, then the blocks of a cluster (as in attention_spans.cu).
+// ---------------------------------------------------------------------------
+#define ST_WARPS 4
+// loads that stay behind the wait before them (what another kernel wrote meanwhile)
+__device__ __forceinline__ float2 st_read(const float2* p) {
+    float2 v;
+    asm volatile("ld.global.cg.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "l"(p) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 st_read(const float4* p) {
+    float4 v;
+    asm volatile("ld.global.cg.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p) : "memory");
+    return v;
+}
+// the sum over the group's eight lanes of v[r], r = lane mod R, in every lane
+template <int R>
+__device__ __forceinline__ float st_deal(float (&v)[R], int lane) {
+    int n = R;
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) {
+        if (n > 1) {                                               // hand over half the rows, take the partner's share of the other half
+            n >>= 1;
+            const bool up = lane & n;
+#pragma unroll
+            for (int i = 0; i < R / 2; ++i)
+                if (i < n) {
+                    const float give = up ? v[i] : v[i + n];
+                    v[i] = (up ? v[i + n] : v[i]) + __shfl_xor_sync(0xffffffffu, give, n);
+                }
+        } else {
+            v[0] += __shfl_xor_sync(0xffffffffu, v[0], o == 4 ? 4 : (R == 2 ? 2 * o : R == 4 ? 4 : o));
+        }
     }
-    if (j > pos || j >= a.reach) return;
-    float* w = a.weights + ((size_t)gl_checked(a.pages[(size_t)b * a.max_pages + p], a.n_pages, GL_BAD_PAGE) * a.nKV + g) * GL_PAGE + threadIdx.x;
-    *w = j < pos ? *w + given : given;
+    return v[0];
+}
+
+template <int CP, int R, int MODE>
+__global__ void __launch_bounds__(32 * ST_WARPS)
+stream_f32_kernel(SpanF32Args a) {
+    extern __shared__ __align__(16) float sf[];
+    constexpr int UN = CP * R <= 4 ? 4 : 2;                        // keys of a group under way
+    const int hd = a.hd, G = a.nH / a.nKV, pieces = hd >> 2;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, sub = lane & 7, grp = lane >> 3;
+    // shared memory: what the warps found [4][R][hd], [4][R][2]; the block's result [R][hd], [R][2]; scores kept; factors of the parts
+    float* o_w = sf;
+    float* ml_w = o_w + ST_WARPS * R * hd;
+    float* fin_o = ml_w + ST_WARPS * R * 2;
+    float* fin_ml = fin_o + R * hd;
+    float* held = fin_ml + 2 * R;
+    if (!a.early) gl_grid_wait();
+    gl_grid_launch_dependents();
+
+    int g, rows, p_begin, p_end, slot, table;
+    int seq[R], head[R], least = 0x7fffffff;
+    if (MODE == SF_SHARED) {
+        const int* it = a.items + 6 * blockIdx.x;
+        g = blockIdx.y;
+        rows = it[2]; p_begin = it[3]; p_end = it[4]; slot = it[5];
+        table = a.order[it[0]];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int i = it[1] + min(r, rows - 1);
+            seq[r] = a.order[it[0] + i / G];
+            head[r] = g * G + i % G;
+            least = min(least, a.seq_ctx[seq[r]]);
+        }
+    } else {
+        const int b = blockIdx.z;
+        g = blockIdx.y / a.chunks;
+        if (a.seq_qlen && a.seq_qlen[b] <= 0) return;
+        const int per_chunk = (G + a.chunks - 1) / a.chunks, h0 = (blockIdx.y - g * a.chunks) * per_chunk;
+        rows = min(per_chunk, G - h0);
+        const int pos = a.seq_ctx[b], first = a.seq_shared ? a.seq_shared[2 * b] : 0;
+        const int n = max(0, pos / GL_PAGE + 1 - first), per = (n + a.splits - 1) / a.splits;
+        p_begin = first + (int)blockIdx.x * per;
+        p_end = min(first + n, p_begin + per);
+        slot = (a.seq_shared ? a.seq_shared[2 * b + 1] : 0) + blockIdx.x;
+        table = b;
+        least = pos;
+#pragma unroll
+        for (int r = 0; r < R; ++r) { seq[r] = b; head[r] = g * G + h0 + min(r, rows - 1); }
+    }
+    const int total = a.seq_ctx[table] + 1, mine = sub % R;        // mine: the row whose softmax this lane keeps
+    int last = least;
+    if (MODE == SF_SHARED) {
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+            if (r == mine) last = a.seq_ctx[seq[r]];
+    }
+    float q[R][CP * 4], o[R][CP * 4];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const float* src = a.q + ((size_t)(MODE != SF_SHARED && a.seq_row ? a.seq_row[seq[r]] : seq[r]) * a.nH + head[r]) * hd;
+#pragma unroll
+        for (int c = 0; c < CP; ++c) {
+            const float4 v = c * 8 + sub < pieces ? *(const float4*)(src + 4 * (c * 8 + sub)) : make_float4(0.f, 0.f, 0.f, 0.f);
+            q[r][4 * c] = v.x; q[r][4 * c + 1] = v.y; q[r][4 * c + 2] = v.z; q[r][4 * c + 3] = v.w;
+            o[r][4 * c] = o[r][4 * c + 1] = o[r][4 * c + 2] = o[r][4 * c + 3] = 0.f;
+        }
+    }
+    float m = -INFINITY, l = 0.f;                                  // of row ``mine`` over this group's keys
+    const int* pg = a.pages + (size_t)table * a.max_pages;
+    // warps take runs of 4 UN keys in turn, group by group of lanes
+    constexpr int RUN = 4 * UN;
+    const int k_end = min(p_end * GL_PAGE, MODE == SF_SHARED ? p_end * GL_PAGE : total);
+    for (int j0 = p_begin * GL_PAGE + warp * RUN; j0 < k_end; j0 += ST_WARPS * RUN) {
+        const size_t at = (((size_t)gl_checked(pg[j0 / GL_PAGE], a.n_pages, GL_BAD_PAGE) * a.nKV + g) * GL_PAGE + j0 % GL_PAGE) * hd;
+        float4 k[UN][CP], v[UN][CP];
+#pragma unroll
+        for (int u = 0; u < UN; ++u)
+#pragma unroll
+            for (int c = 0; c < CP; ++c) {
+                const bool ok = j0 + 4 * u + grp < k_end && c * 8 + sub < pieces;
+                const size_t off = at + (size_t)(4 * u + grp) * hd + 4 * (c * 8 + sub);
+                k[u][c] = ok ? *(const float4*)(a.k_cache + off) : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+#pragma unroll
+        for (int u = 0; u < UN; ++u)
+#pragma unroll
+            for (int c = 0; c < CP; ++c) {
+                const bool ok = j0 + 4 * u + grp < k_end && c * 8 + sub < pieces;
+                const size_t off = at + (size_t)(4 * u + grp) * hd + 4 * (c * 8 + sub);
+                v[u][c] = ok ? *(const float4*)(a.v_cache + off) : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+        float s[UN], m_new = m;
+#pragma unroll
+        for (int u = 0; u < UN; ++u) {
+            float part[R];
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                float x = 0.f;
+#pragma unroll
+                for (int c = 0; c < CP; ++c)
+                    x = fmaf(k[u][c].x, q[r][4 * c], fmaf(k[u][c].y, q[r][4 * c + 1], fmaf(k[u][c].z, q[r][4 * c + 2], fmaf(k[u][c].w, q[r][4 * c + 3], x))));
+                part[r] = x;
+            }
+            s[u] = st_deal<R>(part, lane);
+            const int j = j0 + 4 * u + grp;
+            if (MODE == SF_OWN && a.weights && sub < rows && j < k_end) {
+                if (!a.scores) { if (j - p_begin * GL_PAGE < a.held) held[sub * a.held + j - p_begin * GL_PAGE] = s[u]; }
+                else if (j < a.reach) {
+#pragma unroll
+                    for (int r = 0; r < R; ++r)
+                        if (r == sub) a.scores[((size_t)table * a.nH + head[r]) * a.reach + j] = s[u];
+                }
+            }
+            if (j >= k_end || j > last) s[u] = -INFINITY;
+            m_new = fmaxf(m_new, s[u]);
+        }
+        const float mu = m_new == -INFINITY ? 0.f : m_new, corr = sf_factor(m, m_new);
+        l *= corr;
+#pragma unroll
+        for (int u = 0; u < UN; ++u) { s[u] = expf(s[u] - mu); l += s[u]; }
+        if (__any_sync(0xffffffffu, m != m_new)) {
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const float c = __shfl_sync(0xffffffffu, corr, (lane & 24) + r);
+#pragma unroll
+                for (int i = 0; i < CP * 4; ++i) o[r][i] *= c;
+            }
+        }
+        m = m_new;
+#pragma unroll
+        for (int u = 0; u < UN; ++u)
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const float w = __shfl_sync(0xffffffffu, s[u], (lane & 24) + r);
+#pragma unroll
+                for (int c = 0; c < CP; ++c) {
+                    o[r][4 * c] = fmaf(w, v[u][c].x, o[r][4 * c]); o[r][4 * c + 1] = fmaf(w, v[u][c].y, o[r][4 * c + 1]);
+                    o[r][4 * c + 2] = fmaf(w, v[u][c].z, o[r][4 * c + 2]); o[r][4 * c + 3] = fmaf(w, v[u][c].w, o[r][4 * c + 3]);
+                }
+            }
+    }
+    // the warp's four groups
+#pragma unroll
+    for (int x = 8; x < 32; x <<= 1) {
+        const float om = __shfl_xor_sync(0xffffffffu, m, x), ol = __shfl_xor_sync(0xffffffffu, l, x), m_new = fmaxf(m, om);
+        const float f = sf_factor(m, m_new), of = sf_factor(om, m_new);
+        l = l * f + ol * of;
+        m = m_new;
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const float fr = __shfl_sync(0xffffffffu, f, (lane & 24) + r), ofr = __shfl_sync(0xffffffffu, of, (lane & 24) + r);
+#pragma unroll
+            for (int i = 0; i < CP * 4; ++i) o[r][i] = o[r][i] * fr + __shfl_xor_sync(0xffffffffu, o[r][i], x) * ofr;
+        }
+    }
+    if (lane < R) { ml_w[(warp * R + lane) * 2] = m; ml_w[(warp * R + lane) * 2 + 1] = l; }
+    if (grp == 0)
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int c = 0; c < CP; ++c)
+                if (c * 8 + sub < pieces)
+                    *(float4*)(o_w + (warp * R + r) * hd + 4 * (c * 8 + sub)) = make_float4(o[r][4 * c], o[r][4 * c + 1], o[r][4 * c + 2], o[r][4 * c + 3]);
+    __syncthreads();
+    const bool join = MODE == SF_OWN && a.joined;
+    for (int i = tid; i < rows * pieces; i += 32 * ST_WARPS) {
+        const int r = i / pieces, c = i - r * pieces;
+        float mm = -INFINITY, ll = 0.f;
+#pragma unroll
+        for (int w = 0; w < ST_WARPS; ++w) mm = fmaxf(mm, ml_w[(w * R + r) * 2]);
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < ST_WARPS; ++w) {
+            const float f = sf_factor(ml_w[(w * R + r) * 2], mm);
+            const float4 x = *(const float4*)(o_w + (w * R + r) * hd + 4 * c);
+            sum.x = fmaf(f, x.x, sum.x); sum.y = fmaf(f, x.y, sum.y); sum.z = fmaf(f, x.z, sum.z); sum.w = fmaf(f, x.w, sum.w);
+            ll = fmaf(f, ml_w[(w * R + r) * 2 + 1], ll);
+        }
+        int b = seq[0], h = head[0];
+#pragma unroll
+        for (int k = 1; k < R; ++k)
+            if (k == r) { b = seq[k]; h = head[k]; }
+        const size_t at = ((size_t)b * a.nH + h) * a.slots + slot;
+        *(float4*)(join ? fin_o + r * hd + 4 * c : a.part_o + at * hd + 4 * c) = sum;
+        if (c == 0) *(float2*)(join ? fin_ml + 2 * r : a.part_ml + at * 2) = make_float2(mm, ll);
+    }
+    if (!join) return;
+    // the blocks of the cluster, and what the shared pages gave
+    cg::cluster_group cluster = cg::this_cluster();
+    const int S = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+    const int b = table, n_pre = a.seq_shared ? a.seq_shared[2 * b + 1] : 0, parts = S + n_pre, h_first = head[0];
+    float* fac = held + (a.weights ? rows * a.held : 0);          // [rows][parts]: factor / sum
+    float* stat = ml_w;                                            // [rows][2]: maximum, 1 / sum
+    if (a.early) gl_grid_wait();
+    if (S > 1) cluster.sync();
+    else __syncthreads();
+    for (int r = warp; r < rows; r += ST_WARPS) {
+        const float2* pre = (const float2*)a.part_ml + ((size_t)b * a.nH + h_first + r) * a.slots - S;
+        auto part = [&](int k) { return k < S ? ((const float2*)(S > 1 ? cluster.map_shared_rank(fin_ml, k) : fin_ml))[r] : st_read(pre + k); };
+        float mm = -INFINITY, ll = 0.f;
+        for (int k = lane; k < parts; k += 32) mm = fmaxf(mm, part(k).x);
+        mm = gl_warp_max(mm);
+        for (int k = lane; k < parts; k += 32) {
+            const float2 ml = part(k);
+            const float f = sf_factor(ml.x, mm);
+            fac[r * parts + k] = f;
+            ll = fmaf(f, ml.y, ll);
+        }
+        ll = gl_warp_sum(ll);
+        if (lane == 0) { stat[2 * r] = mm; stat[2 * r + 1] = ll; }
+    }
+    __syncthreads();
+    for (int i = tid * S + rank; i < rows * pieces; i += 32 * ST_WARPS * S) {
+        const int r = i / pieces, c = i - r * pieces;
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+        auto add = [&](float f, const float4 x) {
+            sum.x = fmaf(f, x.x, sum.x); sum.y = fmaf(f, x.y, sum.y); sum.z = fmaf(f, x.z, sum.z); sum.w = fmaf(f, x.w, sum.w);
+        };
+        for (int k = 0; k < S; ++k) add(fac[r * parts + k], ((const float4*)(S > 1 ? cluster.map_shared_rank(fin_o, k) : fin_o))[i]);
+        const float4* pre = (const float4*)a.part_o + ((size_t)b * a.nH + h_first + r) * a.slots * pieces + c;
+#pragma unroll 8
+        for (int k = 0; k < n_pre; ++k) add(fac[r * parts + S + k], st_read(pre + (size_t)k * pieces));
+        const float ll = stat[2 * r + 1];
+        const float4 y = ll == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(sum.x / ll, sum.y / ll, sum.z / ll, sum.w / ll);
+        *(float4*)(a.out + ((size_t)(a.seq_row ? a.seq_row[b] : b) * a.nH + h_first + r) * hd + 4 * c) = y;
+    }
+    if (a.weights) {
+        const int n = min(min(p_end * GL_PAGE, total) - p_begin * GL_PAGE, a.held);
+        for (int i = tid; i < n; i += 32 * ST_WARPS) {
+            float given = 0.f;
+            for (int r = 0; r < rows; ++r) given += expf(held[r * a.held + i] - stat[2 * r]) / stat[2 * r + 1];
+            const int j = p_begin * GL_PAGE + i;
+            float* w = a.weights + ((size_t)gl_checked(pg[j / GL_PAGE], a.n_pages, GL_BAD_PAGE) * a.nKV + g) * GL_PAGE + j % GL_PAGE;
+            *w = j < total - 1 ? *w + given : given;
+        }
+    }
+    if (S > 1) cluster.sync();
 }
 
 // Runs: blockIdx = (page, key/value head, sequence); the page's keys against all rows of the run that see them.
@@ -376,59 +654,111 @@ static int launch_f32(const SpanF32Args& a, dim3 grid, cudaStream_t stream) {
     }
     return gl_launch(span_f32_kernel<R, KIND>, grid, dim3(SF_THREADS), sf_smem(a.hd), stream, 1, a);
 }
+// rows a block takes of heads of a given size, streaming: what the registers hold
+static int stream_rows(int hd) { return hd % 4 ? 8 : hd <= 64 ? 8 : hd <= 128 ? 4 : 2; }
+GL_API int gl_attention_span_rows_f32(int hd) { return stream_rows(hd); }
+
+#define ST_HELD_BYTES (56 * 1024)
+#define ST_FACTOR_BYTES (24 * 1024)
+template <int CP, int R, int KIND>
+static int launch_stream(const SpanF32Args& a, dim3 grid, int cluster, cudaStream_t stream) {
+    static bool allowed[64] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) { cudaGetLastError(); return GL_ERR_DRIVER; }
+    const size_t fixed = sizeof(float) * (ST_WARPS + 1) * R * (a.hd + 2);
+    if (!allowed[dev]) {
+        if (allow_smem(stream_f32_kernel<CP, R, KIND>, sizeof(float) * (ST_WARPS + 1) * R * (32 * CP + 2) + ST_HELD_BYTES + ST_FACTOR_BYTES) != GL_OK) return GL_ERR_SMEM;
+        allowed[dev] = true;
+    }
+    const size_t smem = fixed + (a.joined && KIND == SF_OWN ? sizeof(float) * ((a.weights ? (size_t)a.held * (a.nH / a.nKV) : 0) + R * (size_t)(a.slots + a.splits)) : 0);
+    return gl_launch(stream_f32_kernel<CP, R, KIND>, grid, dim3(32 * ST_WARPS), smem, stream, cluster, a);
+}
+template <int CP, int MOST, int KIND>
+static int launch_stream_rows(const SpanF32Args& a, int rows, dim3 grid, int cluster, cudaStream_t stream) {
+    if (rows <= 1) return launch_stream<CP, 1, KIND>(a, grid, cluster, stream);
+    if (rows <= 2) return launch_stream<CP, 2, KIND>(a, grid, cluster, stream);
+    if constexpr (MOST >= 4)
+        if (rows <= 4) return launch_stream<CP, 4, KIND>(a, grid, cluster, stream);
+    if constexpr (MOST >= 8)
+        if (rows <= 8) return launch_stream<CP, 8, KIND>(a, grid, cluster, stream);
+    return GL_ERR_SHAPE;
+}
 template <int KIND>
-static int launch_f32_rows(const SpanF32Args& a, int rows, dim3 grid, cudaStream_t stream) {
-    if (rows <= 1) return launch_f32<1, KIND>(a, grid, stream);
+static int launch_f32_rows(const SpanF32Args& a, int rows, dim3 grid, int cluster, cudaStream_t stream) {
+    if (a.hd % 4 == 0) {
+        if (a.hd <= 32) return launch_stream_rows<1, 8, KIND>(a, rows, grid, cluster, stream);
+        if (a.hd <= 64) return launch_stream_rows<2, 8, KIND>(a, rows, grid, cluster, stream);
+        if (a.hd <= 96) return launch_stream_rows<3, 4, KIND>(a, rows, grid, cluster, stream);
+        if (a.hd <= 128) return launch_stream_rows<4, 4, KIND>(a, rows, grid, cluster, stream);
+        if (a.hd <= 192) return launch_stream_rows<6, 2, KIND>(a, rows, grid, cluster, stream);
+        return launch_stream_rows<8, 2, KIND>(a, rows, grid, cluster, stream);
+    }
     if (rows <= 2) return launch_f32<2, KIND>(a, grid, stream);
-    if (rows <= 4) return launch_f32<4, KIND>(a, grid, stream);
     return launch_f32<8, KIND>(a, grid, stream);
 }
 
 static int f32_checked(const SpanF32Args& a) {
     if (a.nH <= 0 || a.nKV <= 0 || a.nH % a.nKV || a.nKV > 65535 || a.B > 65535 || a.hd <= 0 || a.hd > SF_MAX_HD || a.max_pages <= 0) return GL_ERR_SHAPE;
-    if ((((uintptr_t)a.k_cache | (uintptr_t)a.v_cache) & 15) && a.hd % 4 == 0) return GL_ERR_ALIGN;
-    return a.part_ml ? GL_OK : GL_ERR_SHAPE;
+    if ((((uintptr_t)a.q | (uintptr_t)a.out | (uintptr_t)a.k_cache | (uintptr_t)a.v_cache) & 15) && a.hd % 4 == 0) return GL_ERR_ALIGN;
+    return GL_OK;
 }
 static int f32_spans_checked(const SpanF32Args& a) {
     const int G = a.nH / a.nKV;
-    if (a.splits < 1 || a.slots < a.splits || !a.part_o) return GL_ERR_SHAPE;
-    if (a.chunks < 1 || a.chunks > G || (long long)a.nKV * a.chunks > 65535 || (G + a.chunks - 1) / a.chunks > 8) return GL_ERR_SHAPE;
+    if (a.splits < 1 || a.slots < 0 || (a.slots > 0 && (!a.part_o || !a.part_ml))) return GL_ERR_SHAPE;
+    if (a.chunks < 1 || a.chunks > G || (long long)a.nKV * a.chunks > 65535 || (G + a.chunks - 1) / a.chunks > stream_rows(a.hd)) return GL_ERR_SHAPE;
     return (a.chunks - 1) * ((G + a.chunks - 1) / a.chunks) >= G ? GL_ERR_SHAPE : GL_OK;
 }
+static int launch_join(const SpanF32Args& a, cudaStream_t stream) {
+    const int G = a.nH / a.nKV, shares = a.weights ? (a.reach + 4 * SF_JOIN_THREADS - 1) / (4 * SF_JOIN_THREADS) : 1;
+    return gl_launch(span_f32_join_kernel, dim3(shares > G ? shares : G, a.nKV, a.B), dim3(SF_JOIN_THREADS), 2 * G * sizeof(float), stream, 1, a);
+}
 
-GL_API int gl_attention_prefix_f32(const SpanF32Args* args, int rows, cudaStream_t stream) {
-    const SpanF32Args& a = *args;
+// rows, joined: as for gl_attention_prefix (joined: heads of whole 16-byte pieces only)
+GL_API int gl_attention_prefix_f32(const SpanF32Args* args, int rows, int joined, cudaStream_t stream) {
+    SpanF32Args a = *args;
     if (a.B <= 0) return GL_OK;
     int rc = f32_checked(a);
     if (rc == GL_OK) rc = f32_spans_checked(a);
     if (rc != GL_OK) return rc;
-    if (a.n_items < 0 || a.scores || a.weights || !a.seq_shared || (a.n_items > 0 && (!a.items || !a.order || rows < 1 || rows > 8))) return GL_ERR_SHAPE;
-    if (a.n_items > 0 && (rc = launch_f32_rows<SF_SHARED>(a, rows, dim3(a.n_items, a.nKV), stream)) != GL_OK) return rc;
-    const int G = a.nH / a.nKV;
-    if ((rc = launch_f32_rows<SF_OWN>(a, (G + a.chunks - 1) / a.chunks, dim3(a.splits, a.nKV * a.chunks, a.B), stream)) != GL_OK) return rc;
-    return gl_launch(span_f32_join_kernel, dim3(a.nH, a.B), dim3(a.hd >= 128 ? 128 : 64), 0, stream, 1, a);
+    if (a.n_items < 0 || a.scores || a.weights || !a.seq_shared || (a.n_items > 0 && (!a.items || !a.order || rows < 1 || rows > stream_rows(a.hd) || a.slots < 1))) return GL_ERR_SHAPE;
+    if (joined ? a.hd % 4 || a.splits > 8 || 8 * (long long)(a.slots + a.splits) * (int)sizeof(float) > ST_FACTOR_BYTES : a.slots < a.splits) return GL_ERR_SHAPE;
+    a.early = a.held = a.joined = 0;
+    if (a.n_items > 0 && (rc = launch_f32_rows<SF_SHARED>(a, rows, dim3(a.n_items, a.nKV), 1, stream)) != GL_OK) return rc;
+    const int G = a.nH / a.nKV, mine = (G + a.chunks - 1) / a.chunks;
+    a.joined = joined;
+    a.early = joined && a.n_items > 0 && gl_pdl;
+    rc = launch_f32_rows<SF_OWN>(a, mine, dim3(a.splits, a.nKV * a.chunks, a.B), joined ? a.splits : 1, stream);
+    return rc != GL_OK || joined ? rc : launch_join(a, stream);
 }
 
 GL_API int gl_attention_weighed_f32(const SpanF32Args* args, cudaStream_t stream) {
-    const SpanF32Args& a = *args;
+    SpanF32Args a = *args;
     if (a.B <= 0) return GL_OK;
     int rc = f32_checked(a);
     if (rc == GL_OK) rc = f32_spans_checked(a);
     if (rc != GL_OK) return rc;
-    if (!a.scores || !a.weights || a.seq_shared || a.reach <= 0) return GL_ERR_SHAPE;
+    if (!a.weights || a.seq_shared || a.reach <= 0) return GL_ERR_SHAPE;
     const int G = a.nH / a.nKV;
-    if ((rc = launch_f32_rows<SF_OWN>(a, (G + a.chunks - 1) / a.chunks, dim3(a.splits, a.nKV * a.chunks, a.B), stream)) != GL_OK) return rc;
-    if ((rc = gl_launch(span_f32_join_kernel, dim3(a.nH, a.B), dim3(a.hd >= 128 ? 128 : 64), 0, stream, 1, a)) != GL_OK) return rc;
-    return gl_launch(span_f32_weigh_kernel, dim3((a.reach + GL_PAGE - 1) / GL_PAGE, a.nKV, a.B), dim3(GL_PAGE), 0, stream, 1, a);
+    a.early = a.held = 0;
+    a.joined = !a.scores;
+    if (a.joined) {
+        a.held = ((a.reach + GL_PAGE - 1) / GL_PAGE + a.splits - 1) / a.splits * GL_PAGE + 4;
+        if (a.hd % 4 || a.chunks > 1 || a.splits > 8 || a.slots > 0 || (long long)a.held * G * (int)sizeof(float) > ST_HELD_BYTES) return GL_ERR_SHAPE;
+    } else if (a.slots < a.splits) {
+        return GL_ERR_SHAPE;
+    }
+    rc = launch_f32_rows<SF_OWN>(a, (G + a.chunks - 1) / a.chunks, dim3(a.splits, a.nKV * a.chunks, a.B), a.joined ? a.splits : 1, stream);
+    return rc != GL_OK || a.joined ? rc : launch_join(a, stream);
 }
 
 // runs of up to max_qlen tokens
 GL_API int gl_attention_weighed_runs_f32(const SpanF32Args* args, int max_qlen, cudaStream_t stream) {
-    const SpanF32Args& a = *args;
+    SpanF32Args a = *args;
+    a.early = a.held = a.joined = 0;
     if (a.B <= 0 || max_qlen <= 0) return GL_OK;
     int rc = f32_checked(a);
     if (rc != GL_OK) return rc;
-    if (!a.weights || !a.seq_row || !a.seq_qlen || a.reach <= 0 || a.last < 0) return GL_ERR_SHAPE;
+    if (!a.weights || !a.part_ml || !a.seq_row || !a.seq_qlen || a.reach <= 0 || a.last < 0) return GL_ERR_SHAPE;
     const long long tiles = ((long long)max_qlen * (a.nH / a.nKV) + 7) / 8;
     if (tiles > 0x7fffffffLL) return GL_ERR_SHAPE;
     if ((rc = launch_f32<8, SF_RUN>(a, dim3((unsigned)tiles, a.nKV, a.B), stream)) != GL_OK) return rc;

@@ -2,16 +2,19 @@
 // and the most recent positions stay and, of those between, the ones with the largest sums; what stays moves, in order, to the
 // head of the sequence's pages (or of other pages).
 //
-// Selection: a block a (layer, sequence, head).  The sums become whole numbers of the same order (a NaN below everything, both
-// zeros the same), the m-th largest is found digit by digit with histograms (11, 11 and 10 bits), and the positions above it,
-// with as many equal to it as are missing, lowest first, are written down in order: every warp counts its stretch, the counts are
-// summed, every warp writes.  Counts are whole numbers, so nothing depends on the order of additions.
+// A (layer, sequence, head) is one block's, or a cluster's, every block of which selects for itself.
+// Selection: the sums become whole numbers of the same order (a NaN below everything, both zeros the same), the m-th largest is found
+// digit by digit with histograms (11, 11 and 10 bits), and the positions above it, with as many equal to it as are missing,
+// lowest first, are written down in order: every warp counts its stretch, the counts are summed, every warp writes.  Counts
+// are whole numbers, so nothing depends on the order of additions.  The sums are read a page a warp, four pages under way.
 //
-// Moving: rows of 16-byte pieces.  What stays at place i came from place kept[i] >= i, and kept grows, so in place a block walks
-// forward: the places it has written lie before everything it has still to read.  A block owns a stretch of columns of all rows of
-// a head, so no two blocks touch the same bytes; rows that stay where they are are not touched.  Into other pages rows are
-// shared out among blocks as well.  Memory bounds it.
+// Moving: a row is its key's and its value's pieces of 16 bytes side by side.  What stays at place i came from place kept[i] >= i,
+// and kept grows, so in place a block walks forward: the places it has written lie before everything it has still to read.  The
+// blocks of a cluster share out the columns of all rows, so no two touch the same bytes, and begin when all have selected; rows
+// that stay where they are are not touched.  Into other pages they share out the rows.  Memory bounds it.
 #include "common.cuh"
+#include <cooperative_groups.h>
+namespace cg = cooperative_groups;
 
 struct EvictArgs {
     void* k_cache;                // [layers, pages, nKV, GL_PAGE, row bytes]
@@ -32,18 +35,116 @@ __device__ __forceinline__ unsigned ev_key(float w) {
 }
 __device__ __forceinline__ int ev_length(const EvictArgs& a, int b) { return min(max(0, a.seq_len[b]), a.max_pages * GL_PAGE); }
 
-// blockIdx = (key/value head, sequence, layer); dynamic shared memory: the keys of ``held`` positions, or none
-__global__ void __launch_bounds__(1024)
-evict_select_kernel(EvictArgs a, int held) {
-    extern __shared__ unsigned keys[];
-    __shared__ int hist[EV_BINS];
-    __shared__ int warp_sum[32], warp_eq[32];
-    __shared__ int found_bin, found_above;
-    const int tid = threadIdx.x, T = blockDim.x, lane = tid & 31, warp = tid >> 5, warps = T >> 5;
-    const int g = blockIdx.x, b = blockIdx.y, layer = blockIdx.z;
-    gl_grid_launch_dependents();
+#define EV_PAGES 4                        // pages of sums a warp has under way
+#define EV_MOST (200 * 1024)              // shared memory for the keys of a sequence's sums and the positions that stay
+
+// The positions of a sequence of n > keep that stay, in order, to ``list``.  keys: room for n, or null: the sums are read again each time.
+template <int T, typename Place>
+__device__ __forceinline__ void ev_select(const EvictArgs& a, int n, unsigned* keys, int* list, int* hist, int* warp_sum, int* warp_eq, int* found, Place place) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    constexpr int warps = T / 32;
+    const int lo = a.first, hi = n - a.recent;                      // the positions to choose from
+    const int want = a.keep - a.first - a.recent;
+    for (int i = tid; i < a.first; i += T) list[i] = i;
+    for (int i = tid; i < a.recent; i += T) list[a.keep - a.recent + i] = hi + i;
+    if (want <= 0) return;
+    unsigned prefix = 0, mask = 0;
+    int missing = want;                                             // how many of the positions that agree with the prefix stay
+#pragma unroll 1
+    for (int pass = 0; pass < 3; ++pass) {
+        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
+        for (int i = tid; i < EV_BINS; i += T) hist[i] = 0;
+        __syncthreads();
+        auto count = [&](int j, unsigned k) {
+            if (j >= lo && j < hi && (k & mask) == prefix) atomicAdd(&hist[(k >> shift) & ((1u << bits) - 1)], 1);
+        };
+        if (pass == 0 || !keys) {
+            for (int p0 = lo / GL_PAGE + warp * EV_PAGES; p0 * GL_PAGE < hi; p0 += warps * EV_PAGES) {
+                float2 w[EV_PAGES];
+#pragma unroll
+                for (int i = 0; i < EV_PAGES; ++i)
+                    if ((p0 + i) * GL_PAGE < hi) w[i] = *(const float2*)place((p0 + i) * GL_PAGE + 2 * lane);
+#pragma unroll
+                for (int i = 0; i < EV_PAGES; ++i)
+                    if ((p0 + i) * GL_PAGE < hi) {
+                        const int j = (p0 + i) * GL_PAGE + 2 * lane;
+                        const unsigned k0 = ev_key(w[i].x), k1 = ev_key(w[i].y);
+                        if (keys) *(uint2*)(keys + j) = make_uint2(k0, k1);
+                        count(j, k0);
+                        count(j + 1, k1);
+                    }
+            }
+        } else {
+            for (int j = lo + tid; j < hi; j += T) count(j, keys[j]);
+        }
+        __syncthreads();
+        // the bin, from the top, in which the count reaches ``missing``: every thread sums a run of bins
+        constexpr int per = EV_BINS / T;
+        const int top = EV_BINS - 1 - tid * per;                    // its highest bin
+        int mine = 0;
+        for (int i = 0; i < per; ++i) mine += hist[top - i];
+        int before = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, before, o);
+            if (lane >= o) before += v;
+        }
+        if (lane == 31) warp_sum[warp] = before;
+        __syncthreads();
+        int ahead = before - mine;
+        for (int w = 0; w < warp; ++w) ahead += warp_sum[w];
+        if (ahead < missing && ahead + mine >= missing) {
+            int i = 0;
+            while (ahead + hist[top - i] < missing) { ahead += hist[top - i]; ++i; }
+            found[0] = top - i;
+            found[1] = ahead;
+        }
+        __syncthreads();
+        prefix |= (unsigned)found[0] << shift;
+        mask |= ((1u << bits) - 1) << shift;
+        missing -= found[1];
+    }
+    // positions above the limit stay, and the first ``missing`` equal to it
+    auto key_of = [&](int j) { return keys ? keys[j] : ev_key(*place(j)); };
+    const int len = hi - lo, stretch = ((len + warps - 1) / warps + 31) & ~31;
+    const int s0 = lo + warp * stretch, s1 = min(hi, s0 + stretch);
+    int above = 0, equal = 0;
+    for (int j = s0 + lane; j - lane < s1; j += 32) {
+        const unsigned k = j < s1 ? key_of(j) : 0u;
+        above += __popc(__ballot_sync(0xffffffffu, j < s1 && k > prefix));
+        equal += __popc(__ballot_sync(0xffffffffu, j < s1 && k == prefix));
+    }
+    if (lane == 0) { warp_sum[warp] = above; warp_eq[warp] = equal; }
+    __syncthreads();
+    int at = a.first, eq = 0;
+    for (int w = 0; w < warp; ++w) {
+        at += warp_sum[w] + min(warp_eq[w], max(0, missing - eq));
+        eq += warp_eq[w];
+    }
+    for (int j = s0 + lane; j - lane < s1; j += 32) {
+        const unsigned k = j < s1 ? key_of(j) : 0u;
+        const unsigned eqs = __ballot_sync(0xffffffffu, j < s1 && k == prefix), below = (1u << lane) - 1;
+        const bool in = j < s1 && (k > prefix || (k == prefix && eq + __popc(eqs & below) < missing));
+        const unsigned ins = __ballot_sync(0xffffffffu, in);
+        if (in) list[at + __popc(ins & below)] = j;
+        at += __popc(ins);
+        eq += __popc(eqs);
+    }
+}
+
+// U: the piece a thread moves (16, 4 or 2 bytes).  blockIdx = (block of the cluster, key/value head, sequence and layer).  Dynamic
+// shared memory: the positions that stay (``listed``: else the output itself serves) and, if there is room (``held``), the sums' keys.
+template <typename U, int T>
+__global__ void __launch_bounds__(T, T == 256 ? 8 : 1)
+evict_kernel(EvictArgs a, int listed, int held) {
+    extern __shared__ __align__(16) unsigned ev[];
+    __shared__ int hist[EV_BINS], warp_sum[32], warp_eq[32], found[2], from;
+    const int tid = threadIdx.x;
+    const int C = gridDim.x, rank = blockIdx.x, g = blockIdx.y, b = blockIdx.z % a.B, layer = blockIdx.z / a.B;
     gl_grid_wait();
+    gl_grid_launch_dependents();
     const int n = ev_length(a, b), stay = min(n, a.keep);
+    const bool same = a.to == a.pages;
     const int* pg = a.pages + (size_t)b * a.max_pages;
     const int* to = a.to + (size_t)b * a.to_pages;
     const size_t base = (size_t)layer * a.n_pages;
@@ -51,196 +152,127 @@ evict_select_kernel(EvictArgs a, int held) {
         return ((base + gl_checked(table[j / GL_PAGE], a.n_pages, GL_BAD_PAGE)) * a.nKV + g) * GL_PAGE + j % GL_PAGE;
     };
     int* kept = a.kept + (((size_t)layer * a.B + b) * a.nKV + g) * a.keep;
+    unsigned* keys = held ? ev : nullptr;
+    int* list = listed ? (int*)(ev + held) : kept;
     if (n <= a.keep) {
-        for (int i = tid; i < a.keep; i += T) kept[i] = i < n ? i : -1;
-    } else {
-        const int lo = a.first, hi = n - a.recent;                  // the positions to choose from
-        int want = a.keep - a.first - a.recent;
-        for (int i = tid; i < a.first; i += T) kept[i] = i;
-        for (int i = tid; i < a.recent; i += T) kept[a.keep - a.recent + i] = hi + i;
-        if (want > 0) {
-            const bool in_smem = hi - lo <= held;
-            if (in_smem)
-                for (int j = lo + tid; j < hi; j += T) keys[j - lo] = ev_key(a.weights[place(pg, j)]);
-            auto key_of = [&](int j) { return in_smem ? keys[j - lo] : ev_key(a.weights[place(pg, j)]); };
-            unsigned prefix = 0, mask = 0;
-            int missing = want;                                     // how many of the positions that agree with the prefix stay
-#pragma unroll 1
-            for (int pass = 0; pass < 3; ++pass) {
-                const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
-                for (int i = tid; i < EV_BINS; i += T) hist[i] = 0;
-                __syncthreads();
-                for (int j = lo + tid; j < hi; j += T) {
-                    const unsigned k = key_of(j);
-                    if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & ((1u << bits) - 1)], 1);
-                }
-                __syncthreads();
-                // the bin, from the top, in which the count reaches ``missing``: every thread sums a run of bins
-                const int per = EV_BINS / T;                        // (T is a power of two up to 1024)
-                const int top = EV_BINS - 1 - tid * per;            // its highest bin
-                int mine = 0;
-                for (int i = 0; i < per; ++i) mine += hist[top - i];
-                int before = mine;
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const int v = __shfl_up_sync(0xffffffffu, before, o);
-                    if (lane >= o) before += v;
-                }
-                if (lane == 31) warp_sum[warp] = before;
-                __syncthreads();
-                int ahead = before - mine;
-                for (int w = 0; w < warp; ++w) ahead += warp_sum[w];
-                if (ahead < missing && ahead + mine >= missing) {
-                    int i = 0;
-                    while (ahead + hist[top - i] < missing) { ahead += hist[top - i]; ++i; }
-                    found_bin = top - i;
-                    found_above = ahead;
-                }
-                __syncthreads();
-                prefix |= (unsigned)found_bin << shift;
-                mask |= ((1u << bits) - 1) << shift;
-                missing -= found_above;
-                __syncthreads();
-            }
-            // positions above the limit stay, and the first ``missing`` equal to it
-            const int len = hi - lo, stretch = ((len + warps - 1) / warps + 31) & ~31;
-            const int s0 = lo + warp * stretch, s1 = min(hi, s0 + stretch);
-            int above = 0, equal = 0;
-            for (int j = s0 + lane; j - lane < s1; j += 32) {
-                const unsigned k = j < s1 ? key_of(j) : 0u;
-                above += __popc(__ballot_sync(0xffffffffu, j < s1 && k > prefix));
-                equal += __popc(__ballot_sync(0xffffffffu, j < s1 && k == prefix));
-            }
-            if (lane == 0) { warp_sum[warp] = above; warp_eq[warp] = equal; }
-            __syncthreads();
-            int at = a.first, eq = 0;
-            for (int w = 0; w < warp; ++w) {
-                at += warp_sum[w] + min(warp_eq[w], max(0, missing - eq));
-                eq += warp_eq[w];
-            }
-            for (int j = s0 + lane; j - lane < s1; j += 32) {
-                const unsigned k = j < s1 ? key_of(j) : 0u;
-                const unsigned eqs = __ballot_sync(0xffffffffu, j < s1 && k == prefix), below = (1u << lane) - 1;
-                const bool in = j < s1 && (k > prefix || (k == prefix && eq + __popc(eqs & below) < missing));
-                const unsigned ins = __ballot_sync(0xffffffffu, in);
-                if (in) kept[at + __popc(ins & below)] = j;
-                at += __popc(ins);
-                eq += __popc(eqs);
-            }
+        for (int i = tid; i < a.keep; i += T) {
+            if (rank == 0) kept[i] = i < n ? i : -1;
+            if (i < n && listed) list[i] = i;
         }
+        if (same) return;
+    } else {
+        ev_select<T>(a, n, keys, list, hist, warp_sum, warp_eq, found, [&](int j) { return a.weights + place(pg, j); });
     }
     __syncthreads();
-    // the sums move with their positions (forward, a block's width at a time: see above)
-    const bool same = a.to == a.pages;
-    if (same && n <= a.keep) return;
-    for (int i0 = 0; i0 < stay; i0 += T) {
-        const int i = i0 + tid;
-        float w = 0.f;
-        int j = i;
-        if (i < stay) {
-            j = kept[i];
-            w = a.weights[place(pg, j)];
-        }
-        __syncthreads();
-        if (i < stay && !(same && j == i)) a.weights[place(to, i)] = w;
-    }
-}
-
-// U: the piece a thread moves (16, 4 or 2 bytes).  blockIdx = (keys or values, stretch of columns, share of the rows; head; sequence and layer)
-template <typename U>
-__global__ void __launch_bounds__(256)
-evict_move_kernel(EvictArgs a, int slices, int shares) {
-    __shared__ int from;
-    const int tid = threadIdx.x;
-    int x = blockIdx.x;
-    const int which = x & 1;
-    x >>= 1;
-    const int slice = x % slices, share = x / slices;
-    const int g = blockIdx.y, b = blockIdx.z % a.B, layer = blockIdx.z / a.B;
-    gl_grid_launch_dependents();
-    gl_grid_wait();
-    const int n = ev_length(a, b), stay = min(n, a.keep);
-    const bool same = a.to == a.pages;
-    if (same && n <= a.keep) return;
-    const int units = (which ? a.v_bytes : a.k_bytes) / (int)sizeof(U);
-    const int per = (units + slices - 1) / slices, u0 = slice * per, width = min(per, units - u0);
-    if (width <= 0) return;
-    U* cache = (U*)(which ? a.v_cache : a.k_cache) + (size_t)layer * a.n_pages * a.nKV * GL_PAGE * units + u0;
-    const int* pg = a.pages + (size_t)b * a.max_pages;
-    const int* to = a.to + (size_t)b * a.to_pages;
-    const int* kept = a.kept + (((size_t)layer * a.B + b) * a.nKV + g) * a.keep;
-    auto row = [&](const int* table, int j) {
-        return cache + (((size_t)gl_checked(table[j / GL_PAGE], a.n_pages, GL_BAD_PAGE) * a.nKV + g) * GL_PAGE + j % GL_PAGE) * units;
-    };
-    int begin = 0, end = stay;
-    if (same) {                                                    // the first row that moves: kept[i] - i never falls
-        if (tid == 0) {
+    if (listed && rank == 0 && n > a.keep)
+        for (int i = tid; i < a.keep; i += T) kept[i] = list[i];
+    int begin = 0, end = stay;                                     // the rows, and of a row's pieces the columns, that this block moves
+    const int ku = a.k_bytes / (int)sizeof(U), vu = a.v_bytes / (int)sizeof(U);
+    int u0 = 0, u1 = ku + vu;
+    if (same) {
+        if (tid == 0) {                                            // the first row that moves: kept[i] - i never falls
             int l = 0, h = stay;
-            while (l < h) { const int m = (l + h) / 2; if (kept[m] > m) h = m; else l = m + 1; }
+            while (l < h) { const int m = (l + h) / 2; if (list[m] > m) h = m; else l = m + 1; }
             from = l;
         }
+        u0 = (int)((long long)(ku + vu) * rank / C);
+        u1 = (int)((long long)(ku + vu) * (rank + 1) / C);
+        if (C > 1) cg::this_cluster().sync();                      // (the sums have been read by all before any moves)
         __syncthreads();
         begin = from;
     } else {
-        const int rows = (stay + shares - 1) / shares;
-        begin = share * rows;
-        end = min(stay, begin + rows);
+        begin = (int)((long long)stay * rank / C);
+        end = (int)((long long)stay * (rank + 1) / C);
     }
-    constexpr int N = 4;                                           // pieces a thread has under way
-    const int step = 256 / width, lane_row = tid / width, col = tid - lane_row * width;      // (width <= 256)
-    const bool active = lane_row < step;
-    for (int i0 = begin; i0 < end; i0 += N * step) {
-        U v[N];
-#pragma unroll
-        for (int k = 0; k < N; ++k) {
-            const int i = i0 + k * step + lane_row;
-            if (active && i < end) v[k] = row(pg, kept[i])[col];
+    // The list now says where a row lies, its page's number and its place there, not which position it is.
+    if (listed) {
+        __syncthreads();
+        for (int i = tid; i < stay; i += T) {
+            const int j = list[i];
+            list[i] = gl_checked(pg[j / GL_PAGE], a.n_pages, GL_BAD_PAGE) * GL_PAGE + j % GL_PAGE;
         }
-        if (same) __syncthreads();
+        __syncthreads();
+    }
+    const size_t first_row = (base * a.nKV + g) * GL_PAGE;
+    auto source = [&](int i) {
+        const int x = list[i];
+        return listed ? first_row + (size_t)(x / GL_PAGE) * a.nKV * GL_PAGE + x % GL_PAGE : place(pg, x);
+    };
+    // the sums: forward, a block's width at a time
+    if (!same || rank == C - 1)
+        for (int i0 = begin; i0 < end; i0 += T) {
+            const int i = i0 + tid;
+            float w = 0.f;
+            if (i < end) w = a.weights[source(i)];
+            if (same) __syncthreads();
+            if (i < end) a.weights[place(to, i)] = w;
+        }
+    // Pieces a thread has under way.  Small blocks, eight an SM, move and select beside one another (24 layers of 4 x 32 heads of 64, 1,024 of
+    // some 1,900 positions stay, 1.66 GB: 295 us; four blocks of eight pieces 358, eight of two 304); a large one is alone on its SM
+    // (4 x 2 x 8 heads of 128, 4,096 of 31,400 stay: 75 us, with four pieces 87).
+    constexpr int N = T == 256 ? 4 : 8;
+    U* kc = (U*)a.k_cache;
+    U* vc = (U*)a.v_cache;
+    for (int c0 = u0; c0 < u1; c0 += T) {
+        const int width = min(T, u1 - c0), step = T / width, row = tid / width, u = c0 + tid - row * width;
+        const bool active = row < step, is_v = u >= ku;
+        U* cache = is_v ? vc : kc;
+        const int units = is_v ? vu : ku, col = is_v ? u - ku : u;
+        for (int i0 = begin; i0 < end; i0 += N * step) {
+            U v[N];
 #pragma unroll
-        for (int k = 0; k < N; ++k) {
-            const int i = i0 + k * step + lane_row;
-            if (active && i < end) row(to, i)[col] = v[k];
+            for (int k = 0; k < N; ++k) {
+                const int i = i0 + k * step + row;
+                if (active && i < end) v[k] = cache[source(i) * units + col];
+            }
+            if (same) __syncthreads();
+#pragma unroll
+            for (int k = 0; k < N; ++k) {
+                const int i = i0 + k * step + row;
+                if (active && i < end) cache[place(to, i) * units + col] = v[k];
+            }
         }
     }
 }
 
-template <typename U>
-static int launch_move(const EvictArgs& a, int slices, int shares, cudaStream_t stream) {
-    return gl_launch(evict_move_kernel<U>, dim3(2 * slices * shares, a.nKV, a.B * a.layers), dim3(256), 0, stream, 1, a, slices, shares);
+template <typename U, int T>
+static int launch_evict(const EvictArgs& a, int blocks, int listed, int held, cudaStream_t stream) {
+    static bool allowed[64] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) { cudaGetLastError(); return GL_ERR_DRIVER; }
+    if (!allowed[dev]) {
+        if (cudaFuncSetAttribute(evict_kernel<U, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, EV_MOST) != cudaSuccess) {
+            cudaGetLastError();
+            return GL_ERR_SMEM;
+        }
+        allowed[dev] = true;
+    }
+    return gl_launch(evict_kernel<U, T>, dim3(blocks, a.nKV, a.B * a.layers), dim3(T), ((size_t)held + (listed ? a.keep : 0)) * 4, stream, blocks, a, listed, held);
 }
 
 GL_API int gl_cache_evict(const EvictArgs* args, int sms, cudaStream_t stream) {
     const EvictArgs& a = *args;
     if (a.B <= 0 || a.layers <= 0) return GL_OK;
     if (a.nKV <= 0 || a.nKV > 65535 || (long long)a.B * a.layers > 65535 || a.keep <= 0 || a.first < 0 || a.recent < 0 || a.first + a.recent > a.keep) return GL_ERR_SHAPE;
-    if (a.n_pages <= 0 || a.max_pages <= 0 || a.to_pages * GL_PAGE < (a.keep < a.max_pages * GL_PAGE ? a.keep : a.max_pages * GL_PAGE)) return GL_ERR_SHAPE;
-    if (a.k_bytes <= 0 || a.v_bytes <= 0 || a.k_bytes > 4096 || a.v_bytes > 4096 || (a.k_bytes | a.v_bytes) % 2) return GL_ERR_SHAPE;
-    const uintptr_t at = (uintptr_t)a.k_cache | (uintptr_t)a.v_cache | (uintptr_t)a.k_bytes | (uintptr_t)a.v_bytes;
-    // a thousand positions or two a block of 256 threads; longer sequences take larger blocks
     const long long most = (long long)a.max_pages * GL_PAGE;
+    if (a.n_pages <= 0 || a.max_pages <= 0 || most > 0x7fffffff || (long long)a.n_pages * GL_PAGE > 0x7fffffff || (long long)a.to_pages * GL_PAGE < (a.keep < most ? a.keep : most)) return GL_ERR_SHAPE;
+    if (a.k_bytes <= 0 || a.v_bytes <= 0 || a.k_bytes > 4096 || a.v_bytes > 4096 || (a.k_bytes | a.v_bytes) % 2) return GL_ERR_SHAPE;
+    if ((uintptr_t)a.weights & 7) return GL_ERR_ALIGN;
+    const uintptr_t at = (uintptr_t)a.k_cache | (uintptr_t)a.v_cache | (uintptr_t)a.k_bytes | (uintptr_t)a.v_bytes;
+    // What fits in shared memory: the list of what stays, then the sums' keys beside it.
+    const int listed = a.keep < most && 4LL * a.keep <= EV_MOST ? 1 : 0;
+    const int held = 4 * (most + (listed ? a.keep : 0)) <= EV_MOST ? (int)most : 0;
+    // Blocks of 256 threads, several an SM, for up to 4,096 positions; larger ones beyond.  A cluster shares the rows out where there
+    // are fewer heads than the machine takes blocks.
     const int threads = most <= 4096 ? 256 : 1024;
-    const int held = (int)(most < 48 * 1024 ? most : 48 * 1024);
-    static bool allowed[64] = {};
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) { cudaGetLastError(); return GL_ERR_DRIVER; }
-    if (!allowed[dev]) {
-        if (cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 48 * 1024 * 4) != cudaSuccess) {
-            cudaGetLastError();
-            return GL_ERR_SMEM;
-        }
-        allowed[dev] = true;
+    const long long heads = (long long)a.layers * a.B * a.nKV, room = (threads == 256 ? 4LL : 1LL) * sms;
+    int blocks = 1;
+    while (blocks < 8 && heads * 2 * blocks <= room && a.keep / (2 * blocks) >= 32) blocks *= 2;
+    if (!listed) blocks = 1;                                       // (the list is then the output itself, which one block writes)
+    if (threads == 256) {
+        if (at % 16 == 0) return launch_evict<uint4, 256>(a, blocks, listed, held, stream);
+        return at % 4 == 0 ? launch_evict<unsigned, 256>(a, blocks, listed, held, stream) : launch_evict<unsigned short, 256>(a, blocks, listed, held, stream);
     }
-    int rc = gl_launch(evict_select_kernel, dim3(a.nKV, a.B, a.layers), dim3(threads), (size_t)held * 4, stream, 1, a, held);
-    if (rc != GL_OK) return rc;
-    const bool same = a.to == a.pages;
-    const long long heads = 2LL * a.layers * a.B * a.nKV;
-    const int size = at % 16 == 0 ? 16 : at % 4 == 0 ? 4 : 2, units = (a.k_bytes > a.v_bytes ? a.k_bytes : a.v_bytes) / size;
-    int slices = (units + 255) / 256, shares = 1;
-    if (same)
-        while (heads * slices < 4LL * sms && units / (2 * slices) * size >= 32) slices *= 2;     // (pieces of 32 bytes still fill a sector)
-    else
-        while (heads * slices * shares < 8LL * sms && a.keep / (2 * shares) >= 32) shares *= 2;
-    if (size == 16) return launch_move<uint4>(a, slices, shares, stream);
-    return size == 4 ? launch_move<unsigned>(a, slices, shares, stream) : launch_move<unsigned short>(a, slices, shares, stream);
+    if (at % 16 == 0) return launch_evict<uint4, 1024>(a, blocks, listed, held, stream);
+    return at % 4 == 0 ? launch_evict<unsigned, 1024>(a, blocks, listed, held, stream) : launch_evict<unsigned short, 1024>(a, blocks, listed, held, stream);
 }

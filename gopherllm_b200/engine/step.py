@@ -54,7 +54,6 @@ class StepContext:
         self.side_stream = None          # a second stream blocks may fork onto (decode steps only)
 
 
-SHARED_POSITIONS = 1024              # positions that reading shared pages once must spare a step before it is worth its own kernels
 GRAPH_F32_RUN_BYTES = 128 << 20      # weights of a model for each run of its schedule, up to which 32-bit decode steps are captured
 
 
@@ -243,8 +242,7 @@ class Engine:
             return ()
         from .. import ops
         groups = self.cache.shared_prefixes(slots)
-        spared = sum((len(members) - 1) * n for members, n in groups)
-        if not groups or spared < SHARED_POSITIONS:
+        if not groups:
             return ()
         shared = [0] * len(slots)
         for members, n in groups:
@@ -252,7 +250,8 @@ class Engine:
                 shared[b] = n
         # (sized for a bucket of lengths, as captured steps are)
         own = self._length_bucket(max(c + 1 - s for c, s in zip(ctxs, shared)))
-        return tuple(ops.PrefixLayout(groups, len(slots), *heads, self.act_dtype, own, ops.sm_count(self.device)) for heads in self.shared_heads)
+        layouts = (ops.PrefixLayout(groups, len(slots), *heads, self.act_dtype, own, ops.sm_count(self.device)) for heads in self.shared_heads)
+        return tuple(x for x in layouts if x.n_items)
 
     def _stage(self, buf: np.ndarray) -> torch.Tensor:
         """The descriptor in pinned host memory, ready for an asynchronous copy."""

@@ -866,11 +866,23 @@ class PrefixLayout:
             seen.update(members)
             checked.append((members, shared // PAGE))
         most = max((len(m) * group for m, _ in checked), default=1)
-        self.rows = min(most, span_rows(dtype, head_dim))         # rows of an item
+        tensor = dtype == torch.bfloat16 and head_dim <= 128 and most > span_rows(dtype, head_dim)
+        self.rows = (128 if most <= 128 else 256) if tensor else min(most, span_rows(dtype, head_dim))      # rows of an item
         tiles = [-(-len(m) * group // self.rows) for m, _ in checked]
-        # blocks walk equal stretches of pages, short enough to fill the machine a few times over
+        # Where reading the shared pages once spares little, every sequence reads them with its own: a kernel less.
+        spared = sum((len(m) - 1) * p for m, p in checked) * 2 * PAGE * num_kv_heads * head_dim * (4 if dtype == torch.float32 else 2)
+        if spared < PREFIX_SPARED_BYTES:
+            own, checked, tiles = own + PAGE * max((p for _, p in checked), default=0), [], []
+        # Blocks walk equal stretches of pages: on the tensor cores one block an SM at a time, so as few rounds of them as the tiles
+        # allow; else short enough to fill the machine a few times over.
         total = sum(t * p for t, (_, p) in zip(tiles, checked)) * num_kv_heads
-        stretch = max(2, -(-total // (PREFIX_BLOCKS_PER_SM * sms)))
+        if tensor:
+            room = sms * -(-sum(tiles) * num_kv_heads // sms)
+            stretch = max(2, total // room)
+            while sum(t * -(-p // stretch) for t, (_, p) in zip(tiles, checked)) * num_kv_heads > room:
+                stretch += 1
+        else:
+            stretch = max(2, -(-total // (PREFIX_BLOCKS_PER_SM * sms)))
         order, items, shared_of = [], [], [[0, 0] for _ in range(batch)]
         slots = 0
         for (members, pages), n_tiles in zip(checked, tiles):
@@ -885,11 +897,16 @@ class PrefixLayout:
             for b in members:
                 shared_of[b] = [pages, n]
             order += members
-        self.max_shared = max((p for _, p in checked), default=0)
+        self.max_shared = max((p for _, p in checked), default=0)      # pages
         own_pages = -(-own // PAGE)
         self.chunks = span_chunks(dtype, head_dim, group)
-        self.splits = span_splits(batch, num_kv_heads * self.chunks, own_pages, sms)
-        self.slots, self.n_items = slots + self.splits, len(items)
+        self.splits = span_splits(batch, num_kv_heads * self.chunks, own_pages, sms, dtype, head_dim)
+        # joined: the blocks of a sequence's own pages put everything together themselves (csrc/attention_spans.cu)
+        self.joined = (head_dim % 4 == 0 and self.splits <= 8
+                       and 4 * (8 if dtype == torch.float32 else span_rows(dtype, head_dim)) * (slots + self.splits) <= SPAN_FACTOR_BYTES)
+        self.slots, self.n_items = slots + (0 if self.joined else self.splits), len(items)
+        self.call = (batch, num_heads, num_kv_heads, head_dim, dtype)
+        self.launches = (1 if items else 0) + (1 if self.joined else 2)
         flat = [v for it in items for v in it]
         self.items_at, self.shared_at = len(order), len(order) + len(flat)
         self.ints = np.array(order + flat + [v for s in shared_of for v in s], dtype=np.int32)
@@ -901,6 +918,8 @@ class PrefixLayout:
 
 
 PREFIX_BLOCKS_PER_SM = 4
+PREFIX_SPARED_BYTES = 12 << 20       # (see PrefixLayout)
+SPAN_FACTOR_BYTES, SPAN_HELD_BYTES = 24 * 1024, 56 * 1024      # shared memory for the factors of a row's parts, for a block's scores
 
 
 def _check_span_heads(what: str, dtype, head_dim: int) -> None:
@@ -925,7 +944,9 @@ def span_heads_fit(dtype, head_dim: int) -> bool:
 
 def span_rows(dtype, head_dim: int) -> int:
     """Rows of queries one block takes over a span of the cache at most."""
-    return 8 if dtype == torch.float32 else 32 if head_dim <= 128 else 16
+    if dtype == torch.float32:
+        return 8 if head_dim % 4 or head_dim <= 64 else 4 if head_dim <= 128 else 2
+    return 32 if head_dim <= 128 else 16
 
 
 def span_chunks(dtype, head_dim: int, group: int) -> int:
@@ -934,9 +955,14 @@ def span_chunks(dtype, head_dim: int, group: int) -> int:
     return -(-group // -(-group // n))
 
 
-def span_splits(batch: int, heads: int, pages: int, sms: int) -> int:
-    """Spans a sequence's own pages are cut into: enough blocks for two on every SM, at most eight pages a block."""
-    return max(1, min(pages, max(-(-2 * sms // max(1, batch * heads)), -(-pages // 8))))
+def span_splits(batch: int, heads: int, pages: int, sms: int, dtype, head_dim: int) -> int:
+    """Blocks that share a sequence's own pages: as many as are resident at once, of four pages at least.  Up to eight form a
+    cluster and join their results themselves; more leave them to a second kernel, so eight it is where those fill two blocks an SM or
+    have no more than eight pages each."""
+    per_sm = 4 if dtype == torch.float32 else max(1, min(8, 227 * 1024 // (4 * PAGE * (2 * head_dim + 16) + 4096)))
+    blocks = max(1, batch * heads)
+    n = max(1, min(per_sm * sms // blocks, pages if dtype == torch.float32 else -(-pages // 4)))
+    return 8 if n > 8 and (8 * blocks >= 2 * sms or pages <= 64) else n
 
 
 def prefix_plan(groups, batch: int, num_heads: int, num_kv_heads: int, head_dim: int, dtype, own: int, device) -> PrefixPlan:
@@ -951,11 +977,11 @@ def prefix_plan(groups, batch: int, num_heads: int, num_kv_heads: int, head_dim:
 class _SpanArgs(Structure):
     _fields_ = [(n, c_void_p) for n in ("q", "out", "k_cache", "v_cache", "seq_row", "seq_qlen", "seq_ctx", "pages", "order", "items",
                                         "seq_shared", "part_o", "part_ml", "scores", "weights")] + \
-               [(n, c_int) for n in ("B", "nH", "nKV", "max_pages", "n_pages", "n_items", "splits", "slots", "chunks", "reach")]
+               [(n, c_int) for n in ("B", "nH", "nKV", "max_pages", "n_pages", "n_items", "splits", "slots", "chunks", "reach", "early", "held")]
 
 
 class _SpanF32Args(Structure):
-    _fields_ = _SpanArgs._fields_ + [("hd", c_int), ("last", c_int)]
+    _fields_ = _SpanArgs._fields_[:-2] + [("hd", c_int), ("last", c_int), ("early", c_int), ("held", c_int), ("joined", c_int)]
 
 
 class _RunArgs(Structure):
@@ -963,8 +989,21 @@ class _RunArgs(Structure):
                [(n, c_int) for n in ("B", "nH", "nKV", "max_pages", "n_pages", "reach", "last")]
 
 
+def _fit(here: int, dtype, *tensors) -> bool:
+    """Whether these are contiguous tensors of this type on the device that is current (the launch goes to its stream)."""
+    for t in tensors:
+        if t.get_device() != here or t.dtype is not dtype or not t.is_contiguous():
+            return False
+    return True
+
+
+def _launch_device(t) -> int:
+    """The device that is current, where ``t`` lies on it; -2 where it does not."""
+    at = t.get_device()
+    return at if at >= 0 and at == torch.cuda.current_device() else -2
+
+
 def _one_device(what: str, *tensors) -> None:
-    """The tensors of a call lie on the device that is current: the launch goes to its stream."""
     here = torch.cuda.current_device()
     for t in tensors:
         if t is not None and t.device.index != here:
@@ -972,26 +1011,27 @@ def _one_device(what: str, *tensors) -> None:
 
 
 def _need_span(what: str, q, out, k_cache, v_cache, seq_ctx, pages, num_heads, num_kv_heads, head_dim) -> int:
-    _check_span_heads(what, q.dtype if isinstance(q, torch.Tensor) else None, head_dim)
-    if num_heads < 1 or num_kv_heads < 1 or num_heads % num_kv_heads:
-        raise KernelError(f"{what}: {num_heads} heads are not a multiple of {num_kv_heads} key/value heads")
-    _need(q, "q")
-    if q.dim() != 2 or q.shape[1] != num_heads * head_dim:
-        raise KernelError(f"{what}: q must be [tokens, {num_heads * head_dim}], is {tuple(q.shape)}")
-    _need(out, "out", q.dtype, q.shape)
-    _need(k_cache, "k_cache", q.dtype)
-    _need(v_cache, "v_cache", q.dtype, k_cache.shape)
-    if k_cache.dim() != 4 or tuple(k_cache.shape[1:]) != (num_kv_heads, PAGE, head_dim):
-        raise KernelError(f"cache pages must be [*, {num_kv_heads}, {PAGE}, {head_dim}], are {tuple(k_cache.shape)}")
-    _need(seq_ctx, "seq_ctx", torch.int32)
-    _need(pages, "pages", torch.int32)
-    B = seq_ctx.numel()
-    if seq_ctx.dim() != 1 or pages.dim() != 2 or pages.shape[0] != B:
-        raise KernelError(f"{what}: pages {tuple(pages.shape)} do not go with {B} sequences")
-    if B > 65535:
-        raise KernelError(f"{what}: {B} sequences are more than a launch takes (65535)")
+    """The checks that attention over spans has in common; the number of sequences."""
+    try:
+        dtype, here = q.dtype, _launch_device(q)
+        _check_span_heads(what, dtype, head_dim)
+        if num_heads < 1 or num_kv_heads < 1 or num_heads % num_kv_heads:
+            raise KernelError(f"{what}: {num_heads} heads are not a multiple of {num_kv_heads} key/value heads")
+        k, B = k_cache.shape, seq_ctx.shape[0]
+        if (_fit(here, dtype, q, out, k_cache, v_cache) and _fit(here, torch.int32, seq_ctx, pages) and k[1:] == (num_kv_heads, PAGE, head_dim)
+                and v_cache.shape == k and len(q.shape) == 2 and q.shape[1] == num_heads * head_dim and out.shape == q.shape and len(seq_ctx.shape) == 1
+                and len(pages.shape) == 2 and pages.shape[0] == B and B <= 65535):
+            return B
+    except (AttributeError, IndexError):
+        pass
+    # something does not fit: say what
+    for t, name, kind in ((q, "q", None), (out, "out", getattr(q, "dtype", None)), (k_cache, "k_cache", getattr(q, "dtype", None)),
+                          (v_cache, "v_cache", getattr(q, "dtype", None)), (seq_ctx, "seq_ctx", torch.int32), (pages, "pages", torch.int32)):
+        _need(t, name, kind)
     _one_device(what, q, out, k_cache, v_cache, seq_ctx, pages)
-    return B
+    raise KernelError(f"{what}: q {tuple(q.shape)}, out {tuple(out.shape)}, cache pages {tuple(k_cache.shape)} and {tuple(v_cache.shape)}, seq_ctx "
+                      f"{tuple(seq_ctx.shape)} and pages {tuple(pages.shape)} do not go with {num_heads} heads on {num_kv_heads} key/value heads of "
+                      f"{head_dim} in pages of {PAGE}, up to 65535 sequences")
 
 
 def attention_prefix(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, seq_ctx: torch.Tensor,
@@ -1002,28 +1042,27 @@ def attention_prefix(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, 
     members have the same ids in their first columns.  ``seq_ctx``, positions cached before this step, is read on the device:
     one call captured in a graph serves later steps.  bfloat16 (heads of 16..256 in steps of 16) or float32 (heads up to 256)."""
     B = _need_span("attention_prefix", q, out, k_cache, v_cache, seq_ctx, pages, num_heads, num_kv_heads, head_dim)
-    lay = plan.layout
-    if (lay.batch, lay.num_heads, lay.num_kv_heads, lay.head_dim, lay.dtype) != (B, num_heads, num_kv_heads, head_dim, q.dtype) or q.shape[0] != B:
+    lay, ints = plan.layout, plan.ints
+    if lay.call != (B, num_heads, num_kv_heads, head_dim, q.dtype) or q.shape[0] != B:
         raise KernelError(f"attention_prefix: a plan for {lay.batch} sequences, {lay.num_heads}/{lay.num_kv_heads} heads of {lay.head_dim} ({lay.dtype}) "
                           f"does not go with {B} sequences, {q.shape[0]} rows, {num_heads}/{num_kv_heads} heads of {head_dim} ({q.dtype})")
     if pages.shape[1] < lay.max_shared:
         raise KernelError(f"attention_prefix: {lay.max_shared} shared pages in a table of {pages.shape[1]}")
-    _need(plan.ints, "plan", torch.int32)
-    _one_device("attention_prefix", plan.ints)
-    n = B * num_heads * lay.slots
-    part = empty((n * (head_dim + 2),), torch.float32, q.device)
-    base, at = plan.ints.data_ptr(), part.data_ptr()
-    fields = (q.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), None, None, seq_ctx.data_ptr(), pages.data_ptr(),
-              base, base + 4 * lay.items_at, base + 4 * lay.shared_at, at, at + 4 * n * head_dim, None, None,
-              B, num_heads, num_kv_heads, pages.shape[1], k_cache.shape[0], lay.n_items, lay.splits, lay.slots, lay.chunks, 0)
-    launches = 3 if lay.n_items else 2
-    if q.dtype == torch.float32:
-        a = _SpanF32Args(*fields, head_dim, 0)
-        _check(_launch(_lib("attention_spans_f32.cu").gl_attention_prefix_f32, byref(a), c_int(lay.rows), _stream()), "attention_prefix", launches)
-    else:
-        a = _SpanArgs(*fields)
-        fn = _lib("attention_spans.cu", catalog.head_dim_defines(head_dim)).gl_attention_prefix
-        _check(_launch(fn, byref(a), c_int(lay.rows), _stream()), "attention_prefix", launches)
+    if ints.get_device() != q.get_device():
+        raise KernelError(f"attention_prefix: the plan is on {ints.device}")
+    base, at, ml = ints.data_ptr(), None, None
+    if lay.slots:
+        n = B * num_heads * lay.slots * head_dim
+        part = empty((n + B * num_heads * lay.slots * 2,), torch.float32, q.device)      # (held until the launch)
+        at = part.data_ptr()
+        ml = at + 4 * n
+    f32 = q.dtype is torch.float32
+    a = (_SpanF32Args if f32 else _SpanArgs)(
+        q.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), None, None, seq_ctx.data_ptr(), pages.data_ptr(),
+        base, base + 4 * lay.items_at, base + 4 * lay.shared_at, at, ml, None, None,
+        B, num_heads, num_kv_heads, pages.shape[1], k_cache.shape[0], lay.n_items, lay.splits, lay.slots, lay.chunks, 0, head_dim if f32 else 0)
+    fn = _lib("attention_spans_f32.cu").gl_attention_prefix_f32 if f32 else _lib("attention_spans.cu", (f"GL_HEAD_DIM={head_dim}",)).gl_attention_prefix
+    _check(_launch(fn, byref(a), c_int(lay.rows), c_int(lay.joined), _stream()), "attention_prefix", lay.launches)
 
 
 def attention_weighed(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, weights: torch.Tensor,
@@ -1037,33 +1076,36 @@ def attention_weighed(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor,
     queries are counted.  Places behind a sequence's last position stay as they are, a sequence without tokens leaves everything
     as it is.  ``max_qlen``, ``max_len``: the longest run, and the longest sequence after the step."""
     B = _need_span("attention_weighed", q, out, k_cache, v_cache, seq_ctx, pages, num_heads, num_kv_heads, head_dim)
-    _need(weights, "weights", torch.float32, k_cache.shape[:3])
-    _need(seq_qstart, "seq_qstart", torch.int32, (B,))
-    _need(seq_qlen, "seq_qlen", torch.int32, (B,))
-    _one_device("attention_weighed", weights, seq_qstart, seq_qlen)
+    here, n_pages, dtype = q.get_device(), k_cache.shape[0], q.dtype
+    if not (isinstance(weights, torch.Tensor) and _fit(here, torch.float32, weights) and weights.shape == k_cache.shape[:3]
+            and _fit(here, torch.int32, seq_qstart, seq_qlen) and seq_qstart.shape == seq_ctx.shape and seq_qlen.shape == seq_ctx.shape):
+        _need(weights, "weights", torch.float32, k_cache.shape[:3])
+        _need(seq_qstart, "seq_qstart", torch.int32, (B,))
+        _need(seq_qlen, "seq_qlen", torch.int32, (B,))
+        _one_device("attention_weighed", weights, seq_qstart, seq_qlen)
     if last < 0 or max_qlen < 0 or max_len < max_qlen or max_len > pages.shape[1] * PAGE:
         raise KernelError(f"attention_weighed: runs of up to {max_qlen} tokens, sequences of up to {max_len} positions in tables of "
                           f"{pages.shape[1]} pages, the last {last} queries counted")
     if B == 0 or max_qlen == 0:
         return
-    group, n_pages = num_heads // num_kv_heads, k_cache.shape[0]
-    f32 = q.dtype == torch.float32
-    lib = _lib("attention_spans_f32.cu") if f32 else _lib("attention_spans.cu", catalog.head_dim_defines(head_dim))
+    f32 = dtype is torch.float32
+    lib = _lib("attention_spans_f32.cu") if f32 else _lib("attention_spans.cu", (f"GL_HEAD_DIM={head_dim}",))
     if max_qlen == 1:
-        chunks = span_chunks(q.dtype, head_dim, group)
-        splits = span_splits(B, num_kv_heads * chunks, -(-max_len // PAGE), sm_count(q.device))
-        n = B * num_heads * splits
-        part = empty((n * (head_dim + 2) + B * num_heads * max_len,), torch.float32, q.device)
-        at = part.data_ptr()
-        fields = (q.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), seq_qstart.data_ptr(), seq_qlen.data_ptr(),
-                  seq_ctx.data_ptr(), pages.data_ptr(), None, None, None, at, at + 4 * n * head_dim, at + 4 * n * (head_dim + 2),
-                  weights.data_ptr(), B, num_heads, num_kv_heads, pages.shape[1], n_pages, 0, splits, splits, chunks, max_len)
-        if f32:
-            a = _SpanF32Args(*fields, head_dim, 0)
-            _check(_launch(lib.gl_attention_weighed_f32, byref(a), _stream()), "attention_weighed", 3)
-        else:
-            a = _SpanArgs(*fields)
-            _check(_launch(lib.gl_attention_weighed, byref(a), _stream()), "attention_weighed", 3)
+        group, used = num_heads // num_kv_heads, -(-max_len // PAGE)
+        chunks = span_chunks(dtype, head_dim, group)
+        splits = span_splits(B, num_kv_heads * chunks, used, sm_count(q.device), dtype, head_dim)
+        slots, at, ml, scores = 0, None, None, None
+        if head_dim % 4 or chunks > 1 or splits > 8 or 4 * group * (-(-used // splits) * PAGE + 4) > SPAN_HELD_BYTES:
+            slots, n = splits, B * num_heads * splits * head_dim
+            part = empty((n + B * num_heads * (2 * splits + max_len),), torch.float32, q.device)
+            at = part.data_ptr()
+            ml, scores = at + 4 * n, at + 4 * (n + B * num_heads * 2 * splits)
+        a = (_SpanF32Args if f32 else _SpanArgs)(
+            q.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), seq_qstart.data_ptr(), seq_qlen.data_ptr(),
+            seq_ctx.data_ptr(), pages.data_ptr(), None, None, None, at, ml, scores,
+            weights.data_ptr(), B, num_heads, num_kv_heads, pages.shape[1], n_pages, 0, splits, slots, chunks, max_len, head_dim if f32 else 0)
+        _check(_launch(lib.gl_attention_weighed_f32 if f32 else lib.gl_attention_weighed, byref(a), _stream()), "attention_weighed",
+               2 if slots else 1)
         return
     ml = empty((q.shape[0], num_heads, 2), torch.float32, q.device)
     if f32:
@@ -1127,7 +1169,7 @@ def cache_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, weights: torch.Ten
         return kept.fill_(-1)
     a = _EvictArgs(k_cache.data_ptr(), v_cache.data_ptr(), weights.data_ptr(), seq_len.data_ptr(), pages.data_ptr(), to.data_ptr(), kept.data_ptr(),
                    layers, B, heads, n_pages, pages.shape[1], to.shape[1], keep, recent, first, k_cache.shape[-1] * es, v_cache.shape[-1] * es)
-    _check(_launch(_lib("cache_evict.cu").gl_cache_evict, byref(a), c_int(sm_count(k_cache.device)), _stream()), "cache_evict", 2)
+    _check(_launch(_lib("cache_evict.cu").gl_cache_evict, byref(a), c_int(sm_count(k_cache.device)), _stream()), "cache_evict")
     return kept
 
 

@@ -9,6 +9,12 @@ PAGE = 64
 BF, F = torch.bfloat16, torch.float32
 
 
+@pytest.fixture(autouse=True)
+def shared_however_little(monkeypatch):
+    from gopherllm_b200 import ops
+    monkeypatch.setattr(ops, "PREFIX_SPARED_BYTES", 0)
+
+
 def build(groups, ctx, H, G, D, dtype, seed, spare=3):
     """Pages in a random order, NaN wherever no position was written; (q, keys, values, seq_ctx, table)."""
     g = torch.Generator().manual_seed(seed)
@@ -157,3 +163,16 @@ def test_a_call_on_a_device_tensor_of_another_type_is_refused():
             ops.attention_prefix(*args, plan, 4, 2, 64)
     with pytest.raises(ops.KernelError):
         ops.attention_prefix(q, out, k, v, c, table, ops.prefix_plan([], 2, 4, 4, 64, BF, 2, "cuda"), 4, 2, 64)
+
+
+@pytest.mark.parametrize("dtype", [BF, F])
+def test_pages_not_worth_a_kernel_are_read_by_each(dtype, monkeypatch):
+    from gopherllm_b200 import ops
+    monkeypatch.setattr(ops, "PREFIX_SPARED_BYTES", 1 << 40)
+    H, G, D, groups = 4, 2, 64, [([0, 2], 640), ([1], 64)]
+    q, k, v, c, table = build(groups, [640 + 70, 64 + 7, 640], H, G, D, dtype, 12)
+    plan = ops.prefix_plan(groups, 3, H, G, D, dtype, 71, "cuda")
+    assert plan.layout.n_items == 0 and plan.layout.launches == 1
+    out = torch.full_like(q, float("nan"))
+    ops.attention_prefix(q, out, k, v, c, table, plan, H, G, D)
+    check(out, q, k, v, c, table, H, G, D)

@@ -12,8 +12,8 @@ pytestmark = pytest.mark.gpu
 @pytest.fixture
 def load(monkeypatch):
     import gopherllm_b200 as gl
-    from gopherllm_b200.engine import step
-    monkeypatch.setattr(step, "SHARED_POSITIONS", 1)               # (tiny models would never be worth it)
+    from gopherllm_b200 import ops
+    monkeypatch.setattr(ops, "PREFIX_SPARED_BYTES", 0)             # (tiny models would never be worth it)
     models = []
 
     def make(name, dtype, **kw):
