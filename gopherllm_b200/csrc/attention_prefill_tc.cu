@@ -105,6 +105,9 @@ struct AttnPlace {
     int chunk;                // > 0: a query sees the keys of its own chunk of positions alone (window is then 0)
 };
 
+// Each row's maximum, as a power of two and as of the last rescaling, and its sum of powers beside that: [nH, rows, 2] or null.
+struct AttnStats { float2* ml; int rows; };
+
 struct AttnMaps { CUtensorMap q[4], k[4], v; };
 
 __device__ __forceinline__ float at_exp2(float x) {
@@ -115,7 +118,7 @@ __device__ __forceinline__ float at_exp2(float x) {
 
 template <int NT>
 __global__ void __launch_bounds__(AT_THREADS(NT), 3 - NT)
-attn_prefill_tc_kernel(AttnArgs a, AttnGate gate, AttnPlace place, const __grid_constant__ AttnMaps maps) {
+attn_prefill_tc_kernel(AttnArgs a, AttnGate gate, AttnPlace place, AttnStats stats, const __grid_constant__ AttnMaps maps) {
     extern __shared__ unsigned char smem_raw[];
     __shared__ unsigned tmem_slot;
     __shared__ volatile int failed;
@@ -378,6 +381,7 @@ attn_prefill_tc_kernel(AttnArgs a, AttnGate gate, AttnPlace place, const __grid_
             if (ok) {
                 tc_fence_after();
                 const float inv = l_run > 0.f ? 1.f / l_run : 0.f;
+                if (stats.ml && r < rows) stats.ml[(size_t)h * stats.rows + qstart + q0 + t * AT_BM + r] = make_float2(m_run * LOG2E, l_run);
                 __nv_bfloat16* dst = (__nv_bfloat16*)a.out + ((size_t)(qstart + q0 + t * AT_BM + r) * a.nH + h) * AT_HD;
 #pragma unroll
                 for (int c = 0; c < AT_HD; c += 16) {
@@ -444,8 +448,8 @@ static bool at_allow() {
 }
 template <int NT>
 static int at_launch(long long blocks, cudaStream_t stream, const AttnArgs& a, const AttnGate& gate, const AttnPlace& place,
-                     const AttnMaps& maps) {
-    return gl_launch(attn_prefill_tc_kernel<NT>, dim3((unsigned)blocks), dim3(AT_THREADS(NT)), at_smem(NT), stream, 1, a, gate, place, maps);
+                     const AttnStats& stats, const AttnMaps& maps) {
+    return gl_launch(attn_prefill_tc_kernel<NT>, dim3((unsigned)blocks), dim3(AT_THREADS(NT)), at_smem(NT), stream, 1, a, gate, place, stats, maps);
 }
 
 // Tiles a block.  Blocks of one tile, two an SM, overlap one's start and end with the other's pages and share the work
@@ -459,7 +463,8 @@ static int at_choose(const AttnArgs& a, const AttnPlace& place, int sms) {
     return a.window > 0 || place.chunk > 0 || pairs < sms ? 1 : 2;
 }
 
-static int prefill_tc(const AttnArgs& a, const AttnGate& gate, const AttnPlace& place, int n_tokens, int n_pages, cudaStream_t stream) {
+static int prefill_tc(const AttnArgs& a, const AttnGate& gate, const AttnPlace& place, int n_tokens, int n_pages, cudaStream_t stream,
+                      const AttnStats& stats = {nullptr, 0}) {
     if (a.B <= 0 || a.max_qlen <= 0) return GL_OK;
     if (a.hd != AT_HD || a.nH <= 0 || a.nKV <= 0 || a.nH % a.nKV) return GL_ERR_SHAPE;
     if (!(a.score_scale > 0.f) || place.chunk < 0 || (place.chunk > 0 && a.window > 0)) return GL_ERR_SHAPE;
@@ -495,8 +500,8 @@ static int prefill_tc(const AttnArgs& a, const AttnGate& gate, const AttnPlace& 
     }
     const long long blocks = (long long)((a.max_qlen + nt * AT_BM - 1) / (nt * AT_BM)) * a.nH * a.B;
     if (blocks > 0x7fffffffLL) return GL_ERR_SHAPE;
-    const int rc = nt == 1 ? at_launch<(AT_ONE_TILE ? 1 : 2)>(blocks, stream, a, gate, place, maps)
-                           : at_launch<2>(blocks, stream, a, gate, place, maps);
+    const int rc = nt == 1 ? at_launch<(AT_ONE_TILE ? 1 : 2)>(blocks, stream, a, gate, place, stats, maps)
+                           : at_launch<2>(blocks, stream, a, gate, place, stats, maps);
     return rc == 0 ? GL_OK : GL_ERR_LAUNCH;
 }
 
@@ -519,4 +524,12 @@ GL_API int gl_attention_prefill_tc_gated(const AttnArgs* args, const AttnGate* g
 GL_API int gl_attention_prefill_tc_placed(const AttnArgs* args, const AttnPlace* place, int n_tokens, int n_pages, cudaStream_t stream) {
     const AttnGate none = {nullptr, 0, 0};
     return prefill_tc(*args, none, *place, n_tokens, n_pages, stream);
+}
+
+// the same, leaving each row's statistics behind (score_scale 1)
+GL_API int gl_attention_prefill_tc_stats(const AttnArgs* args, const AttnStats* stats, int n_tokens, int n_pages, cudaStream_t stream) {
+    if (!stats->ml || stats->rows < n_tokens || args->score_scale != 1.0f) return GL_ERR_SHAPE;
+    const AttnGate none = {nullptr, 0, 0};
+    const AttnPlace cache = {nullptr, 0, 0, 0, 0};
+    return prefill_tc(*args, none, cache, n_tokens, n_pages, stream, *stats);
 }

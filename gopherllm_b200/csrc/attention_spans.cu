@@ -107,6 +107,68 @@ __device__ __forceinline__ float4 sp_read(const float4* p) {
     return v;
 }
 
+
+// The end of a block whose split is one of a cluster: fin_o [rows][hd] and fin_ml [rows][2] are its result, in its shared memory.
+// The blocks put their results and what the shared pages gave together: every block the factors of all parts, a row a warp, then its
+// share of the outputs, four at a time.  held [rows][a.held]: its scores, which ``scale`` makes powers of two, or nothing; behind them room
+// for the factors; stat: room for [rows][2].
+struct SpanEnd { int seq, g, head, rows, p_begin, p_end, total; };
+__device__ __forceinline__ void span_join(const SpanArgs& a, const SpanEnd& e, const float* fin_o, const float* fin_ml, float* held, float* stat,
+                                          const int* pg, float scale) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rows = e.rows, b = e.seq;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int S = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+    const int n_pre = a.seq_shared ? a.seq_shared[2 * b + 1] : 0, parts = S + n_pre;
+    float* fac = held + (a.weights ? rows * a.held : 0);           // [rows][parts]: factor / sum
+    if (a.early) gl_grid_wait();
+    if (S > 1) cluster.sync();
+    else __syncthreads();
+    for (int r = warp; r < rows; r += blockDim.x / 32) {
+        const float2* pre = (const float2*)a.part_ml + ((size_t)b * a.nH + e.head + r) * a.slots - S;
+        auto part = [&](int k) { return k < S ? ((const float2*)(S > 1 ? cluster.map_shared_rank((float*)fin_ml, k) : fin_ml))[r] : sp_read(pre + k); };
+        float m = -INFINITY, l = 0.f;
+        for (int k = lane; k < parts; k += 32) m = fmaxf(m, part(k).x);
+        m = gl_warp_max(m);
+        for (int k = lane; k < parts; k += 32) {
+            const float2 ml = part(k);
+            const float f = sp_factor(ml.x, m);
+            fac[r * parts + k] = f;
+            l = fmaf(f, ml.y, l);
+        }
+        l = gl_warp_sum(l);
+        const float inv = l == 0.f ? 0.f : 1.0f / l;
+        for (int k = lane; k < parts; k += 32) fac[r * parts + k] *= inv;
+        if (lane == 0) { stat[2 * r] = m; stat[2 * r + 1] = inv; }
+    }
+    __syncthreads();
+    for (int i = tid * S + rank; i < rows * (SP_HD / 4); i += blockDim.x * S) {
+        const int r = i / (SP_HD / 4), c = i - r * (SP_HD / 4);
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+        auto add = [&](float f, const float4 v) {
+            sum.x = fmaf(f, v.x, sum.x); sum.y = fmaf(f, v.y, sum.y); sum.z = fmaf(f, v.z, sum.z); sum.w = fmaf(f, v.w, sum.w);
+        };
+        for (int k = 0; k < S; ++k) add(fac[r * parts + k], ((const float4*)(S > 1 ? cluster.map_shared_rank((float*)fin_o, k) : fin_o))[i]);
+        const float4* pre = (const float4*)a.part_o + (((size_t)b * a.nH + e.head + r) * a.slots) * (SP_HD / 4) + c;
+#pragma unroll 8
+        for (int k = 0; k < n_pre; ++k) add(fac[r * parts + S + k], sp_read(pre + (size_t)k * (SP_HD / 4)));
+        const __nv_bfloat162 lo = __floats2bfloat162_rn(sum.x, sum.y), hi = __floats2bfloat162_rn(sum.z, sum.w);
+        *(uint2*)(a.out + ((size_t)(a.seq_row ? a.seq_row[b] : b) * a.nH + e.head + r) * SP_HD + 4 * c) = make_uint2(*(const unsigned*)&lo, *(const unsigned*)&hi);
+    }
+    if (a.weights) {                                       // this block's scores become weights
+        const int n = min(min((e.p_end - e.p_begin) * GL_PAGE, e.total - e.p_begin * GL_PAGE), a.held);
+        for (int i = tid; i < n; i += blockDim.x) {
+            float given = 0.f;
+            for (int r = 0; r < rows; ++r) given = fmaf(sp_exp2(fmaf(held[r * a.held + i], scale, -stat[2 * r])), stat[2 * r + 1], given);
+            const int j = e.p_begin * GL_PAGE + i;
+            float* w = a.weights + ((size_t)gl_checked(pg[j / GL_PAGE], a.n_pages, GL_BAD_PAGE) * a.nKV + e.g) * GL_PAGE + j % GL_PAGE;
+            // (an addition that nobody waits for; one a position, so their order is no matter)
+            if (j < e.total - 1) atomicAdd(w, given);
+            else *w = given;
+        }
+    }
+    if (S > 1) cluster.sync();                             // a block's memory stays until its peers have read it
+}
+
 template <int NT>
 __host__ __device__ constexpr int sp_fixed_bytes() {       // queries, then per row: sequence, head, last position seen
     return 8 * NT * SP_ROW + 8 * NT * 12;
@@ -363,58 +425,8 @@ attn_span_kernel(SpanArgs a) {
         if (d == 0) { a.part_ml[at * 2] = m; a.part_ml[at * 2 + 1] = l; }
     }
     if (MODE != SP_JOIN) return;
-    // The blocks of the cluster put their results and what the shared pages gave together: every block the factors of all parts,
-    // a row a warp, then its share of the outputs, four at a time.
-    cg::cluster_group cluster = cg::this_cluster();
-    const int S = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-    const int b = table, n_pre = a.seq_shared ? a.seq_shared[2 * b + 1] : 0, parts = S + n_pre;
-    float* fac = held + (a.weights ? rows * a.held : 0);          // [rows][parts]: factor / sum
-    float* stat = ml_w;                                    // [rows][2]: maximum, 1 / sum (the warps' results are done with)
-    if (a.early) gl_grid_wait();
-    if (S > 1) cluster.sync();
-    else __syncthreads();
-    for (int r = warp; r < rows; r += SP_THREADS / 32) {
-        const float2* pre = (const float2*)a.part_ml + ((size_t)b * a.nH + row_head[r]) * a.slots - S;
-        auto part = [&](int k) { return k < S ? ((const float2*)(S > 1 ? cluster.map_shared_rank(fin_ml, k) : fin_ml))[r] : sp_read(pre + k); };
-        float m = -INFINITY, l = 0.f;
-        for (int k = lane; k < parts; k += 32) m = fmaxf(m, part(k).x);
-        m = gl_warp_max(m);
-        for (int k = lane; k < parts; k += 32) {
-            const float2 ml = part(k);
-            const float f = sp_factor(ml.x, m);
-            fac[r * parts + k] = f;
-            l = fmaf(f, ml.y, l);
-        }
-        l = gl_warp_sum(l);
-        const float inv = l == 0.f ? 0.f : 1.0f / l;
-        for (int k = lane; k < parts; k += 32) fac[r * parts + k] *= inv;
-        if (lane == 0) { stat[2 * r] = m; stat[2 * r + 1] = inv; }
-    }
-    __syncthreads();
-    for (int i = tid * S + rank; i < rows * (SP_HD / 4); i += SP_THREADS * S) {
-        const int r = i / (SP_HD / 4), c = i - r * (SP_HD / 4);
-        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-        auto add = [&](float f, const float4 v) {
-            sum.x = fmaf(f, v.x, sum.x); sum.y = fmaf(f, v.y, sum.y); sum.z = fmaf(f, v.z, sum.z); sum.w = fmaf(f, v.w, sum.w);
-        };
-        for (int k = 0; k < S; ++k) add(fac[r * parts + k], ((const float4*)(S > 1 ? cluster.map_shared_rank(fin_o, k) : fin_o))[i]);
-        const float4* pre = (const float4*)a.part_o + (((size_t)b * a.nH + row_head[r]) * a.slots) * (SP_HD / 4) + c;
-#pragma unroll 8
-        for (int k = 0; k < n_pre; ++k) add(fac[r * parts + S + k], sp_read(pre + (size_t)k * (SP_HD / 4)));
-        const __nv_bfloat162 lo = __floats2bfloat162_rn(sum.x, sum.y), hi = __floats2bfloat162_rn(sum.z, sum.w);
-        *(uint2*)(a.out + ((size_t)(a.seq_row ? a.seq_row[b] : b) * a.nH + row_head[r]) * SP_HD + 4 * c) = make_uint2(*(const unsigned*)&lo, *(const unsigned*)&hi);
-    }
-    if (a.weights) {                                       // this block's scores become weights
-        const int n = min(min((p_end - p_begin) * GL_PAGE, total - p_begin * GL_PAGE), a.held);
-        for (int i = tid; i < n; i += SP_THREADS) {
-            float given = 0.f;
-            for (int r = 0; r < rows; ++r) given = fmaf(sp_exp2(fmaf(held[r * a.held + i], SP_LOG2E, -stat[2 * r])), stat[2 * r + 1], given);
-            const int j = p_begin * GL_PAGE + i;
-            float* w = a.weights + ((size_t)gl_checked(pg[j / GL_PAGE], a.n_pages, GL_BAD_PAGE) * a.nKV + g) * GL_PAGE + j % GL_PAGE;
-            *w = j < total - 1 ? *w + given : given;
-        }
-    }
-    if (S > 1) cluster.sync();                             // a block's memory stays until its peers have read it
+    const SpanEnd e = {table, g, row_head[0], rows, p_begin, p_end, total};
+    span_join(a, e, fin_o, fin_ml, held, ml_w, pg, SP_LOG2E);
 }
 
 // The spans of a sequence put together: blockIdx = (share of the positions, key/value head, sequence).  The blocks of a head share its
@@ -457,8 +469,185 @@ attn_span_join_kernel(SpanArgs a) {
 #pragma unroll 4
         for (int i = 0; i < G; ++i) given = fmaf(sp_exp2(fmaf(sc[(size_t)i * a.reach], SP_LOG2E, -ml_all[2 * i])), ml_all[2 * i + 1], given);
         float* w = a.weights + ((size_t)gl_checked(a.pages[(size_t)b * a.max_pages + j / GL_PAGE], a.n_pages, GL_BAD_PAGE) * a.nKV + g) * GL_PAGE + j % GL_PAGE;
-        *w = j < pos ? *w + given : given;
+        if (j < pos) atomicAdd(w, given);                  // (one addition a position)
+        else *w = given;
     }
+}
+
+
+// ---------------------------------------------------------------------------
+// One or two query heads on a key/value head: a sequence's own pages go from the cache straight to registers, as in
+// attention_spans_f32.cu.  Eight lanes take a key, a warp four keys at a time with 2 UN of their rows under way; no barrier stands between
+// two keys, and the weights stay in 32 bits.  Eight columns of a tensor-core product would be empty but for one or two; what
+// bounds it is memory.
+// ---------------------------------------------------------------------------
+#define SW_CP ((SP_CHUNKS + 7) / 8)       // 16-byte pieces of a row that a lane takes
+#define SW_WARPS 4
+// eight bfloat16 numbers times eight others, added to x
+__device__ __forceinline__ float sw_dot(const uint4& k, const float (&q)[8], float x) {
+    const unsigned w[4] = {k.x, k.y, k.z, k.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x = fmaf(__uint_as_float(w[i] << 16), q[2 * i], fmaf(__uint_as_float(w[i] & 0xffff0000u), q[2 * i + 1], x));
+    return x;
+}
+__device__ __forceinline__ void sw_add(const uint4& v, float w, float (&o)[8]) {
+    const unsigned u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        o[2 * i] = fmaf(w, __uint_as_float(u[i] << 16), o[2 * i]);
+        o[2 * i + 1] = fmaf(w, __uint_as_float(u[i] & 0xffff0000u), o[2 * i + 1]);
+    }
+}
+template <int R>
+__host__ __device__ constexpr size_t sw_smem() { return sizeof(float) * (SW_WARPS + 1) * R * (SP_HD + 2); }
+
+template <int R, int MODE>
+__global__ void __launch_bounds__(32 * SW_WARPS)
+stream_span_kernel(SpanArgs a) {
+    extern __shared__ __align__(16) unsigned char smem[];
+    constexpr int UN = SW_CP * R <= 2 ? 4 : 2, RUN = 4 * UN;       // keys of a group of lanes, and of a warp, under way
+    float* o_w = (float*)smem;                                     // [4][R][hd] what the warps found, [4][R][2]; the block's result [R][hd], [R][2]
+    float* ml_w = o_w + SW_WARPS * R * SP_HD;
+    float* fin_o = ml_w + SW_WARPS * R * 2;
+    float* fin_ml = fin_o + R * SP_HD;
+    float* held = fin_ml + 2 * R;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, sub = lane & 7, grp = lane >> 3;
+    if (!a.early) gl_grid_wait();
+    gl_grid_launch_dependents();
+    const int b = blockIdx.z, g = blockIdx.y;
+    if (a.seq_qlen && a.seq_qlen[b] <= 0) return;
+    const int pos = a.seq_ctx[b], total = pos + 1, first = a.seq_shared ? a.seq_shared[2 * b] : 0;
+    const int n = max(0, pos / GL_PAGE + 1 - first), per = (n + a.splits - 1) / a.splits;
+    const int p_begin = first + (int)blockIdx.x * per, p_end = min(first + n, p_begin + per);
+    const int n_pre = a.seq_shared ? a.seq_shared[2 * b + 1] : 0, slot = n_pre + blockIdx.x;
+    const int* pg = a.pages + (size_t)b * a.max_pages;
+    const size_t q_row = (size_t)(a.seq_row ? a.seq_row[b] : b) * a.nH + g * R;
+    float q[R][SW_CP][8], o[R][SW_CP][8];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int c = 0; c < SW_CP; ++c) {
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (c * 8 + sub < SP_CHUNKS) v = *(const uint4*)(a.q + (q_row + r) * SP_HD + 8 * (c * 8 + sub));
+            const unsigned w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                q[r][c][2 * i] = __uint_as_float(w[i] << 16) * SP_LOG2E;      // (scores as powers of two)
+                q[r][c][2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u) * SP_LOG2E;
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) o[r][c][i] = 0.f;
+        }
+    float m[R], l[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) { m[r] = -INFINITY; l[r] = 0.f; }
+    const int k_end = min(p_end * GL_PAGE, total);
+    for (int j0 = p_begin * GL_PAGE + warp * RUN; j0 < k_end; j0 += SW_WARPS * RUN) {
+        const size_t at = (((size_t)gl_checked(pg[j0 / GL_PAGE], a.n_pages, GL_BAD_PAGE) * a.nKV + g) * GL_PAGE + j0 % GL_PAGE + grp) * SP_HD + 8 * sub;
+        uint4 k[UN][SW_CP], v[UN][SW_CP];
+#pragma unroll
+        for (int u = 0; u < UN; ++u)
+#pragma unroll
+            for (int c = 0; c < SW_CP; ++c) {
+                const bool ok = j0 + 4 * u + grp < k_end && c * 8 + sub < SP_CHUNKS;
+                k[u][c] = ok ? *(const uint4*)(a.k_cache + at + 4 * u * SP_HD + 64 * c) : make_uint4(0, 0, 0, 0);
+            }
+#pragma unroll
+        for (int u = 0; u < UN; ++u)
+#pragma unroll
+            for (int c = 0; c < SW_CP; ++c) {
+                const bool ok = j0 + 4 * u + grp < k_end && c * 8 + sub < SP_CHUNKS;
+                v[u][c] = ok ? *(const uint4*)(a.v_cache + at + 4 * u * SP_HD + 64 * c) : make_uint4(0, 0, 0, 0);
+            }
+        float s[R][UN];
+#pragma unroll
+        for (int u = 0; u < UN; ++u) {
+            const int j = j0 + 4 * u + grp;
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                float x = 0.f;
+#pragma unroll
+                for (int c = 0; c < SW_CP; ++c) x = sw_dot(k[u][c], q[r][c], x);
+                x += __shfl_xor_sync(0xffffffffu, x, 1);
+                x += __shfl_xor_sync(0xffffffffu, x, 2);
+                x += __shfl_xor_sync(0xffffffffu, x, 4);
+                if (a.weights && sub == r && j < k_end) {
+                    if (MODE == SP_JOIN) { if (j - p_begin * GL_PAGE < a.held) held[r * a.held + j - p_begin * GL_PAGE] = x; }
+                    else if (j < a.reach) a.scores[((size_t)b * a.nH + g * R + r) * a.reach + j] = x / SP_LOG2E;
+                }
+                s[r][u] = j < k_end ? x : -INFINITY;
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            float m_new = m[r];
+#pragma unroll
+            for (int u = 0; u < UN; ++u) m_new = fmaxf(m_new, s[r][u]);
+            const float mu = m_new == -INFINITY ? 0.f : m_new, corr = sp_factor(m[r], m_new);
+            if (__any_sync(0xffffffffu, m[r] != m_new)) {
+                l[r] *= corr;
+#pragma unroll
+                for (int c = 0; c < SW_CP; ++c)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) o[r][c][i] *= corr;
+            }
+            m[r] = m_new;
+#pragma unroll
+            for (int u = 0; u < UN; ++u) {
+                const float w = sp_exp2(s[r][u] - mu);
+                l[r] += w;
+#pragma unroll
+                for (int c = 0; c < SW_CP; ++c) sw_add(v[u][c], w, o[r][c]);
+            }
+        }
+    }
+    // the warp's four groups of lanes, then the warps
+#pragma unroll
+    for (int x = 8; x < 32; x <<= 1)
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const float om = __shfl_xor_sync(0xffffffffu, m[r], x), ol = __shfl_xor_sync(0xffffffffu, l[r], x), m_new = fmaxf(m[r], om);
+            const float f = sp_factor(m[r], m_new), of = sp_factor(om, m_new);
+            l[r] = l[r] * f + ol * of;
+            m[r] = m_new;
+#pragma unroll
+            for (int c = 0; c < SW_CP; ++c)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) o[r][c][i] = o[r][c][i] * f + __shfl_xor_sync(0xffffffffu, o[r][c][i], x) * of;
+        }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        if (lane == 0) *(float2*)(ml_w + (warp * R + r) * 2) = make_float2(m[r], l[r]);
+        if (grp == 0)
+#pragma unroll
+            for (int c = 0; c < SW_CP; ++c)
+                if (c * 8 + sub < SP_CHUNKS) {
+                    float4* dst = (float4*)(o_w + (warp * R + r) * SP_HD + 8 * (c * 8 + sub));
+                    dst[0] = make_float4(o[r][c][0], o[r][c][1], o[r][c][2], o[r][c][3]);
+                    dst[1] = make_float4(o[r][c][4], o[r][c][5], o[r][c][6], o[r][c][7]);
+                }
+    }
+    __syncthreads();
+    for (int i = tid; i < R * (SP_HD / 4); i += 32 * SW_WARPS) {
+        const int r = i / (SP_HD / 4), c = i - r * (SP_HD / 4);
+        float mm = -INFINITY, ll = 0.f;
+#pragma unroll
+        for (int w = 0; w < SW_WARPS; ++w) mm = fmaxf(mm, ml_w[(w * R + r) * 2]);
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < SW_WARPS; ++w) {
+            const float f = sp_factor(ml_w[(w * R + r) * 2], mm);
+            const float4 x = *(const float4*)(o_w + (w * R + r) * SP_HD + 4 * c);
+            sum.x = fmaf(f, x.x, sum.x); sum.y = fmaf(f, x.y, sum.y); sum.z = fmaf(f, x.z, sum.z); sum.w = fmaf(f, x.w, sum.w);
+            ll = fmaf(f, ml_w[(w * R + r) * 2 + 1], ll);
+        }
+        const size_t at = ((size_t)b * a.nH + g * R + r) * a.slots + slot;
+        *(float4*)(MODE == SP_JOIN ? fin_o + 4 * i : a.part_o + at * SP_HD + 4 * c) = sum;
+        if (c == 0) *(float2*)(MODE == SP_JOIN ? fin_ml + 2 * r : a.part_ml + at * 2) = make_float2(mm, ll);
+    }
+    if (MODE != SP_JOIN) return;
+    const SpanEnd e = {b, g, g * R, R, p_begin, p_end, total};
+    span_join(a, e, fin_o, fin_ml, held, ml_w, pg, 1.0f);
 }
 
 #define SP_HELD_BYTES (56 * 1024)                  // scores a block keeps in shared memory at most
@@ -482,8 +671,28 @@ static int launch_span(const SpanArgs& a, dim3 grid, int cluster, cudaStream_t s
     return gl_launch(attn_span_kernel<NT, MODE>, grid, dim3(SP_THREADS), smem, stream, cluster, a);
 }
 
+template <int R, int MODE>
+static int launch_stream(const SpanArgs& a, dim3 grid, int cluster, cudaStream_t stream) {
+    static bool allowed[64] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) { cudaGetLastError(); return GL_ERR_DRIVER; }
+    if (!allowed[dev]) {
+        if (cudaFuncSetAttribute(stream_span_kernel<R, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(sw_smem<R>() + SP_HELD_BYTES + SP_FACTOR_BYTES)) != cudaSuccess) {
+            cudaGetLastError();
+            return GL_ERR_SMEM;
+        }
+        allowed[dev] = true;
+    }
+    const size_t smem = sw_smem<R>() + (MODE == SP_JOIN ? sizeof(float) * ((a.weights ? (size_t)a.held * R : 0) + R * (size_t)(a.slots + a.splits)) : 0);
+    return gl_launch(stream_span_kernel<R, MODE>, grid, dim3(32 * SW_WARPS), smem, stream, cluster, a);
+}
+
 template <int MODE>
 static int launch_spans(const SpanArgs& a, int rows, dim3 grid, int cluster, cudaStream_t stream) {
+    if constexpr (MODE != SP_ITEM) {
+        if (a.nH == a.nKV) return launch_stream<1, MODE>(a, grid, cluster, stream);
+        if (a.nH == 2 * a.nKV) return launch_stream<2, MODE>(a, grid, cluster, stream);
+    }
     if (rows <= 8) return launch_span<1, MODE>(a, grid, cluster, stream);
     if (rows <= 16) return launch_span<2, MODE>(a, grid, cluster, stream);
     return launch_span<SP_MAX_NT, MODE>(a, grid, cluster, stream);
@@ -555,11 +764,11 @@ GL_API int gl_attention_weighed(const SpanArgs* args, cudaStream_t stream) {
 // Shared pages with many rows, on the 5th-generation tensor cores: the same partial results as attn_span_kernel<SP_ITEM>.
 //
 // A block takes 128 or 256 rows of an item (members x query heads, whatever their places in q) as one or two tiles and walks
-// the item's pages.  One warp feeds key and value pages by TMA through two rings; each tile has a thread of its own that issues
+// the item's pages.  One warp feeds key and value pages by TMA through a ring; each tile has a thread of its own that issues
 // tcgen05.mma: scores S = Q K^T (M 128, N 64) into one of two buffers in tensor memory, two pages ahead of the rows, and O += P V
 // (M 128, N = head size, the weights read from tensor memory where their scores were, the values MN-major as the cache holds
-// them).  Four warps a tile own a row a thread: no shuffles for maximum and sum.  The output in tensor memory is rescaled only
-// when a row's maximum has grown by 2^8.  All pages are seen whole, so there is no mask but for a caller whose sequences end inside.
+// them).  Four warps a tile own a row a thread: no shuffles for the sum, and a maximum only where a page needs one.  All
+// pages are seen whole, so there is no mask but for a caller whose sequences end inside.
 // Bound by the issue of the products (12 a page of 64 keys at a head size of 128) beside the powers, and by memory where one tile holds
 // all rows.  Waits are bounded; a block whose wait runs out records it, frees its tensor memory and returns.
 // ---------------------------------------------------------------------------
@@ -606,8 +815,8 @@ shared_tc_kernel(SpanArgs a, const __grid_constant__ StMaps maps) {
     constexpr int STAGES = st_stages(NT), PRODUCER = 4 * NT;
     const unsigned base = gl_smem_u32(smem);
     const unsigned sQ = base, sK = sQ + NT * ST_Q_BYTES, sV = sK + STAGES * ST_K_BYTES, bars = sV + STAGES * ST_V_BYTES;
-    const unsigned bar_kf = bars, bar_ke = bar_kf + 8 * STAGES, bar_vf = bar_ke + 8 * STAGES, bar_ve = bar_vf + 8 * STAGES;
-    const unsigned bar_t = bar_ve + 8 * STAGES;            // per tile: scores full [2], weights full [2], product done, output full, queries there
+    const unsigned bar_f = bars, bar_e = bar_f + 8 * STAGES;       // a page's keys and values are there; are done with
+    const unsigned bar_t = bar_e + 8 * STAGES;             // per tile: scores full [2], weights full [2], last product but one done, output full, queries there
 #define ST_SF(t, i) (bar_t + 64 * (t) + 8 * (i))
 #define ST_PF(t, i) (bar_t + 64 * (t) + 16 + 8 * (i))
 #define ST_PD(t) (bar_t + 64 * (t) + 32)
@@ -616,10 +825,7 @@ shared_tc_kernel(SpanArgs a, const __grid_constant__ StMaps maps) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         failed = 0;
-        for (int s = 0; s < STAGES; ++s) {
-            mbar_init(bar_kf + 8 * s, 1); mbar_init(bar_ke + 8 * s, NT);
-            mbar_init(bar_vf + 8 * s, 1); mbar_init(bar_ve + 8 * s, NT);
-        }
+        for (int s = 0; s < STAGES; ++s) { mbar_init(bar_f + 8 * s, 1); mbar_init(bar_e + 8 * s, NT); }
         for (int t = 0; t < NT; ++t) {
             for (int i = 0; i < 2; ++i) { mbar_init(ST_SF(t, i), 1); mbar_init(ST_PF(t, i), 4); }
             mbar_init(ST_PD(t), 1); mbar_init(ST_OF(t), 1); mbar_init(ST_QF(t), 4);
@@ -649,16 +855,14 @@ shared_tc_kernel(SpanArgs a, const __grid_constant__ StMaps maps) {
                 const int st = j % STAGES;
                 const unsigned par = ((j / STAGES) - 1) & 1;
                 const int row = (gl_checked(pg[j], a.n_pages, GL_BAD_PAGE) * a.nKV + g) * GL_PAGE;
-                if (j >= STAGES && !mbar_wait(bar_ke + 8 * st, par)) { failed = 1; break; }
-                mbar_expect_tx(bar_kf + 8 * st, GL_PAGE * SP_HD * 2);
+                if (j >= STAGES && !mbar_wait(bar_e + 8 * st, par)) { failed = 1; break; }
+                mbar_expect_tx(bar_f + 8 * st, GL_PAGE * SP_HD * 2 + ST_V_BYTES);       // zero fill counts
 #pragma unroll
                 for (int s = 0; s < ST_NSEG; ++s)
-                    tma_load_2d(sK + st * ST_K_BYTES + st_seg_base(s, GL_PAGE), &maps.k[s], st_seg(s).off, row, bar_kf + 8 * st);
-                if (j >= STAGES && !mbar_wait(bar_ve + 8 * st, par)) { failed = 1; break; }
-                mbar_expect_tx(bar_vf + 8 * st, ST_V_BYTES);                       // zero fill counts
+                    tma_load_2d(sK + st * ST_K_BYTES + st_seg_base(s, GL_PAGE), &maps.k[s], st_seg(s).off, row, bar_f + 8 * st);
 #pragma unroll
                 for (int c = 0; c < ST_VATOMS; ++c)
-                    tma_load_2d(sV + st * ST_V_BYTES + c * ST_VATOM_BYTES, &maps.v, 64 * c, row, bar_vf + 8 * st);
+                    tma_load_2d(sV + st * ST_V_BYTES + c * ST_VATOM_BYTES, &maps.v, 64 * c, row, bar_f + 8 * st);
             }
         }
     } else if (warp > PRODUCER) {
@@ -681,27 +885,30 @@ shared_tc_kernel(SpanArgs a, const __grid_constant__ StMaps maps) {
                     }
                 }
                 umma_commit(ST_SF(t, j & 1));
-                umma_commit(bar_ke + 8 * st);
             };
+            // What this thread does a page is what the kernel waits for, and a wait costs it some 250 clocks even where there is nothing to wait
+            // for, a commit 40: so a page's keys and values arrive together (that page's wait was made before its scores), go back
+            // together behind the second product, and the products done are announced by the scores behind them (a commit
+            // speaks for all that its thread issued before) but for the last product that has none.
             bool ok = nt == 0 || mbar_wait(ST_QF(t), 0);
             for (int j = 0; ok && j < 2 && j < nt; ++j) {
-                ok = mbar_wait(bar_kf + 8 * (j % STAGES), (j / STAGES) & 1);
+                ok = mbar_wait(bar_f + 8 * (j % STAGES), (j / STAGES) & 1);
                 if (ok) { tc_fence_after(); issue_scores(j); }
             }
-            for (int j = 0; ok && j < nt && !failed; ++j) {
+            for (int j = 0; ok && j < nt; ++j) {
                 const int st = j % STAGES;
-                ok = mbar_wait(ST_PF(t, j & 1), (j >> 1) & 1) && mbar_wait(bar_vf + 8 * st, (j / STAGES) & 1);
+                ok = mbar_wait(ST_PF(t, j & 1), (j >> 1) & 1);
                 if (!ok) break;
                 tc_fence_after();
                 const uint64_t dv = umma_smem_desc(sV + st * ST_V_BYTES, ST_VATOM_BYTES, 1024, 2);
 #pragma unroll
                 for (int k = 0; k < GL_PAGE / 16; ++k)
                     umma_bf16_tmem_a(tmem + 256 * t + 128, tmem + 256 * t + 64 * (j & 1) + 8 * k, dv + (uint64_t)((16 * 128) >> 4) * k, idesc_o, (j | k) ? 1u : 0u);
-                umma_commit(ST_PD(t));
+                umma_commit(bar_e + 8 * st);
+                if (j == nt - 2) umma_commit(ST_PD(t));
                 if (j == nt - 1) umma_commit(ST_OF(t));
-                umma_commit(bar_ve + 8 * st);
                 if (j + 2 < nt) {                          // over S_j and P_j, which the rows and the product above are done with
-                    ok = mbar_wait(bar_kf + 8 * ((j + 2) % STAGES), ((j + 2) / STAGES) & 1);
+                    ok = mbar_wait(bar_f + 8 * ((j + 2) % STAGES), ((j + 2) / STAGES) & 1);
                     if (!ok) break;
                     tc_fence_after();
                     issue_scores(j + 2);
@@ -710,10 +917,8 @@ shared_tc_kernel(SpanArgs a, const __grid_constant__ StMaps maps) {
             // a tile without rows still hands every page back, once it has been loaded
             for (int j = nt; ok && j < n && !failed; ++j) {
                 const int st = j % STAGES;
-                ok = mbar_wait(bar_kf + 8 * st, (j / STAGES) & 1);
-                if (ok) mbar_arrive(bar_ke + 8 * st);
-                ok = ok && mbar_wait(bar_vf + 8 * st, (j / STAGES) & 1);
-                if (ok) mbar_arrive(bar_ve + 8 * st);
+                ok = mbar_wait(bar_f + 8 * st, (j / STAGES) & 1);
+                if (ok) mbar_arrive(bar_e + 8 * st);
             }
             if (!ok) failed = 1;
         }
@@ -759,51 +964,51 @@ shared_tc_kernel(SpanArgs a, const __grid_constant__ StMaps maps) {
                 for (int i = 0; i < GL_PAGE; ++i)
                     if (j0 + i > last) sc[i] = -INFINITY;
             }
-            float mx8[8];
+            // The powers' reference is a maximum of an earlier page, whichever: what lies above it by less than 2^60 loses nothing, in the
+            // weights (bfloat16 has the range of 32 bits) or in the sums, and takes no search for the maximum.  The first page,
+            // and one whose sum says that a score lay higher, is done with its own maximum, the output rescaled.
+            float mu = m_run == -INFINITY ? 0.f : m_run, sum;
+            unsigned pk[32];
+            auto weigh = [&]() {
+                float ps4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int i = 0; i < 8; ++i) mx8[i] = sc[i];
-#pragma unroll
-            for (int i = 8; i < GL_PAGE; i += 8)
-#pragma unroll
-                for (int k = 0; k < 8; ++k) mx8[k] = fmaxf(mx8[k], sc[i + k]);
-            const float mx = fmaxf(fmaxf(fmaxf(mx8[0], mx8[1]), fmaxf(mx8[2], mx8[3])), fmaxf(fmaxf(mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7])));
-            const float m_new = fmaxf(m_run, mx * SP_LOG2E);
-            const bool rescale = __any_sync(0xffffffffu, m_new - m_run > 8.f);      // (-inf to finite: yes; -inf to -inf: no)
-            float corr = 1.f;
-            if (rescale && m_new != -INFINITY) {
-                corr = sp_exp2(m_run - m_new);
-                m_run = m_new;
-            }
-            const float mu = m_run == -INFINITY ? 0.f : m_run;
-            if (rescale && j >= 1) {
-                ok = mbar_wait(ST_PD(t), (j - 1) & 1);     // the products so far are complete
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) { failed = 1; alive = false; break; }
-                tc_fence_after();
-#pragma unroll
-                for (int c = 0; c < SP_HD; c += 16) {
-                    unsigned t16[16];
-                    tmem_ld16(tO + c, t16);
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) t16[i] = __float_as_uint(__uint_as_float(t16[i]) * corr);
-                    tmem_st16(tO + c, t16);
-                }
-            }
-            float ps4[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int c = 0; c < GL_PAGE; c += 32) {
-                unsigned pk[16];
-#pragma unroll
-                for (int i = 0; i < 32; i += 4) {
-                    const float e0 = sp_exp2(fmaf(sc[c + i], SP_LOG2E, -mu)), e1 = sp_exp2(fmaf(sc[c + i + 1], SP_LOG2E, -mu));
-                    const float e2 = sp_exp2(fmaf(sc[c + i + 2], SP_LOG2E, -mu)), e3 = sp_exp2(fmaf(sc[c + i + 3], SP_LOG2E, -mu));
+                for (int i = 0; i < GL_PAGE; i += 4) {
+                    const float e0 = sp_exp2(fmaf(sc[i], SP_LOG2E, -mu)), e1 = sp_exp2(fmaf(sc[i + 1], SP_LOG2E, -mu));
+                    const float e2 = sp_exp2(fmaf(sc[i + 2], SP_LOG2E, -mu)), e3 = sp_exp2(fmaf(sc[i + 3], SP_LOG2E, -mu));
                     ps4[0] += e0; ps4[1] += e1; ps4[2] += e2; ps4[3] += e3;
                     __nv_bfloat162 p0 = __floats2bfloat162_rn(e0, e1), p1 = __floats2bfloat162_rn(e2, e3);
                     pk[i / 2] = *(unsigned*)&p0; pk[i / 2 + 1] = *(unsigned*)&p1;
                 }
-                tmem_st16(tS + 64 * (j & 1) + c / 2, pk);
+                sum = (ps4[0] + ps4[1]) + (ps4[2] + ps4[3]);
+            };
+            weigh();
+            if (__any_sync(0xffffffffu, m_run == -INFINITY || !(sum <= 1.152921504606847e18f))) {
+                float mx = sc[0];
+#pragma unroll
+                for (int i = 1; i < GL_PAGE; ++i) mx = fmaxf(mx, sc[i]);
+                const float m_new = fmaxf(m_run, mx * SP_LOG2E), corr = sp_factor(m_run, m_new);
+                m_run = m_new;
+                mu = m_run == -INFINITY ? 0.f : m_run;
+                if (j >= 1) {
+                    // the products so far are complete: the scores behind them are there, or the last but one is announced
+                    ok = j + 1 < n ? mbar_wait(ST_SF(t, (j + 1) & 1), ((j + 1) >> 1) & 1) : mbar_wait(ST_PD(t), 0);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) { failed = 1; alive = false; break; }
+                    tc_fence_after();
+#pragma unroll
+                    for (int c = 0; c < SP_HD; c += 16) {
+                        unsigned t16[16];
+                        tmem_ld16(tO + c, t16);
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) t16[i] = __float_as_uint(__uint_as_float(t16[i]) * corr);
+                        tmem_st16(tO + c, t16);
+                    }
+                }
+                l_run *= corr;
+                weigh();
             }
-            l_run = l_run * corr + ((ps4[0] + ps4[1]) + (ps4[2] + ps4[3]));
+            tmem_st32(tS + 64 * (j & 1), pk);
+            l_run += sum;
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();
@@ -884,9 +1089,10 @@ struct RunArgs {
     const int* seq_qlen;          // [B]
     const int* seq_ctx;           // [B]
     const int* pages;             // [B, max_pages]
-    float* ml;                    // [rows, nH, 2]
+    float* ml;                    // [nH, rows, 2]: maximum, sum
     float* weights;               // [pages, nKV, GL_PAGE]
-    int B, nH, nKV, max_pages, n_pages, reach, last;
+    float* sums;                  // [parts, B, nKV, reach], where parts > 1
+    int B, nH, nKV, max_pages, n_pages, reach, last, parts, rows;
 };
 #define RW_ROWS 64                                  // rows of q of a tile
 
@@ -982,7 +1188,7 @@ run_stats_kernel(RunArgs a) {
         }
         const int row = row_lo + 8 * i;
         if (t == 0 && row < end) {
-            float* ml = a.ml + ((size_t)(row0 + row / G) * a.nH + g * G + row % G) * 2;
+            float* ml = a.ml + ((size_t)(g * G + row % G) * a.rows + row0 + row / G) * 2;
             ml[0] = m[i];
             ml[1] = l[i];
         }
@@ -1010,7 +1216,7 @@ run_weigh_kernel(RunArgs a) {
         if (tid < RW_ROWS) {
             const int row = r0 + tid;
             float2 ml = make_float2(0.f, 1.f);
-            if (row < end) ml = *(const float2*)(a.ml + ((size_t)(row0 + row / G) * a.nH + g * G + row % G) * 2);
+            if (row < end) ml = *(const float2*)(a.ml + ((size_t)(g * G + row % G) * a.rows + row0 + row / G) * 2);
             stat[(i & 1) * 2 * RW_ROWS + 2 * tid] = ml.x;
             stat[(i & 1) * 2 * RW_ROWS + 2 * tid + 1] = 1.0f / ml.y;
         }
@@ -1075,13 +1281,331 @@ run_weigh_kernel(RunArgs a) {
     sp_wait<0>();
 }
 
+// The same on the 5th-generation tensor cores, for heads of up to 128: a block has 128 keys (two pages) and walks the run's queries
+// 128 at a time, head by head of the key/value head; S = Q K^T (M 128, N 128) goes to one of two buffers in tensor memory.  A thread
+// owns a row, whose statistics it holds in registers, and a quarter of the keys, whose sums over its rows it holds in 32 more: per score
+// one FMA, one power, one FMA, and no shared memory (with a key a thread the queries' statistics come from shared memory, which
+// takes as long as the powers).  At the end the 128 rows' sums are added up in a fixed order.  2,048 tokens, 32 heads of 80: 36 us, of
+// which the powers (16 a clock and SM) need 17; the rest is what a warp does between two tiles.  Where there are few keys and heads the queries are shared
+// out among ``parts`` blocks, whose sums a last kernel adds up in order.  Waits are bounded, as above.
+#if SP_HD <= 128
+#define RT_WARPS 16                       // four times four warps of rows, each four with a quarter of the keys
+#define RT_COLS 32
+#define RT_THREADS (32 * RT_WARPS + 64)   // and one that feeds shared memory, one that issues
+#define RT_TILE_BYTES ST_Q_BYTES          // 128 rows of keys, or of queries
+__host__ __device__ constexpr int rt_stages() { return 200 * 1024 / RT_TILE_BYTES - 2 > 6 ? 6 : 200 * 1024 / RT_TILE_BYTES - 2; }
+static_assert(rt_stages() >= 3, "shared memory holds too few queries");
+struct RtMaps { CUtensorMap q[4], k[4]; };
+
+// The sum over a warp's lanes of v[i]: lane l ends with that of column l.
+__device__ __forceinline__ float rt_sum_lanes(float (&v)[RT_COLS], int lane) {
+#pragma unroll
+    for (int n = 16; n >= 1; n >>= 1) {                    // a lane keeps half of its columns and takes its partner's share of them
+        const bool up = lane & n;
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            if (i < n) {
+                const float give = up ? v[i] : v[i + n], keep = up ? v[i + n] : v[i];
+                v[i] = keep + __shfl_xor_sync(0xffffffffu, give, n);
+            }
+    }
+    return v[0];
+}
+
+// An item is a block of 128 keys of a key/value head and a share of the queries that see them.
+struct RtItem { int g, b, k0, part, qlen, ctx, row0, start, n_q, t0, n; };
+__device__ __forceinline__ RtItem rt_item(const RunArgs& a, int i) {
+    RtItem x;
+    const int G = a.nH / a.nKV;
+    x.g = i % a.nKV; i /= a.nKV;
+    x.b = i % a.B; i /= a.B;
+    x.part = i % a.parts;
+    x.k0 = i / a.parts * ST_BM;
+    x.qlen = a.seq_qlen[x.b]; x.ctx = a.seq_ctx[x.b]; x.row0 = a.seq_row[x.b];
+    x.start = max(max(0, x.k0 - x.ctx), a.last > 0 ? x.qlen - a.last : 0);
+    x.n_q = (x.qlen - x.start + ST_BM - 1) / ST_BM;
+    const int all = x.n_q > 0 && x.k0 < x.ctx + x.qlen ? x.n_q * G : 0;
+    // its tiles: head by head, queries rising
+    x.t0 = (int)((long long)all * x.part / a.parts);
+    x.n = (int)((long long)all * (x.part + 1) / a.parts) - x.t0;
+    return x;
+}
+
+// A block an SM takes items in turn.  The items are numbered with the keys' positions as the slowest index, so those that most
+// queries see come first, and dealt out forwards and backwards in turn, which evens their sums out; while the rows add up
+// one item's sums, the next one's keys and scores are under way.
+__global__ void __launch_bounds__(RT_THREADS, 1)
+run_weigh_tc_kernel(RunArgs a, int n_items, const __grid_constant__ RtMaps maps) {
+    extern __shared__ unsigned char smem_raw[];
+    __shared__ unsigned tmem_slot;
+    __shared__ volatile int failed;
+    __shared__ __align__(8) float sums[2][RT_WARPS][RT_COLS];
+    unsigned char* smem = smem_raw + ((1024u - (gl_smem_u32(smem_raw) & 1023u)) & 1023u);
+    constexpr int STAGES = rt_stages(), PRODUCER = RT_WARPS;
+    const unsigned sK = gl_smem_u32(smem), sQ = sK + 2 * RT_TILE_BYTES, bars = sQ + STAGES * RT_TILE_BYTES;
+    const unsigned bar_kf = bars, bar_ke = bars + 16, bar_sf = bars + 32, bar_se = bars + 48, bar_qf = bars + 64, bar_qe = bar_qf + 8 * STAGES;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        failed = 0;
+        for (int s = 0; s < STAGES; ++s) { mbar_init(bar_qf + 8 * s, 1); mbar_init(bar_qe + 8 * s, 1); }
+        for (int s = 0; s < 2; ++s) { mbar_init(bar_kf + 8 * s, 1); mbar_init(bar_ke + 8 * s, 1); mbar_init(bar_sf + 8 * s, 1); mbar_init(bar_se + 8 * s, RT_WARPS); }
+        mbar_fence_init();
+    }
+    if (warp == PRODUCER) tmem_alloc(gl_smem_u32(&tmem_slot), 256);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const unsigned tmem = tmem_slot;
+    gl_grid_wait();
+    gl_grid_launch_dependents();
+    const int G = a.nH / a.nKV;
+    auto item_of = [&](int round) { return round * (int)gridDim.x + (round & 1 ? (int)gridDim.x - 1 - (int)blockIdx.x : (int)blockIdx.x); };
+    const int rounds = (n_items + gridDim.x - 1) / gridDim.x;
+
+    if (warp == PRODUCER) {
+        if (lane == 0) {
+            int j = 0, k = 0;                              // tiles and items so far
+            bool ok = true;
+            for (int round = 0; round < rounds && ok && !failed; ++round) {
+                if (item_of(round) >= n_items) continue;
+                const RtItem x = rt_item(a, item_of(round));
+                if (x.n == 0) continue;
+                const int* pg = a.pages + (size_t)x.b * a.max_pages;
+                const int total = x.ctx + x.qlen, kb = k & 1;
+                if (k >= 2 && !(ok = mbar_wait(bar_ke + 8 * kb, ((k >> 1) - 1) & 1))) break;
+                mbar_expect_tx(bar_kf + 8 * kb, ST_BM * SP_HD * 2);
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const int p = x.k0 / GL_PAGE + half, page = gl_checked(pg[p * GL_PAGE < total ? p : x.k0 / GL_PAGE], a.n_pages, GL_BAD_PAGE);
+#pragma unroll
+                    for (int s = 0; s < ST_NSEG; ++s)
+                        tma_load_2d(sK + kb * RT_TILE_BYTES + st_seg_base(s, ST_BM) + half * GL_PAGE * st_seg(s).width * 2, &maps.k[s], st_seg(s).off,
+                                    (page * a.nKV + x.g) * GL_PAGE, bar_kf + 8 * kb);
+                }
+                ++k;
+                int h = x.g * G + x.t0 / x.n_q, i0 = x.start + x.t0 % x.n_q * ST_BM;
+                for (int i = 0; i < x.n; ++i, ++j) {
+                    const int st = j % STAGES;
+                    if (j >= STAGES && !(ok = mbar_wait(bar_qe + 8 * st, ((j / STAGES) - 1) & 1))) break;
+                    mbar_expect_tx(bar_qf + 8 * st, ST_BM * SP_HD * 2);
+#pragma unroll
+                    for (int s = 0; s < ST_NSEG; ++s)
+                        tma_load_2d(sQ + st * RT_TILE_BYTES + st_seg_base(s, ST_BM), &maps.q[s], h * SP_HD + st_seg(s).off, x.row0 + i0, bar_qf + 8 * st);
+                    i0 += ST_BM;
+                    if (i0 >= x.qlen) { i0 = x.start; ++h; }
+                }
+            }
+            if (!ok) failed = 1;
+        }
+    } else if (warp == PRODUCER + 1) {
+        if (lane == 0) {
+            constexpr uint32_t idesc = umma_idesc_bf16(ST_BM, 0);
+            int j = 0, k = 0;
+            bool ok = true;
+            for (int round = 0; round < rounds && ok && !failed; ++round) {
+                if (item_of(round) >= n_items) continue;
+                const int n = rt_item(a, item_of(round)).n, kb = k & 1;
+                if (n == 0) continue;
+                ok = mbar_wait(bar_kf + 8 * kb, (k >> 1) & 1);
+                for (int i = 0; ok && i < n; ++i, ++j) {
+                    const int st = j % STAGES;
+                    ok = mbar_wait(bar_qf + 8 * st, (j / STAGES) & 1) && (j < 2 || mbar_wait(bar_se + 8 * (j & 1), ((j >> 1) - 1) & 1));
+                    if (!ok) break;
+                    tc_fence_after();
+                    bool begin = true;
+#pragma unroll
+                    for (int s = 0; s < ST_NSEG; ++s) {
+                        const int rb = st_seg(s).width * 2;
+                        const uint64_t dk = umma_tile_desc(sK + kb * RT_TILE_BYTES + st_seg_base(s, ST_BM), rb);
+                        const uint64_t dq = umma_tile_desc(sQ + st * RT_TILE_BYTES + st_seg_base(s, ST_BM), rb);
+#pragma unroll
+                        for (int c = 0; c < st_seg(s).width / 16; ++c) {
+                            umma_bf16(tmem + ST_BM * (j & 1), dq + 2 * c, dk + 2 * c, idesc, begin ? 0u : 1u);
+                            begin = false;
+                        }
+                    }
+                    umma_commit(bar_sf + 8 * (j & 1));
+                    umma_commit(bar_qe + 8 * st);
+                }
+                if (ok) umma_commit(bar_ke + 8 * kb);
+                ++k;
+            }
+            if (!ok) failed = 1;
+        }
+    } else {
+        const int r = (warp & 3) * 32 + lane, col = (warp >> 2) * RT_COLS;      // the row of each tile, the first of its keys
+        const unsigned tS = tmem + ((unsigned)((warp & 3) * 32) << 16) + col;
+        // What an item needs of global memory is asked for while the one before is under way, and its sums leave by additions that nobody
+        // waits for: every stall here would be the tensor core's too.  (One addition a position: their order is no matter.)
+        auto skipped = [&](const RtItem& x) { return x.n == 0 && (a.parts == 1 || x.k0 >= x.ctx + x.qlen || x.qlen <= 0); };
+        auto item_from = [&](int& round) {                 // the next item with something to do, from ``round`` on
+            RtItem x = {};
+            for (; round < rounds; ++round) {
+                if (item_of(round) >= n_items) continue;
+                x = rt_item(a, item_of(round));
+                if (!skipped(x)) break;
+            }
+            return x;
+        };
+        int j = 0, round = 0, done = 0;
+        bool ok = true;
+        RtItem x = item_from(round);
+        // the rows' statistics, a tile ahead of the scores: where the next tile's lie, and how many tiles its head has left
+        const float2* at = nullptr;
+        int f0 = 0, left = 0;
+        auto begin = [&](const RtItem& y) {
+            const int q = y.n > 0 ? y.t0 % y.n_q : 0, h = y.g * G + (y.n > 0 ? y.t0 / y.n_q : 0);
+            f0 = y.start + q * ST_BM + r;
+            at = (const float2*)a.ml + (size_t)h * a.rows + y.row0 + f0;
+            left = y.n_q - q;
+        };
+        auto fetch = [&](const RtItem& y) {
+            const float2 v = f0 < y.qlen ? *at : make_float2(0.f, 1.f);
+            at += ST_BM;
+            f0 += ST_BM;
+            if (--left == 0) {                             // on to the next head's first tile
+                at += a.rows - y.n_q * ST_BM;
+                f0 -= y.n_q * ST_BM;
+                left = y.n_q;
+            }
+            return v;
+        };
+        auto page_of = [&](const RtItem& y) {              // of the key whose sum this thread writes
+            const int key = y.k0 + threadIdx.x;
+            return threadIdx.x < ST_BM && key < y.ctx + y.qlen ? gl_checked(a.pages[(size_t)y.b * a.max_pages + key / GL_PAGE], a.n_pages, GL_BAD_PAGE) : 0;
+        };
+        float2 next = make_float2(0.f, 1.f);
+        int page = 0;
+        if (round < rounds) {
+            begin(x);
+            if (x.n > 0) next = fetch(x);
+            page = page_of(x);
+        }
+        while (round < rounds) {
+            int after = round + 1;
+            const RtItem y = item_from(after);             // (the one behind)
+            const int total = x.ctx + x.qlen;
+            // of this thread's keys the row of the tile at i0 sees the first i0 + r + ahead; none if there is no such query
+            const int ahead = x.ctx - x.k0 - col + 1, sure = RT_COLS - ahead - (warp & 3) * 32, end = x.qlen - (warp & 3) * 32 - 31;
+            int i0 = x.start + (x.n > 0 ? x.t0 % x.n_q * ST_BM : 0);
+            float acc[RT_COLS];
+#pragma unroll
+            for (int i = 0; i < RT_COLS; ++i) acc[i] = 0.f;
+            for (int i = 0; i < x.n; ++i, ++j) {
+                const float m = next.x, inv = __fdividef(1.0f, next.y);
+                if (i + 1 < x.n) next = fetch(x);
+                // (a warp whose wait ran out goes on through the motions: the others meet it at the barrier)
+                ok = ok && mbar_wait(bar_sf + 8 * (j & 1), (j >> 1) & 1);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) continue;
+                tc_fence_after();
+                unsigned su[RT_COLS];
+                tmem_ld32(tS + ST_BM * (j & 1), su);
+                tc_fence_before();                         // (all read: the buffer may be written again)
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar_se + 8 * (j & 1));
+                if (i0 >= sure && i0 < end) {              // the warp's rows are there and see all of its keys
+#pragma unroll
+                    for (int q = 0; q < RT_COLS; ++q) acc[q] = fmaf(sp_exp2(fmaf(__uint_as_float(su[q]), SP_LOG2E, -m)), inv, acc[q]);
+                } else {
+                    const int seen = i0 + r < x.qlen ? i0 + r + ahead : 0;
+#pragma unroll
+                    for (int q = 0; q < RT_COLS; ++q) {
+                        const float e = sp_exp2(fmaf(__uint_as_float(su[q]), SP_LOG2E, -m)) * inv;
+                        acc[q] += q < seen ? e : 0.f;
+                    }
+                }
+                i0 += ST_BM;
+                if (i0 >= x.qlen) i0 = x.start;
+            }
+            if (!ok) failed = 1;
+            const int mine = page;
+            if (after < rounds) {
+                begin(y);
+                if (y.n > 0) next = fetch(y);
+                page = page_of(y);
+            }
+            sums[done & 1][warp][lane] = rt_sum_lanes(acc, lane);
+            asm volatile("bar.sync 1, %0;" ::"n"(32 * RT_WARPS) : "memory");
+            const int key = x.k0 + threadIdx.x;
+            if (threadIdx.x < ST_BM && key < total && !failed) {
+                const float (*f)[RT_COLS] = &sums[done & 1][threadIdx.x / RT_COLS * 4];
+                const int c = threadIdx.x % RT_COLS;
+                const float given = (f[0][c] + f[1][c]) + (f[2][c] + f[3][c]);
+                if (a.parts > 1) {
+                    if (key < a.reach) a.sums[(((size_t)x.part * a.B + x.b) * a.nKV + x.g) * a.reach + key] = given;
+                } else {
+                    float* w = a.weights + ((size_t)mine * a.nKV + x.g) * GL_PAGE + key % GL_PAGE;
+                    if (key < x.ctx) atomicAdd(w, given);
+                    else *w = given;
+                }
+            }
+            x = y;
+            round = after;
+            ++done;
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == PRODUCER) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 256);
+    }
+    if (threadIdx.x == 0 && failed) atomicExch(&gl_wait_failed, 1);
+}
+
+// the parts' sums, in order: blockIdx = (stretch of the positions, key/value head, sequence)
+__global__ void run_weigh_join_kernel(RunArgs a) {
+    gl_grid_wait();
+    gl_grid_launch_dependents();
+    const int b = blockIdx.z, g = blockIdx.y, j = blockIdx.x * blockDim.x + threadIdx.x;
+    const int ctx = a.seq_ctx[b], qlen = a.seq_qlen[b];
+    if (qlen <= 0 || j >= min(ctx + qlen, a.reach)) return;
+    float given = 0.f;
+    for (int p = 0; p < a.parts; ++p) given += a.sums[(((size_t)p * a.B + b) * a.nKV + g) * a.reach + j];
+    float* w = a.weights + ((size_t)gl_checked(a.pages[(size_t)b * a.max_pages + j / GL_PAGE], a.n_pages, GL_BAD_PAGE) * a.nKV + g) * GL_PAGE + j % GL_PAGE;
+    *w = j < ctx ? *w + given : given;
+}
+
+static int launch_run_tc(const RunArgs& a, int n_tokens, int sms, cudaStream_t stream) {
+    RtMaps maps;
+    const uint64_t kv_rows = (uint64_t)a.n_pages * a.nKV * GL_PAGE;
+    if (kv_rows > 0x7fffffffULL || a.parts < 1 || a.parts > 65535 || (a.parts > 1 && !a.sums)) return GL_ERR_SHAPE;
+    for (int s = 0; s < ST_NSEG; ++s) {
+        int rc = gl_cached_map(&maps.k[s], a.k_cache, kv_rows, SP_HD, GL_PAGE, st_seg(s).width, 2);
+        if (rc == GL_OK) rc = gl_cached_map(&maps.q[s], a.q, (uint64_t)n_tokens, (uint64_t)a.nH * SP_HD, ST_BM, st_seg(s).width, 2);
+        if (rc != GL_OK) return rc;
+    }
+    static bool allowed[64] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) { cudaGetLastError(); return GL_ERR_DRIVER; }
+    const size_t smem = (size_t)RT_TILE_BYTES * (2 + rt_stages()) + 16 * rt_stages() + 64 + 1024;
+    if (!allowed[dev]) {
+        if (cudaFuncSetAttribute(run_weigh_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) {
+            cudaGetLastError();
+            return GL_ERR_SMEM;
+        }
+        allowed[dev] = true;
+    }
+    const long long items = (long long)((a.reach + ST_BM - 1) / ST_BM) * a.nKV * a.B * a.parts;
+    if (items > 0x3fffffffLL || sms < 1) return GL_ERR_SHAPE;
+    const int rc = gl_launch(run_weigh_tc_kernel, dim3((unsigned)(items < sms ? items : sms)), dim3(RT_THREADS), smem, stream, 1, a, (int)items, maps);
+    if (rc != GL_OK || a.parts == 1) return rc;
+    return gl_launch(run_weigh_join_kernel, dim3((a.reach + 255) / 256, a.nKV, a.B), dim3(256), 0, stream, 1, a);
+}
+#else
+static int launch_run_tc(const RunArgs&, int, int, cudaStream_t) { return GL_ERR_SHAPE; }
+#endif
+
 #define RW_SMEM (3 * SP_TILE + 2 * RW_ROWS * 2 * 4)
-// The weights of runs of up to max_qlen tokens whose attention has been computed (ml: scratch).
-GL_API int gl_attention_weigh_runs(const RunArgs* args, int max_qlen, cudaStream_t stream) {
+// The weights of runs of up to max_qlen tokens whose attention has been computed.  known: ml holds the rows' statistics already (the
+// tcgen05 attention left them), else they are computed into it.  tensor > 0: on tcgen05, on that many SMs (heads of up to 128; known).
+GL_API int gl_attention_weigh_runs(const RunArgs* args, int max_qlen, int n_tokens, int known, int tensor, cudaStream_t stream) {
     const RunArgs& a = *args;
     if (a.B <= 0 || max_qlen <= 0) return GL_OK;
     if (a.nH <= 0 || a.nKV <= 0 || a.nH % a.nKV || a.B > 65535 || a.nKV > 65535 || a.reach <= 0 || a.last < 0 || !a.ml || !a.weights) return GL_ERR_SHAPE;
-    if (((uintptr_t)a.q | (uintptr_t)a.k_cache) & 15) return GL_ERR_ALIGN;
+    if (((uintptr_t)a.q | (uintptr_t)a.k_cache) & 15 || (uintptr_t)a.ml & 7) return GL_ERR_ALIGN;
+    if (tensor) return known ? launch_run_tc(a, n_tokens, tensor, stream) : GL_ERR_SHAPE;
     static bool allowed[64] = {};
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) { cudaGetLastError(); return GL_ERR_DRIVER; }
@@ -1093,10 +1617,12 @@ GL_API int gl_attention_weigh_runs(const RunArgs* args, int max_qlen, cudaStream
         }
         allowed[dev] = true;
     }
-    const int counted = a.last > 0 && a.last < max_qlen ? a.last : max_qlen;
-    const long long tiles = ((long long)counted * (a.nH / a.nKV) + RW_ROWS - 1) / RW_ROWS;
-    if (tiles > 0x7fffffffLL) return GL_ERR_SHAPE;
-    const int rc = gl_launch(run_stats_kernel, dim3((unsigned)tiles, a.nKV, a.B), dim3(SP_THREADS), (size_t)RW_SMEM, stream, 1, a);
-    if (rc != GL_OK) return rc;
+    if (!known) {
+        const int counted = a.last > 0 && a.last < max_qlen ? a.last : max_qlen;
+        const long long tiles = ((long long)counted * (a.nH / a.nKV) + RW_ROWS - 1) / RW_ROWS;
+        if (tiles > 0x7fffffffLL) return GL_ERR_SHAPE;
+        const int rc = gl_launch(run_stats_kernel, dim3((unsigned)tiles, a.nKV, a.B), dim3(SP_THREADS), (size_t)RW_SMEM, stream, 1, a);
+        if (rc != GL_OK) return rc;
+    }
     return gl_launch(run_weigh_kernel, dim3((a.reach + GL_PAGE - 1) / GL_PAGE, a.nKV, a.B), dim3(SP_THREADS), (size_t)RW_SMEM, stream, 1, a);
 }

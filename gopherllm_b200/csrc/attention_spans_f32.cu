@@ -302,7 +302,8 @@ span_f32_join_kernel(SpanF32Args a) {
 #pragma unroll 4
         for (int i = 0; i < G; ++i) given += expf(sc[(size_t)i * a.reach] - sf[2 * i]) / sf[2 * i + 1];
         float* w = a.weights + ((size_t)gl_checked(a.pages[(size_t)b * a.max_pages + j / GL_PAGE], a.n_pages, GL_BAD_PAGE) * a.nKV + g) * GL_PAGE + j % GL_PAGE;
-        *w = j < pos ? *w + given : given;
+        if (j < pos) atomicAdd(w, given);                          // (one addition a position)
+        else *w = given;
     }
 }
 
@@ -577,7 +578,8 @@ stream_f32_kernel(SpanF32Args a) {
             for (int r = 0; r < rows; ++r) given += expf(held[r * a.held + i] - stat[2 * r]) / stat[2 * r + 1];
             const int j = p_begin * GL_PAGE + i;
             float* w = a.weights + ((size_t)gl_checked(pg[j / GL_PAGE], a.n_pages, GL_BAD_PAGE) * a.nKV + g) * GL_PAGE + j % GL_PAGE;
-            *w = j < total - 1 ? *w + given : given;
+            if (j < total - 1) atomicAdd(w, given);               // (nobody waits for it; one a position, so their order is no matter)
+            else *w = given;
         }
     }
     if (S > 1) cluster.sync();

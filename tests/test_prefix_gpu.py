@@ -176,3 +176,20 @@ def test_pages_not_worth_a_kernel_are_read_by_each(dtype, monkeypatch):
     out = torch.full_like(q, float("nan"))
     ops.attention_prefix(q, out, k, v, c, table, plan, H, G, D)
     check(out, q, k, v, c, table, H, G, D)
+
+
+@pytest.mark.parametrize("dtype,H,G,D,members", [(BF, 4, 4, 64, 40), (BF, 8, 1, 128, 40), (BF, 4, 2, 64, 3), (F, 4, 2, 64, 6)])
+@pytest.mark.parametrize("rise", [30.0, -30.0])
+def test_scores_that_rise_or_fall_from_page_to_page(dtype, H, G, D, members, rise):
+    """Each page's scores lie e^+-30 and more above the page's before: every page of a span has its own maximum to deal with, and all but the
+    largest few weights vanish."""
+    from gopherllm_b200 import ops
+    groups = [(list(range(members)), 64 * 7)]
+    q, k, v, c, table = build(groups, [64 * 7 + b % 70 for b in range(members)], H, G, D, dtype, 13)
+    with torch.no_grad():
+        q.view(members, H, D)[..., 0] = 1.0
+        for p in range(table.shape[1]):
+            k[table[0, p].long(), :, :, 0] += rise * p
+    out = torch.full_like(q, float("nan"))
+    ops.attention_prefix(q, out, k, v, c, table, ops.prefix_plan(groups, members, H, G, D, dtype, 70, "cuda"), H, G, D)
+    check(out, q, k, v, c, table, H, G, D)
