@@ -34,9 +34,6 @@ static_assert(GL_HEAD_DIM % 16 == 0 && GL_HEAD_DIM >= 16 && GL_HEAD_DIM <= 256, 
 #define SP_CHUNKS (SP_HD / 8)                       // 16-byte pieces of a row
 #define SP_ROW (SP_HD * 2 + 16)                     // padded row in bytes: conflict-free ldmatrix
 #define SP_TILE (GL_PAGE * SP_ROW)                  // one page of keys (or values) of one head
-#ifndef SP_STAGES
-#define SP_STAGES 2                                 // pages of keys and values in flight
-#endif
 #define SP_MAX_NT (SP_HD <= 128 ? 4 : 2)            // columns of 8 rows: the accumulators of more do not fit the registers
 #define SP_LOG2E 1.4426950408889634f
 
@@ -57,6 +54,7 @@ struct SpanArgs {
     float* scores;                // [B, nH, reach] or null
     float* weights;               // [pages, nKV, GL_PAGE] or null
     int B, nH, nKV, max_pages, n_pages, n_items, splits, slots, chunks, reach;
+    int short_spans;              // a block has a page or two to walk
     int early, held;              // set by the launchers: see the kernel
 };
 
@@ -173,9 +171,9 @@ template <int NT>
 __host__ __device__ constexpr int sp_fixed_bytes() {       // queries, then per row: sequence, head, last position seen
     return 8 * NT * SP_ROW + 8 * NT * 12;
 }
-template <int NT>
+template <int NT, int STAGES>
 __host__ __device__ constexpr size_t sp_smem() {
-    const size_t pages = 2 * SP_STAGES * (size_t)SP_TILE;
+    const size_t pages = 2 * STAGES * (size_t)SP_TILE;
     const size_t merge = sizeof(float) * (4 * 8 * NT * 2 + 5 * (size_t)SP_HD * 8 * NT + 8 * NT * 2);       // over the pages, when they are done
     return (pages > merge ? pages : merge) + sp_fixed_bytes<NT>();
 }
@@ -186,18 +184,18 @@ __host__ __device__ constexpr size_t sp_smem() {
 // distributed shared memory, take in what the shared pages gave and write the output.
 enum { SP_ITEM = 0, SP_SPLIT = 1, SP_JOIN = 2 };
 
-template <int NT, int MODE>
+template <int NT, int MODE, int STAGES>
 __global__ void __launch_bounds__(SP_THREADS)
 attn_span_kernel(SpanArgs a) {
     extern __shared__ __align__(16) unsigned char smem[];
     constexpr bool SHARED = MODE == SP_ITEM;
-    constexpr size_t AREA = sp_smem<NT>() - sp_fixed_bytes<NT>();
+    constexpr size_t AREA = sp_smem<NT, STAGES>() - sp_fixed_bytes<NT>();
     const unsigned sbase = ad_smem(smem);
     unsigned char* qs = smem + AREA;                               // [8 NT] rows of queries
     int* row_seq = (int*)(qs + 8 * NT * SP_ROW);                   // [8 NT]
     int* row_head = row_seq + 8 * NT;
     int* row_last = row_head + 8 * NT;
-    float* held = (float*)(smem + sp_smem<NT>());                  // [rows][a.held] scores of the split's keys, where they are kept
+    float* held = (float*)(smem + sp_smem<NT, STAGES>());                  // [rows][a.held] scores of the split's keys, where they are kept
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int grp = lane >> 2, t = lane & 3;
     const int G = a.nH / a.nKV;
@@ -248,11 +246,7 @@ attn_span_kernel(SpanArgs a) {
         sp_load_page(sbase + 2 * st * SP_TILE, a.k_cache + at, nv);
         sp_load_page(sbase + (2 * st + 1) * SP_TILE, a.v_cache + at, nv);
     };
-#pragma unroll
-    for (int s = 0; s < SP_STAGES - 1; ++s) {
-        if (p_begin + s < p_end) load(s, p_begin + s);
-        sp_commit();
-    }
+    if (p_begin < p_end) load(0, p_begin);
     __syncthreads();
     for (int i = tid; i < 8 * NT * SP_CHUNKS; i += SP_THREADS) {
         const int r = i / SP_CHUNKS, c = i - r * SP_CHUNKS, b = row_seq[r];
@@ -276,14 +270,15 @@ attn_span_kernel(SpanArgs a) {
     for (int n = 0; n < NT; ++n) { m_run[n][0] = m_run[n][1] = -INFINITY; l_run[n][0] = l_run[n][1] = 0.f; }
 
     for (int p = p_begin; p < p_end; ++p) {
-        const int st = (p - p_begin) % SP_STAGES;
-        sp_wait<SP_STAGES - 2>();
-        __syncthreads();                                   // page p has landed; the stage read last time is free
-        {
-            const int pn = p + SP_STAGES - 1;
-            if (pn < p_end) load((pn - p_begin) % SP_STAGES, pn);
-            sp_commit();
+        const int st = STAGES == 2 ? (p - p_begin) & 1 : 0;
+        if (STAGES == 1 && p > p_begin) {
+            __syncthreads();                               // the page read last time is free
+            load(0, p);
         }
+        sp_commit();
+        sp_wait<0>();
+        __syncthreads();                                   // page p has landed; the stage read last time is free
+        if (STAGES == 2 && p + 1 < p_end) load(st ^ 1, p + 1);
         const int j0 = p * GL_PAGE + warp * 16;            // this warp's first key
         if (!SHARED && j0 >= total) continue;
         const unsigned Ks = sbase + 2 * st * SP_TILE, Vs = Ks + SP_TILE;
@@ -653,22 +648,22 @@ stream_span_kernel(SpanArgs a) {
 #define SP_HELD_BYTES (56 * 1024)                  // scores a block keeps in shared memory at most
 #define SP_FACTOR_BYTES (24 * 1024)                // factors of the parts of its rows
 
-template <int NT, int MODE>
+template <int NT, int MODE, int STAGES = 2>
 static int launch_span(const SpanArgs& a, dim3 grid, int cluster, cudaStream_t stream) {
     static bool allowed[64] = {};
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) { cudaGetLastError(); return GL_ERR_DRIVER; }
-    const size_t most = sp_smem<NT>() + (MODE == SP_JOIN ? SP_HELD_BYTES + SP_FACTOR_BYTES : 0);
+    const size_t most = sp_smem<NT, STAGES>() + (MODE == SP_JOIN ? SP_HELD_BYTES + SP_FACTOR_BYTES : 0);
     if (!allowed[dev]) {
-        if (cudaFuncSetAttribute(attn_span_kernel<NT, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most) != cudaSuccess) {
+        if (cudaFuncSetAttribute(attn_span_kernel<NT, MODE, STAGES>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most) != cudaSuccess) {
             cudaGetLastError();
             return GL_ERR_SMEM;
         }
         allowed[dev] = true;
     }
-    const size_t smem = sp_smem<NT>() + (MODE == SP_JOIN ? sizeof(float) * ((a.weights ? (size_t)a.held * (a.nH / a.nKV) : 0) + 8 * NT * (size_t)(a.slots + a.splits)) : 0);
+    const size_t smem = sp_smem<NT, STAGES>() + (MODE == SP_JOIN ? sizeof(float) * ((a.weights ? (size_t)a.held * (a.nH / a.nKV) : 0) + 8 * NT * (size_t)(a.slots + a.splits)) : 0);
     if (smem > most) return GL_ERR_SMEM;
-    return gl_launch(attn_span_kernel<NT, MODE>, grid, dim3(SP_THREADS), smem, stream, cluster, a);
+    return gl_launch(attn_span_kernel<NT, MODE, STAGES>, grid, dim3(SP_THREADS), smem, stream, cluster, a);
 }
 
 template <int R, int MODE>
@@ -693,6 +688,10 @@ static int launch_spans(const SpanArgs& a, int rows, dim3 grid, int cluster, cud
         if (a.nH == a.nKV) return launch_stream<1, MODE>(a, grid, cluster, stream);
         if (a.nH == 2 * a.nKV) return launch_stream<2, MODE>(a, grid, cluster, stream);
     }
+    // Pages in flight: two; one, and more blocks an SM, where a block has one page or two to walk (behind shared pages: 1,024 blocks
+    // of a page each, heads of 128, 59 us against 64 with what the shared pages take).
+    if constexpr (MODE == SP_JOIN)
+        if (rows <= 8 && a.short_spans) return launch_span<1, MODE, 1>(a, grid, cluster, stream);
     if (rows <= 8) return launch_span<1, MODE>(a, grid, cluster, stream);
     if (rows <= 16) return launch_span<2, MODE>(a, grid, cluster, stream);
     return launch_span<SP_MAX_NT, MODE>(a, grid, cluster, stream);

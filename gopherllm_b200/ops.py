@@ -8,6 +8,7 @@ not build, is an error.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 from ctypes import POINTER, Structure, byref, c_float, c_int, c_void_p
 from typing import Optional
@@ -873,16 +874,14 @@ class PrefixLayout:
         spared = sum((len(m) - 1) * p for m, p in checked) * 2 * PAGE * num_kv_heads * head_dim * (4 if dtype == torch.float32 else 2)
         if spared < PREFIX_SPARED_BYTES:
             own, checked, tiles = own + PAGE * max((p for _, p in checked), default=0), [], []
-        # Blocks walk equal stretches of pages: on the tensor cores one block an SM at a time, so as few rounds of them as the tiles
-        # allow; else short enough to fill the machine a few times over.
+        # Blocks walk equal stretches of pages, as few rounds of them as the tiles allow: on the tensor cores a block an SM at a time, else
+        # what the registers and shared memory hold.
         total = sum(t * p for t, (_, p) in zip(tiles, checked)) * num_kv_heads
-        if tensor:
-            room = sms * -(-sum(tiles) * num_kv_heads // sms)
-            stretch = max(2, total // room)
-            while sum(t * -(-p // stretch) for t, (_, p) in zip(tiles, checked)) * num_kv_heads > room:
-                stretch += 1
-        else:
-            stretch = max(2, -(-total // (PREFIX_BLOCKS_PER_SM * sms)))
+        slots = sms * (1 if tensor else 2 if self.rows > 4 and (dtype == torch.float32 or self.rows > 16) else 3)
+        room = slots * max(1, -(-sum(tiles) * num_kv_heads // slots))
+        stretch = max(2, total // room)
+        while sum(t * -(-p // stretch) for t, (_, p) in zip(tiles, checked)) * num_kv_heads > room:
+            stretch += 1
         order, items, shared_of = [], [], [[0, 0] for _ in range(batch)]
         slots = 0
         for (members, pages), n_tiles in zip(checked, tiles):
@@ -900,10 +899,11 @@ class PrefixLayout:
         self.max_shared = max((p for _, p in checked), default=0)      # pages
         own_pages = -(-own // PAGE)
         self.chunks = span_chunks(dtype, head_dim, group)
-        self.splits = span_splits(batch, num_kv_heads * self.chunks, own_pages, sms, dtype, head_dim)
+        self.splits = span_splits(batch, num_kv_heads * self.chunks, own_pages, sms, dtype, head_dim, group)
         # joined: the blocks of a sequence's own pages put everything together themselves (csrc/attention_spans.cu)
         self.joined = (head_dim % 4 == 0 and self.splits <= 8
                        and 4 * (8 if dtype == torch.float32 else span_rows(dtype, head_dim)) * (slots + self.splits) <= SPAN_FACTOR_BYTES)
+        self.short = int(-(-own_pages // self.splits) <= 2)
         self.slots, self.n_items = slots + (0 if self.joined else self.splits), len(items)
         self.call = (batch, num_heads, num_kv_heads, head_dim, dtype)
         self.launches = (1 if items else 0) + (1 if self.joined else 2)
@@ -917,7 +917,6 @@ class PrefixLayout:
                 self.items_at, self.shared_at)
 
 
-PREFIX_BLOCKS_PER_SM = 4
 PREFIX_SPARED_BYTES = 12 << 20       # (see PrefixLayout)
 SPAN_FACTOR_BYTES, SPAN_HELD_BYTES = 24 * 1024, 56 * 1024      # shared memory for the factors of a row's parts, for a block's scores
 
@@ -955,14 +954,29 @@ def span_chunks(dtype, head_dim: int, group: int) -> int:
     return -(-group // -(-group // n))
 
 
-def span_splits(batch: int, heads: int, pages: int, sms: int, dtype, head_dim: int) -> int:
-    """Blocks that share a sequence's own pages: as many as are resident at once, of four pages at least.  Up to eight form a
-    cluster and join their results themselves; more leave them to a second kernel, so eight it is where those fill two blocks an SM or
-    have no more than eight pages each."""
-    per_sm = 4 if dtype == torch.float32 else max(1, min(8, 227 * 1024 // (4 * PAGE * (2 * head_dim + 16) + 4096)))
+def span_splits(batch: int, heads: int, pages: int, sms: int, dtype, head_dim: int, group: int) -> int:
+    """Blocks that share a sequence's own pages: as many as are resident at once, of four pages at least (in 32 bits, one).  Up to eight
+    form a cluster and join their results themselves, more leave them to a second kernel: eight it is where those fill two
+    blocks an SM or have no more than eight pages each.  Clusters have 1, 2, 4 or 8 blocks: six, 6 x 64 blocks of heads of 128, took
+    23.5 us where four took 18.0."""
     blocks = max(1, batch * heads)
+    if dtype == torch.float32 or group <= 2:
+        per_sm = 4                                         # (registers; the others shared memory)
+    else:
+        per_sm = max(1, min(8, 227 * 1024 // (4 * PAGE * (2 * head_dim + 16) + 4096)))
     n = max(1, min(per_sm * sms // blocks, pages if dtype == torch.float32 else -(-pages // 4)))
-    return 8 if n > 8 and (8 * blocks >= 2 * sms or pages <= 64) else n
+    if n > 8 and not (8 * blocks >= 2 * sms or pages <= 64):
+        return n
+    return 1 << (min(n, 8).bit_length() - 1)
+
+
+@functools.lru_cache(maxsize=4096)
+def _weigh_shape(B: int, num_heads: int, num_kv_heads: int, head_dim: int, dtype, max_len: int, sms: int):
+    """(chunks, splits, whether the splits join in place) of one token a sequence with weights."""
+    group, used = num_heads // num_kv_heads, -(-max_len // PAGE)
+    chunks = span_chunks(dtype, head_dim, group)
+    splits = span_splits(B, num_kv_heads * chunks, used, sms, dtype, head_dim, group)
+    return chunks, splits, not (head_dim % 4 or chunks > 1 or splits > 8 or 4 * group * (-(-used // splits) * PAGE + 4) > SPAN_HELD_BYTES)
 
 
 def prefix_plan(groups, batch: int, num_heads: int, num_kv_heads: int, head_dim: int, dtype, own: int, device) -> PrefixPlan:
@@ -977,11 +991,11 @@ def prefix_plan(groups, batch: int, num_heads: int, num_kv_heads: int, head_dim:
 class _SpanArgs(Structure):
     _fields_ = [(n, c_void_p) for n in ("q", "out", "k_cache", "v_cache", "seq_row", "seq_qlen", "seq_ctx", "pages", "order", "items",
                                         "seq_shared", "part_o", "part_ml", "scores", "weights")] + \
-               [(n, c_int) for n in ("B", "nH", "nKV", "max_pages", "n_pages", "n_items", "splits", "slots", "chunks", "reach", "early", "held")]
+               [(n, c_int) for n in ("B", "nH", "nKV", "max_pages", "n_pages", "n_items", "splits", "slots", "chunks", "reach", "short", "early", "held")]
 
 
 class _SpanF32Args(Structure):
-    _fields_ = _SpanArgs._fields_[:-2] + [("hd", c_int), ("last", c_int), ("early", c_int), ("held", c_int), ("joined", c_int)]
+    _fields_ = _SpanArgs._fields_[:-3] + [("hd", c_int), ("last", c_int), ("early", c_int), ("held", c_int), ("joined", c_int)]
 
 
 class _RunArgs(Structure):
@@ -1060,7 +1074,7 @@ def attention_prefix(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, 
     a = (_SpanF32Args if f32 else _SpanArgs)(
         q.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), None, None, seq_ctx.data_ptr(), pages.data_ptr(),
         base, base + 4 * lay.items_at, base + 4 * lay.shared_at, at, ml, None, None,
-        B, num_heads, num_kv_heads, pages.shape[1], k_cache.shape[0], lay.n_items, lay.splits, lay.slots, lay.chunks, 0, head_dim if f32 else 0)
+        B, num_heads, num_kv_heads, pages.shape[1], k_cache.shape[0], lay.n_items, lay.splits, lay.slots, lay.chunks, 0, head_dim if f32 else lay.short)
     fn = _lib("attention_spans_f32.cu").gl_attention_prefix_f32 if f32 else _lib("attention_spans.cu", (f"GL_HEAD_DIM={head_dim}",)).gl_attention_prefix
     _check(_launch(fn, byref(a), c_int(lay.rows), c_int(lay.joined), _stream()), "attention_prefix", lay.launches)
 
@@ -1091,11 +1105,9 @@ def attention_weighed(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor,
     f32 = dtype is torch.float32
     lib = _lib("attention_spans_f32.cu") if f32 else _lib("attention_spans.cu", (f"GL_HEAD_DIM={head_dim}",))
     if max_qlen == 1:
-        group, used = num_heads // num_kv_heads, -(-max_len // PAGE)
-        chunks = span_chunks(dtype, head_dim, group)
-        splits = span_splits(B, num_kv_heads * chunks, used, sm_count(q.device), dtype, head_dim)
+        chunks, splits, joined = _weigh_shape(B, num_heads, num_kv_heads, head_dim, dtype, max_len, sm_count(q.device))
         slots, at, ml, scores = 0, None, None, None
-        if head_dim % 4 or chunks > 1 or splits > 8 or 4 * group * (-(-used // splits) * PAGE + 4) > SPAN_HELD_BYTES:
+        if not joined:
             slots, n = splits, B * num_heads * splits * head_dim
             part = empty((n + B * num_heads * (2 * splits + max_len),), torch.float32, q.device)
             at = part.data_ptr()
