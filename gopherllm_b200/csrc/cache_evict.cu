@@ -2,11 +2,12 @@
 // and the most recent positions stay and, of those between, the ones with the largest sums; what stays moves, in order, to the
 // head of the sequence's pages (or of other pages).
 //
-// A (layer, sequence, head) is one block's, or a cluster's, every block of which selects for itself.
+// A (layer, sequence, head) is one block's, or a cluster's.  Of short sequences every block of a cluster selects for itself; the blocks of
+// long ones read and count a share of the positions each and add their histograms up in distributed shared memory.
 // Selection: the sums become whole numbers of the same order (a NaN below everything, both zeros the same), the m-th largest is found
 // digit by digit with histograms (11, 11 and 10 bits), and the positions above it, with as many equal to it as are missing,
 // lowest first, are written down in order: every warp counts its stretch, the counts are summed, every warp writes.  Counts
-// are whole numbers, so nothing depends on the order of additions.  The sums are read a page a warp, four pages under way.
+// are whole numbers, so nothing depends on the order of additions.  The sums are read a page a warp, several pages under way.
 //
 // Moving: a row is its key's and its value's pieces of 16 bytes side by side.  What stays at place i came from place kept[i] >= i,
 // and kept grows, so in place a block walks forward: the places it has written lie before everything it has still to read.  The
@@ -35,54 +36,94 @@ __device__ __forceinline__ unsigned ev_key(float w) {
 }
 __device__ __forceinline__ int ev_length(const EvictArgs& a, int b) { return min(max(0, a.seq_len[b]), a.max_pages * GL_PAGE); }
 
-#define EV_PAGES 4                        // pages of sums a warp has under way
+#define EV_SMALL 256                      // threads of a block for up to 4,096 positions, and beyond
+#define EV_LARGE 512
 #define EV_MOST (200 * 1024)              // shared memory for the keys of a sequence's sums and the positions that stay
 
+// The sum of the counts of the warps before this one; lane w holds warp w's.
+__device__ __forceinline__ int ev_before(int v, int warp, int lane) {
+    int sum = lane < warp ? v : 0;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    return sum;
+}
+
 // The positions of a sequence of n > keep that stay, in order, to ``list``.  keys: room for n, or null: the sums are read again each time.
+// With T = EV_LARGE the C blocks of the cluster share the positions out: keys holds those of this block's pages (p_lo on), list is global memory.
 template <int T, typename Place>
-__device__ __forceinline__ void ev_select(const EvictArgs& a, int n, unsigned* keys, int* list, int* hist, int* warp_sum, int* warp_eq, int* found, Place place) {
+__device__ __forceinline__ void ev_select(const EvictArgs& a, int n, unsigned* keys, int* list, int (*hists)[EV_BINS], int* warp_sum, int* warp_eq, int* found,
+                                          int rank, int C, Place place) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    constexpr int warps = T / 32;
-    const int lo = a.first, hi = n - a.recent;                      // the positions to choose from
+    constexpr int warps = T / 32, PAGES = T == EV_SMALL ? 4 : 8;    // pages of sums a warp has under way
+    constexpr bool SHARED = T == EV_LARGE;
+    int lo = a.first, hi = n - a.recent;                            // the positions to choose from
     const int want = a.keep - a.first - a.recent;
-    for (int i = tid; i < a.first; i += T) list[i] = i;
-    for (int i = tid; i < a.recent; i += T) list[a.keep - a.recent + i] = hi + i;
+    if (!SHARED || rank == 0)
+        for (int i = tid; i < a.first; i += T) list[i] = i;
+    if (!SHARED || rank == C - 1)
+        for (int i = tid; i < a.recent; i += T) list[a.keep - a.recent + i] = hi + i;
     if (want <= 0) return;
+    if (SHARED) {
+        const int p0 = lo / GL_PAGE, pages = (hi + GL_PAGE - 1) / GL_PAGE - p0;
+        const int mine = p0 + (int)((long long)pages * rank / C), behind = p0 + (int)((long long)pages * (rank + 1) / C);
+        lo = max(lo, mine * GL_PAGE);
+        hi = max(lo, min(hi, behind * GL_PAGE));
+    }
+    const int key0 = SHARED ? lo / GL_PAGE * GL_PAGE : 0;           // the position whose key is keys[0]
     unsigned prefix = 0, mask = 0;
     int missing = want;                                             // how many of the positions that agree with the prefix stay
 #pragma unroll 1
     for (int pass = 0; pass < 3; ++pass) {
         const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
+        int* hist = hists[SHARED ? pass & 1 : 0];                   // (the other one may still be read by the cluster)
         for (int i = tid; i < EV_BINS; i += T) hist[i] = 0;
         __syncthreads();
         auto count = [&](int j, unsigned k) {
             if (j >= lo && j < hi && (k & mask) == prefix) atomicAdd(&hist[(k >> shift) & ((1u << bits) - 1)], 1);
         };
         if (pass == 0 || !keys) {
-            for (int p0 = lo / GL_PAGE + warp * EV_PAGES; p0 * GL_PAGE < hi; p0 += warps * EV_PAGES) {
-                float2 w[EV_PAGES];
+            for (int p0 = lo / GL_PAGE + warp * PAGES; p0 * GL_PAGE < hi; p0 += warps * PAGES) {
+                float2 w[PAGES];
 #pragma unroll
-                for (int i = 0; i < EV_PAGES; ++i)
+                for (int i = 0; i < PAGES; ++i)
                     if ((p0 + i) * GL_PAGE < hi) w[i] = *(const float2*)place((p0 + i) * GL_PAGE + 2 * lane);
 #pragma unroll
-                for (int i = 0; i < EV_PAGES; ++i)
+                for (int i = 0; i < PAGES; ++i)
                     if ((p0 + i) * GL_PAGE < hi) {
                         const int j = (p0 + i) * GL_PAGE + 2 * lane;
                         const unsigned k0 = ev_key(w[i].x), k1 = ev_key(w[i].y);
-                        if (keys) *(uint2*)(keys + j) = make_uint2(k0, k1);
+                        if (keys) *(uint2*)(keys + j - key0) = make_uint2(k0, k1);
                         count(j, k0);
                         count(j + 1, k1);
                     }
             }
         } else {
-            for (int j = lo + tid; j < hi; j += T) count(j, keys[j]);
+            for (int j = lo + tid; j < hi; j += T) count(j, keys[j - key0]);
         }
-        __syncthreads();
         // the bin, from the top, in which the count reaches ``missing``: every thread sums a run of bins
         constexpr int per = EV_BINS / T;
         const int top = EV_BINS - 1 - tid * per;                    // its highest bin
-        int mine = 0;
-        for (int i = 0; i < per; ++i) mine += hist[top - i];
+        int bins[per], mine = 0;
+        if (SHARED) {
+            cg::cluster_group cluster = cg::this_cluster();
+            cluster.sync();
+#pragma unroll
+            for (int i = 0; i < per; ++i) bins[i] = 0;
+            for (int c = 0; c < C; ++c) {
+                const int4* theirs = (const int4*)cluster.map_shared_rank(hist + top - (per - 1), c);
+#pragma unroll
+                for (int i = 0; i < per; i += 4) {
+                    const int4 v = theirs[(per - 4 - i) / 4];
+                    bins[i] += v.w; bins[i + 1] += v.z; bins[i + 2] += v.y; bins[i + 3] += v.x;
+                }
+            }
+        } else {
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < per; ++i) bins[i] = hist[top - i];
+        }
+#pragma unroll
+        for (int i = 0; i < per; ++i) mine += bins[i];
         int before = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -91,13 +132,15 @@ __device__ __forceinline__ void ev_select(const EvictArgs& a, int n, unsigned* k
         }
         if (lane == 31) warp_sum[warp] = before;
         __syncthreads();
-        int ahead = before - mine;
-        for (int w = 0; w < warp; ++w) ahead += warp_sum[w];
+        const int ahead_all = ev_before(lane < warps ? warp_sum[lane] : 0, warp, lane);
+        int ahead = before - mine + ahead_all;
         if (ahead < missing && ahead + mine >= missing) {
-            int i = 0;
-            while (ahead + hist[top - i] < missing) { ahead += hist[top - i]; ++i; }
-            found[0] = top - i;
-            found[1] = ahead;
+            bool here = false;
+#pragma unroll
+            for (int i = 0; i < per; ++i) {
+                if (!here && ahead + bins[i] >= missing) { here = true; found[0] = top - i; found[1] = ahead; }
+                ahead += bins[i];
+            }
         }
         __syncthreads();
         prefix |= (unsigned)found[0] << shift;
@@ -105,7 +148,7 @@ __device__ __forceinline__ void ev_select(const EvictArgs& a, int n, unsigned* k
         missing -= found[1];
     }
     // positions above the limit stay, and the first ``missing`` equal to it
-    auto key_of = [&](int j) { return keys ? keys[j] : ev_key(*place(j)); };
+    auto key_of = [&](int j) { return keys ? keys[j - key0] : ev_key(*place(j)); };
     const int len = hi - lo, stretch = ((len + warps - 1) / warps + 31) & ~31;
     const int s0 = lo + warp * stretch, s1 = min(hi, s0 + stretch);
     int above = 0, equal = 0;
@@ -116,11 +159,20 @@ __device__ __forceinline__ void ev_select(const EvictArgs& a, int n, unsigned* k
     }
     if (lane == 0) { warp_sum[warp] = above; warp_eq[warp] = equal; }
     __syncthreads();
-    int at = a.first, eq = 0;
-    for (int w = 0; w < warp; ++w) {
-        at += warp_sum[w] + min(warp_eq[w], max(0, missing - eq));
-        eq += warp_eq[w];
+    // (of the positions equal to the limit the first ``missing`` of all warps')
+    int eq = ev_before(lane < warps ? warp_eq[lane] : 0, warp, lane);
+    int at = a.first + ev_before(lane < warps ? warp_sum[lane] : 0, warp, lane);
+    if (SHARED) {                                                   // the blocks before this one
+        if (warp == warps - 1 && lane == 0) { found[2] = at - a.first + above; found[3] = eq + equal; }
+        cg::cluster_group cluster = cg::this_cluster();
+        cluster.sync();
+        for (int c = 0; c < rank; ++c) {
+            const int* theirs = cluster.map_shared_rank(found, c);
+            at += theirs[2];
+            eq += theirs[3];
+        }
     }
+    at += min(eq, missing);
     for (int j = s0 + lane; j - lane < s1; j += 32) {
         const unsigned k = j < s1 ? key_of(j) : 0u;
         const unsigned eqs = __ballot_sync(0xffffffffu, j < s1 && k == prefix), below = (1u << lane) - 1;
@@ -135,10 +187,12 @@ __device__ __forceinline__ void ev_select(const EvictArgs& a, int n, unsigned* k
 // U: the piece a thread moves (16, 4 or 2 bytes).  blockIdx = (block of the cluster, key/value head, sequence and layer).  Dynamic
 // shared memory: the positions that stay (``listed``: else the output itself serves) and, if there is room (``held``), the sums' keys.
 template <typename U, int T>
-__global__ void __launch_bounds__(T, T == 256 ? 8 : 1)
+__global__ void __launch_bounds__(T, T == EV_SMALL ? 8 : 2)
 evict_kernel(EvictArgs a, int listed, int held) {
     extern __shared__ __align__(16) unsigned ev[];
-    __shared__ int hist[EV_BINS], warp_sum[32], warp_eq[32], found[2], from;
+    constexpr bool SHARED = T == EV_LARGE;
+    __shared__ __align__(16) int hists[SHARED ? 2 : 1][EV_BINS];
+    __shared__ int warp_sum[32], warp_eq[32], found[4], from;
     const int tid = threadIdx.x;
     const int C = gridDim.x, rank = blockIdx.x, g = blockIdx.y, b = blockIdx.z % a.B, layer = blockIdx.z / a.B;
     gl_grid_wait();
@@ -161,10 +215,15 @@ evict_kernel(EvictArgs a, int listed, int held) {
         }
         if (same) return;
     } else {
-        ev_select<T>(a, n, keys, list, hist, warp_sum, warp_eq, found, [&](int j) { return a.weights + place(pg, j); });
+        ev_select<T>(a, n, keys, SHARED ? kept : list, hists, warp_sum, warp_eq, found, rank, C, [&](int j) { return a.weights + place(pg, j); });
+        if (SHARED) {
+            cg::this_cluster().sync();                             // the list is whole, and no block reads another's memory any more
+            if (listed)
+                for (int i = tid; i < a.keep; i += T) list[i] = kept[i];
+        }
     }
     __syncthreads();
-    if (listed && rank == 0 && n > a.keep)
+    if (!SHARED && listed && rank == 0 && n > a.keep)
         for (int i = tid; i < a.keep; i += T) kept[i] = list[i];
     int begin = 0, end = stay;                                     // the rows, and of a row's pieces the columns, that this block moves
     const int ku = a.k_bytes / (int)sizeof(U), vu = a.v_bytes / (int)sizeof(U);
@@ -177,7 +236,7 @@ evict_kernel(EvictArgs a, int listed, int held) {
         }
         u0 = (int)((long long)(ku + vu) * rank / C);
         u1 = (int)((long long)(ku + vu) * (rank + 1) / C);
-        if (C > 1) cg::this_cluster().sync();                      // (the sums have been read by all before any moves)
+        if (!SHARED && C > 1) cg::this_cluster().sync();           // (the sums have been read by all before any moves)
         __syncthreads();
         begin = from;
     } else {
@@ -208,9 +267,8 @@ evict_kernel(EvictArgs a, int listed, int held) {
             if (i < end) a.weights[place(to, i)] = w;
         }
     // Pieces a thread has under way.  Small blocks, eight an SM, move and select beside one another (24 layers of 4 x 32 heads of 64, 1,024 of
-    // some 1,900 positions stay, 1.66 GB: 295 us; four blocks of eight pieces 358, eight of two 304); a large one is alone on its SM
-    // (4 x 2 x 8 heads of 128, 4,096 of 31,400 stay: 75 us, with four pieces 87).
-    constexpr int N = T == 256 ? 4 : 8;
+    // some 1,900 positions stay, 1.66 GB: 295 us; four blocks of eight pieces 358, eight of two 304).
+    constexpr int N = T == EV_SMALL ? 4 : 8;
     U* kc = (U*)a.k_cache;
     U* vc = (U*)a.v_cache;
     for (int c0 = u0; c0 < u1; c0 += T) {
@@ -259,20 +317,21 @@ GL_API int gl_cache_evict(const EvictArgs* args, int sms, cudaStream_t stream) {
     if (a.k_bytes <= 0 || a.v_bytes <= 0 || a.k_bytes > 4096 || a.v_bytes > 4096 || (a.k_bytes | a.v_bytes) % 2) return GL_ERR_SHAPE;
     if ((uintptr_t)a.weights & 7) return GL_ERR_ALIGN;
     const uintptr_t at = (uintptr_t)a.k_cache | (uintptr_t)a.v_cache | (uintptr_t)a.k_bytes | (uintptr_t)a.v_bytes;
-    // What fits in shared memory: the list of what stays, then the sums' keys beside it.
-    const int listed = a.keep < most && 4LL * a.keep <= EV_MOST ? 1 : 0;
-    const int held = 4 * (most + (listed ? a.keep : 0)) <= EV_MOST ? (int)most : 0;
     // Blocks of 256 threads, several an SM, for up to 4,096 positions; larger ones beyond.  A cluster shares the rows out where there
     // are fewer heads than the machine takes blocks.
-    const int threads = most <= 4096 ? 256 : 1024;
-    const long long heads = (long long)a.layers * a.B * a.nKV, room = (threads == 256 ? 4LL : 1LL) * sms;
+    const int threads = most <= 4096 ? EV_SMALL : EV_LARGE;
+    const long long heads = (long long)a.layers * a.B * a.nKV, room = (threads == EV_SMALL ? 4LL : 2LL) * sms;
     int blocks = 1;
     while (blocks < 8 && heads * 2 * blocks <= room && a.keep / (2 * blocks) >= 32) blocks *= 2;
-    if (!listed) blocks = 1;                                       // (the list is then the output itself, which one block writes)
-    if (threads == 256) {
-        if (at % 16 == 0) return launch_evict<uint4, 256>(a, blocks, listed, held, stream);
-        return at % 4 == 0 ? launch_evict<unsigned, 256>(a, blocks, listed, held, stream) : launch_evict<unsigned short, 256>(a, blocks, listed, held, stream);
+    // What fits in shared memory: the list of what stays, then the keys of the sums that a block reads beside it.
+    const int listed = a.keep < most && 4LL * a.keep <= EV_MOST ? 1 : 0;
+    if (!listed && threads == EV_SMALL) blocks = 1;                // (the list is then the output itself, which one block writes)
+    const long long keys = threads == EV_SMALL ? most : ((a.max_pages + blocks - 1) / blocks + 1LL) * GL_PAGE;
+    const int held = 4 * (keys + (listed ? a.keep : 0)) <= EV_MOST ? (int)keys : 0;
+    if (threads == EV_SMALL) {
+        if (at % 16 == 0) return launch_evict<uint4, EV_SMALL>(a, blocks, listed, held, stream);
+        return at % 4 == 0 ? launch_evict<unsigned, EV_SMALL>(a, blocks, listed, held, stream) : launch_evict<unsigned short, EV_SMALL>(a, blocks, listed, held, stream);
     }
-    if (at % 16 == 0) return launch_evict<uint4, 1024>(a, blocks, listed, held, stream);
-    return at % 4 == 0 ? launch_evict<unsigned, 1024>(a, blocks, listed, held, stream) : launch_evict<unsigned short, 1024>(a, blocks, listed, held, stream);
+    if (at % 16 == 0) return launch_evict<uint4, EV_LARGE>(a, blocks, listed, held, stream);
+    return at % 4 == 0 ? launch_evict<unsigned, EV_LARGE>(a, blocks, listed, held, stream) : launch_evict<unsigned short, EV_LARGE>(a, blocks, listed, held, stream);
 }
