@@ -4,10 +4,7 @@
 // A block takes one span for up to R rows (8 at most).  Pages of keys and values come to shared memory by cp.async; a thread
 // multiplies one key with half the rows (its key in 16-byte pieces at an odd pitch of them, so that eight lanes touch all
 // banks; the rows' pieces are broadcasts), a warp takes the softmax of a row, and a thread adds up one or two dims of the
-// values for all rows.  What bounds it is the FMA pipe once a block has eight rows, memory below.
-//
-// Runs of several tokens take rows of consecutive queries; a second kernel then walks the cache page by page, multiplies its
-// keys with all the rows that see them and adds up e^(s - m) / l.  No sum depends on the order in which blocks run.
+// values for all rows.  So it is for heads that are no whole 16-byte pieces; all others stream (below).
 #include "common.cuh"
 #include <cooperative_groups.h>
 namespace cg = cooperative_groups;
@@ -20,7 +17,7 @@ struct SpanF32Args {
     float* out;
     const float* k_cache;         // [pages, nKV, GL_PAGE, hd]
     const float* v_cache;
-    const int* seq_row;           // [B] first row of q and out, or null (row b is sequence b)
+    const int* seq_row;           // [B] row of q and out, or null (row b is sequence b)
     const int* seq_qlen;          // [B] or null (one token each)
     const int* seq_ctx;           // [B] positions cached before this step
     const int* pages;             // [B, max_pages]
@@ -28,14 +25,14 @@ struct SpanF32Args {
     const int* items;
     const int* seq_shared;
     float* part_o;                // [B, nH, slots, hd]
-    float* part_ml;               // [B, nH, slots, 2], for runs [rows, nH, 2]
+    float* part_ml;               // [B, nH, slots, 2]
     float* scores;                // [B, nH, reach] or null
     float* weights;               // [pages, nKV, GL_PAGE] or null
-    int B, nH, nKV, max_pages, n_pages, n_items, splits, slots, chunks, reach, hd, last;
+    int B, nH, nKV, max_pages, n_pages, n_items, splits, slots, chunks, reach, hd;
     int early, held, joined;      // set by the launchers
 };
 
-enum { SF_OWN = 0, SF_SHARED = 1, SF_RUN = 2 };
+enum { SF_OWN = 0, SF_SHARED = 1 };
 
 __host__ __device__ inline int sf_pitch(int hd) { return 4 * (((hd + 3) / 4) | 1); }      // floats between two keys: an odd number of 16-byte pieces
 __host__ __device__ inline int sf_stages(int hd) { return hd <= 128 ? 2 : 1; }
@@ -91,7 +88,7 @@ span_f32_kernel(SpanF32Args a) {
     float* row_l = row_m + 8;
     float* row_c = row_l + 8;
     float* halves = row_c + 8;                                     // [8][hd <= 64] the second half of the keys' sums
-    int* row_seq = (int*)(halves + 8 * SF_MAX_HD);                 // [8] sequence (runs: row of q), head, last position seen
+    int* row_seq = (int*)(halves + 8 * SF_MAX_HD);                 // [8] sequence, head, last position seen
     int* row_head = row_seq + 8;
     int* row_last = row_head + 8;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -110,18 +107,6 @@ span_f32_kernel(SpanF32Args a) {
             row_seq[tid] = b;
             row_head[tid] = g * G + r % G;
             row_last[tid] = b >= 0 ? a.seq_ctx[b] : -1;
-        }
-    } else if (KIND == SF_RUN) {
-        const int b = blockIdx.z, n = a.seq_qlen[b] * G, r0 = blockIdx.x * R;
-        if (r0 >= n) return;
-        g = blockIdx.y; rows = min(R, n - r0); slot = 0; table = b;
-        p_begin = 0;
-        p_end = (a.seq_ctx[b] + (r0 + rows - 1) / G) / GL_PAGE + 1;
-        if (tid < 8) {
-            const int i = (r0 + tid) / G;
-            row_seq[tid] = tid < rows ? a.seq_row[b] + i : -1;
-            row_head[tid] = g * G + (r0 + tid) % G;
-            row_last[tid] = tid < rows ? a.seq_ctx[b] + i : -1;
         }
     } else {
         const int b = blockIdx.z;
@@ -142,7 +127,7 @@ span_f32_kernel(SpanF32Args a) {
         }
     }
     if (tid < 8) { row_m[tid] = -INFINITY; row_l[tid] = 0.f; }
-    const int total = a.seq_ctx[table] + (KIND == SF_RUN ? a.seq_qlen[table] : 1);      // positions of the sequence that were written
+    const int total = a.seq_ctx[table] + 1;                       // positions of the sequence that were written
     const int* pg = a.pages + (size_t)table * a.max_pages;
     auto load = [&](int st, int p) {
         const size_t at = ((size_t)gl_checked(pg[p], a.n_pages, GL_BAD_PAGE) * a.nKV + g) * GL_PAGE * hd;
@@ -157,7 +142,7 @@ span_f32_kernel(SpanF32Args a) {
     __syncthreads();
     for (int i = tid; i < 8 * 4 * n4; i += SF_THREADS) {
         const int r = i / (4 * n4), c = i - r * 4 * n4, b = row_seq[r];
-        const int at = b >= 0 && KIND != SF_RUN && a.seq_row ? a.seq_row[b] : b;
+        const int at = b >= 0 && a.seq_row ? a.seq_row[b] : b;
         qs[r * pitch + c] = b >= 0 && c < hd ? a.q[((size_t)at * a.nH + row_head[r]) * hd + c] : 0.f;
     }
     int least = 0x7fffffff;                                       // the earliest last position among the block's rows
@@ -253,11 +238,10 @@ span_f32_kernel(SpanF32Args a) {
             const int d = d0 + i * SF_THREADS;
             if (d >= hd || (narrow && i)) continue;
             const float v = narrow ? o[r][0] + halves[r * 64 + d] : o[r][i];
-            if (KIND == SF_RUN) a.out[((size_t)row_seq[r] * a.nH + row_head[r]) * hd + d] = l == 0.f ? 0.f : v / l;
-            else a.part_o[(((size_t)row_seq[r] * a.nH + row_head[r]) * a.slots + slot) * hd + d] = v;
+            a.part_o[(((size_t)row_seq[r] * a.nH + row_head[r]) * a.slots + slot) * hd + d] = v;
         }
         if (tid == 0) {
-            float* ml = a.part_ml + ((size_t)row_seq[r] * a.nH + row_head[r]) * 2 * (KIND == SF_RUN ? 1 : a.slots) + 2 * slot;
+            float* ml = a.part_ml + ((size_t)row_seq[r] * a.nH + row_head[r]) * 2 * a.slots + 2 * slot;
             ml[0] = row_m[r];
             ml[1] = l;
         }
@@ -585,57 +569,196 @@ stream_f32_kernel(SpanF32Args a) {
     if (S > 1) cluster.sync();
 }
 
-// Runs: blockIdx = (page, key/value head, sequence); the page's keys against all rows of the run that see them.
-__global__ void __launch_bounds__(SF_THREADS)
-run_f32_weigh_kernel(SpanF32Args a) {
-    extern __shared__ __align__(16) float sf[];
-    const int hd = a.hd, pitch = sf_pitch(hd), n4 = (hd + 3) / 4, G = a.nH / a.nKV;
-    float* ks = sf;                                                // [64][pitch]
-    float* qs = ks + GL_PAGE * pitch;                              // [8][pitch]
-    float* row_m = qs + 8 * pitch;                                 // [8]
-    float* row_l = row_m + 8;
-    float* halves = row_l + 8;                                     // [64]
-    int* row_last = (int*)(halves + GL_PAGE);                      // [8]
-    const int tid = threadIdx.x, b = blockIdx.z, g = blockIdx.y, p = blockIdx.x;
-    gl_grid_launch_dependents();
-    gl_grid_wait();
-    const int qlen = a.seq_qlen[b], ctx = a.seq_ctx[b], total = ctx + qlen;
-    if (qlen <= 0 || p * GL_PAGE >= total) return;
+// ---------------------------------------------------------------------------
+// Runs of several tokens: the weights their positions are given (the attention itself is attention_generic.cu's).  Rows are (query, query
+// head of a key/value head), queries first.  A first kernel finds each row's maximum and sum, a second walks the cache page by page:
+// w[j] += sum over the rows that see j of e^(s - m) / l.  Both multiply 64 rows with a page of keys at a time: a thread has 8 x 4 of the
+// scores in registers and reads 12 pieces of 16 bytes for 128 products, so the FMA pipe bounds them.  Where there are few pages and heads
+// the rows are shared out among ``parts`` blocks, whose sums a last kernel adds up in order.
+// ---------------------------------------------------------------------------
+struct RunF32Args {
+    const float* q;               // [rows, nH*hd], scaled
+    const float* k_cache;         // [pages, nKV, GL_PAGE, hd]
+    const int* seq_row;           // [B] first row of q
+    const int* seq_qlen;          // [B]
+    const int* seq_ctx;           // [B]
+    const int* pages;             // [B, max_pages]
+    float* ml;                    // [nH, rows, 2]: maximum, sum
+    float* weights;               // [pages, nKV, GL_PAGE]
+    float* sums;                  // [parts, B, nKV, reach], where parts > 1
+    int B, nH, nKV, max_pages, n_pages, reach, last, parts, rows, hd;
+};
+#define RF_ROWS 64
+// rows [r0, r0 + 64) of a run to the pitch of shared memory; what lies behind ``end`` or the head size is zero
+__device__ __forceinline__ void rf_load_rows(float* dst, const RunF32Args& a, int row0, int g, int G, int r0, int end, int pitch) {
+    const unsigned d = (unsigned)__cvta_generic_to_shared(dst);
+    const int vec = (a.hd & 3) == 0 ? 4 : 1, n = (a.hd + 3) / 4 * (4 / vec);
+    for (int i = threadIdx.x; i < RF_ROWS * n; i += SF_THREADS) {
+        const int r = i / n, c = (i - r * n) * vec, row = r0 + r, tok = row / G;
+        const bool ok = row < end && c < a.hd;
+        const float* src = ok ? a.q + ((size_t)(row0 + tok) * a.nH + g * G + row - tok * G) * a.hd + c : a.q;
+        if (vec == 4) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d + (r * pitch + c) * 4), "l"(src), "r"(ok ? 16 : 0));
+        else asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(d + (r * pitch + c) * 4), "l"(src), "r"(ok ? 4 : 0));
+    }
+}
+// scores of rows ty + 8 i with keys tx + 16 j
+__device__ __forceinline__ void rf_scores(const float* q, const float* k, int pitch, int n4, int ty, int tx, float (&s)[8][4]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[i][j] = 0.f;
+    for (int c = 0; c < n4; ++c) {
+        float4 x[8], y[4];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = *(const float4*)(q + (ty + 8 * i) * pitch + 4 * c);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[j] = *(const float4*)(k + (tx + 16 * j) * pitch + 4 * c);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                s[i][j] = fmaf(x[i].x, y[j].x, fmaf(x[i].y, y[j].y, fmaf(x[i].z, y[j].z, fmaf(x[i].w, y[j].w, s[i][j]))));
+    }
+}
+__device__ __forceinline__ void rf_load_keys(float* dst, const RunF32Args& a, int b, int g, int p, int total, int pitch) {
     const size_t page = (size_t)gl_checked(a.pages[(size_t)b * a.max_pages + p], a.n_pages, GL_BAD_PAGE);
-    sf_load_page(ks, a.k_cache + (page * a.nKV + g) * GL_PAGE * hd, min(GL_PAGE, total - p * GL_PAGE), hd, pitch);
+    sf_load_page(dst, a.k_cache + (page * a.nKV + g) * GL_PAGE * a.hd, min(GL_PAGE, total - p * GL_PAGE), a.hd, pitch);
+}
+
+// blockIdx = (tile of 64 rows from the far end, key/value head, sequence)
+__global__ void __launch_bounds__(SF_THREADS)
+run_f32_stats_kernel(RunF32Args a) {
+    extern __shared__ __align__(16) float sf[];
+    const int pitch = sf_pitch(a.hd), n4 = (a.hd + 3) / 4, tile = RF_ROWS * pitch, G = a.nH / a.nKV;
+    const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4, b = blockIdx.z, g = blockIdx.y;
+    gl_grid_wait();
+    gl_grid_launch_dependents();
+    const int qlen = a.seq_qlen[b], ctx = a.seq_ctx[b], row0 = a.seq_row[b], end = qlen * G;
+    const int start = a.last > 0 ? max(0, qlen - a.last) * G : 0;
+    const int r0 = start + (int)(gridDim.x - 1 - blockIdx.x) * RF_ROWS;
+    if (r0 >= end) return;
+    const int n = (ctx + (min(r0 + RF_ROWS, end) - 1) / G) / GL_PAGE + 1, least = ctx + r0 / G;
+    rf_load_rows(sf, a, row0, g, G, r0, end, pitch);
+    rf_load_keys(sf + tile, a, b, g, 0, ctx + qlen, pitch);
+    float m[8], l[8];
+    int last[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) { m[i] = -INFINITY; l[i] = 0.f; last[i] = ctx + (r0 + ty + 8 * i) / G; }
+    for (int p = 0; p < n; ++p) {
+        asm volatile("cp.async.commit_group;");
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        __syncthreads();
+        if (p + 1 < n) rf_load_keys(sf + (1 + ((p + 1) & 1)) * tile, a, b, g, p + 1, ctx + qlen, pitch);
+        float s[8][4];
+        rf_scores(sf, sf + (1 + (p & 1)) * tile, pitch, n4, ty, tx, s);
+        const bool cut = p * GL_PAGE + GL_PAGE - 1 > least;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            float mx = m[i];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (cut && p * GL_PAGE + tx + 16 * j > last[i]) s[i][j] = -INFINITY;
+                mx = fmaxf(mx, s[i][j]);
+            }
+            const float mu = mx == -INFINITY ? 0.f : mx;
+            float sum = 0.f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) sum += expf(s[i][j] - mu);
+            l[i] = m[i] == mx ? l[i] + sum : fmaf(l[i], expf(m[i] - mx), sum);
+            m[i] = mx;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+#pragma unroll
+        for (int x = 1; x < 16; x <<= 1) {
+            const float om = __shfl_xor_sync(0xffffffffu, m[i], x), ol = __shfl_xor_sync(0xffffffffu, l[i], x), mx = fmaxf(m[i], om);
+            l[i] = l[i] * sf_factor(m[i], mx) + ol * sf_factor(om, mx);
+            m[i] = mx;
+        }
+        const int row = r0 + ty + 8 * i;
+        if (tx == 0 && row < end) *(float2*)(a.ml + ((size_t)(g * G + row % G) * a.rows + row0 + row / G) * 2) = make_float2(m[i], l[i]);
+    }
+}
+
+// blockIdx = (page and part, key/value head, sequence): the first pages, which most rows see, start first
+__global__ void __launch_bounds__(SF_THREADS)
+run_f32_weigh_kernel(RunF32Args a) {
+    extern __shared__ __align__(16) float sf[];
+    const int pitch = sf_pitch(a.hd), n4 = (a.hd + 3) / 4, tile = RF_ROWS * pitch, G = a.nH / a.nKV;
+    float2* stat = (float2*)(sf + 3 * tile);                       // [2][64]: maximum, 1 / sum
+    float* sums = (float*)(stat + 2 * RF_ROWS);                    // [8][64]
+    const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4, b = blockIdx.z, g = blockIdx.y, p = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
+    gl_grid_wait();
+    gl_grid_launch_dependents();
+    const int qlen = a.seq_qlen[b], ctx = a.seq_ctx[b], row0 = a.seq_row[b], end = qlen * G, total = ctx + qlen;
+    if (qlen <= 0 || p * GL_PAGE >= total) return;
+    const int start = max(max(0, p * GL_PAGE - ctx), a.last > 0 ? qlen - a.last : 0) * G;
+    const int all = (end - start + RF_ROWS - 1) / RF_ROWS, t0 = (int)((long long)all * part / a.parts), n = (int)((long long)all * (part + 1) / a.parts) - t0;
+    auto load = [&](int i) {
+        const int r0 = start + (t0 + i) * RF_ROWS;
+        rf_load_rows(sf + (1 + (i & 1)) * tile, a, row0, g, G, r0, end, pitch);
+        if (tid < RF_ROWS) {
+            const int row = r0 + tid;
+            float2 v = make_float2(0.f, 1.f);
+            if (row < end) v = *(const float2*)(a.ml + ((size_t)(g * G + row % G) * a.rows + row0 + row / G) * 2);
+            stat[(i & 1) * RF_ROWS + tid] = make_float2(v.x, 1.0f / v.y);
+        }
+    };
+    rf_load_keys(sf, a, b, g, p, total, pitch);
+    if (n > 0) load(0);
+    float given[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < n; ++i) {
+        asm volatile("cp.async.commit_group;");
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        __syncthreads();
+        if (i + 1 < n) load(i + 1);
+        float s[8][4];
+        rf_scores(sf + (1 + (i & 1)) * tile, sf, pitch, n4, ty, tx, s);
+        const int r0 = start + (t0 + i) * RF_ROWS;
+        const bool cut = p * GL_PAGE + GL_PAGE - 1 > ctx + r0 / G || r0 + RF_ROWS > end;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const float2 x = stat[(i & 1) * RF_ROWS + ty + 8 * k];
+            const int row = r0 + ty + 8 * k, last = row < end ? ctx + row / G : -1;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float w = expf(s[k][j] - x.x) * x.y;
+                given[j] += !cut || p * GL_PAGE + tx + 16 * j <= last ? w : 0.f;
+            }
+        }
+    }
     asm volatile("cp.async.commit_group;");
     asm volatile("cp.async.wait_group 0;" ::: "memory");
-    const int key = tid & 63, half = tid >> 6, j = p * GL_PAGE + key;
-    const int i0 = max(max(0, p * GL_PAGE - ctx), a.last > 0 ? qlen - a.last : 0);
-    float given = 0.f;
-    for (int r0 = i0 * G; r0 < qlen * G; r0 += 8) {
-        __syncthreads();
-        for (int i = tid; i < 8 * 4 * n4; i += SF_THREADS) {
-            const int r = i / (4 * n4), c = i - r * 4 * n4, row = r0 + r;
-            const bool ok = row < qlen * G && c < hd;
-            qs[r * pitch + c] = ok ? a.q[((size_t)(a.seq_row[b] + row / G) * a.nH + g * G + row % G) * hd + c] : 0.f;
-        }
-        if (tid < 8) {
-            const int row = r0 + tid;
-            const bool ok = row < qlen * G;
-            const float* ml = a.part_ml + ((size_t)(a.seq_row[b] + (ok ? row / G : 0)) * a.nH + g * G + (ok ? row % G : 0)) * 2;
-            row_m[tid] = ml[0];
-            row_l[tid] = ml[1];
-            row_last[tid] = ok ? ctx + row / G : -1;
-        }
-        __syncthreads();
-        float s[4];
-        sf_scores<4>(ks + key * pitch, qs + half * 4 * pitch, pitch, n4, s);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (j <= row_last[half * 4 + i]) given += expf(s[i] - row_m[half * 4 + i]) / row_l[half * 4 + i];
-    }
-    if (half) halves[key] = given;
+    for (int j = 0; j < 4; ++j) sums[ty * GL_PAGE + tx + 16 * j] = given[j];
     __syncthreads();
-    if (half || j >= total) return;
-    float* w = a.weights + (page * a.nKV + g) * GL_PAGE + key;
-    given += halves[key];
-    *w = j < ctx ? *w + given : given;
+    const int key = p * GL_PAGE + tid;
+    if (tid >= GL_PAGE || key >= total) return;
+    float x = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x += sums[k * GL_PAGE + tid];
+    if (a.parts > 1) {
+        if (key < a.reach) a.sums[(((size_t)part * a.B + b) * a.nKV + g) * a.reach + key] = x;
+    } else {
+        float* w = a.weights + ((size_t)gl_checked(a.pages[(size_t)b * a.max_pages + p], a.n_pages, GL_BAD_PAGE) * a.nKV + g) * GL_PAGE + tid;
+        if (key < ctx) atomicAdd(w, x);                            // (one addition a position)
+        else *w = x;
+    }
+}
+
+// the parts' sums, in order: blockIdx = (stretch of the positions, key/value head, sequence)
+__global__ void run_f32_join_kernel(RunF32Args a) {
+    gl_grid_wait();
+    gl_grid_launch_dependents();
+    const int b = blockIdx.z, g = blockIdx.y, j = blockIdx.x * blockDim.x + threadIdx.x;
+    const int ctx = a.seq_ctx[b], qlen = a.seq_qlen[b];
+    if (qlen <= 0 || j >= min(ctx + qlen, a.reach)) return;
+    float x = 0.f;
+    for (int p = 0; p < a.parts; ++p) x += a.sums[(((size_t)p * a.B + b) * a.nKV + g) * a.reach + j];
+    float* w = a.weights + ((size_t)gl_checked(a.pages[(size_t)b * a.max_pages + j / GL_PAGE], a.n_pages, GL_BAD_PAGE) * a.nKV + g) * GL_PAGE + j % GL_PAGE;
+    if (j < ctx) atomicAdd(w, x);
+    else *w = x;
 }
 
 template <typename F>
@@ -753,24 +876,26 @@ GL_API int gl_attention_weighed_f32(const SpanF32Args* args, cudaStream_t stream
     return rc != GL_OK || a.joined ? rc : launch_join(a, stream);
 }
 
-// runs of up to max_qlen tokens
-GL_API int gl_attention_weighed_runs_f32(const SpanF32Args* args, int max_qlen, cudaStream_t stream) {
-    SpanF32Args a = *args;
-    a.early = a.held = a.joined = 0;
+// The weights of runs of up to max_qlen tokens.
+GL_API int gl_attention_weigh_runs_f32(const RunF32Args* args, int max_qlen, cudaStream_t stream) {
+    const RunF32Args& a = *args;
     if (a.B <= 0 || max_qlen <= 0) return GL_OK;
-    int rc = f32_checked(a);
-    if (rc != GL_OK) return rc;
-    if (!a.weights || !a.part_ml || !a.seq_row || !a.seq_qlen || a.reach <= 0 || a.last < 0) return GL_ERR_SHAPE;
-    const long long tiles = ((long long)max_qlen * (a.nH / a.nKV) + 7) / 8;
-    if (tiles > 0x7fffffffLL) return GL_ERR_SHAPE;
-    if ((rc = launch_f32<8, SF_RUN>(a, dim3((unsigned)tiles, a.nKV, a.B), stream)) != GL_OK) return rc;
+    if (a.nH <= 0 || a.nKV <= 0 || a.nH % a.nKV || a.nKV > 65535 || a.B > 65535 || a.hd <= 0 || a.hd > SF_MAX_HD || a.max_pages <= 0 || a.reach <= 0 || a.last < 0) return GL_ERR_SHAPE;
+    if (!a.ml || !a.weights || !a.seq_row || !a.seq_qlen || a.parts < 1 || (a.parts > 1 && !a.sums)) return GL_ERR_SHAPE;
+    if (((((uintptr_t)a.q | (uintptr_t)a.k_cache) & 15) && a.hd % 4 == 0) || ((uintptr_t)a.ml & 7)) return GL_ERR_ALIGN;
+    const int G = a.nH / a.nKV, counted = a.last > 0 && a.last < max_qlen ? a.last : max_qlen;
+    const long long tiles = ((long long)counted * G + RF_ROWS - 1) / RF_ROWS, pages = (long long)((a.reach + GL_PAGE - 1) / GL_PAGE) * a.parts;
+    if (tiles > 0x7fffffffLL || pages > 0x7fffffffLL) return GL_ERR_SHAPE;
     static bool allowed[64] = {};
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) { cudaGetLastError(); return GL_ERR_DRIVER; }
-    auto need = [](int hd) { return sizeof(float) * ((GL_PAGE + 8) * (size_t)sf_pitch(hd) + 16 + GL_PAGE) + sizeof(int) * 8; };
+    auto need = [](int hd) { return sizeof(float) * (3 * RF_ROWS * (size_t)sf_pitch(hd) + 4 * RF_ROWS + 8 * GL_PAGE); };
     if (!allowed[dev]) {
-        if (allow_smem(run_f32_weigh_kernel, need(SF_MAX_HD)) != GL_OK) return GL_ERR_SMEM;
+        if (allow_smem(run_f32_stats_kernel, need(SF_MAX_HD)) != GL_OK || allow_smem(run_f32_weigh_kernel, need(SF_MAX_HD)) != GL_OK) return GL_ERR_SMEM;
         allowed[dev] = true;
     }
-    return gl_launch(run_f32_weigh_kernel, dim3((a.reach + GL_PAGE - 1) / GL_PAGE, a.nKV, a.B), dim3(SF_THREADS), need(a.hd), stream, 1, a);
+    int rc = gl_launch(run_f32_stats_kernel, dim3((unsigned)tiles, a.nKV, a.B), dim3(SF_THREADS), need(a.hd), stream, 1, a);
+    if (rc == GL_OK) rc = gl_launch(run_f32_weigh_kernel, dim3((unsigned)pages, a.nKV, a.B), dim3(SF_THREADS), need(a.hd), stream, 1, a);
+    if (rc != GL_OK || a.parts == 1) return rc;
+    return gl_launch(run_f32_join_kernel, dim3((a.reach + 255) / 256, a.nKV, a.B), dim3(256), 0, stream, 1, a);
 }

@@ -995,12 +995,16 @@ class _SpanArgs(Structure):
 
 
 class _SpanF32Args(Structure):
-    _fields_ = _SpanArgs._fields_[:-3] + [("hd", c_int), ("last", c_int), ("early", c_int), ("held", c_int), ("joined", c_int)]
+    _fields_ = _SpanArgs._fields_[:-3] + [("hd", c_int), ("early", c_int), ("held", c_int), ("joined", c_int)]
 
 
 class _RunArgs(Structure):
     _fields_ = [(n, c_void_p) for n in ("q", "k_cache", "seq_row", "seq_qlen", "seq_ctx", "pages", "ml", "weights", "sums")] + \
                [(n, c_int) for n in ("B", "nH", "nKV", "max_pages", "n_pages", "reach", "last", "parts", "rows")]
+
+
+class _RunF32Args(Structure):
+    _fields_ = _RunArgs._fields_ + [("hd", c_int)]
 
 
 def _fit(here: int, dtype, *tensors) -> bool:
@@ -1119,33 +1123,33 @@ def attention_weighed(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor,
         _check(_launch(lib.gl_attention_weighed_f32 if f32 else lib.gl_attention_weighed, byref(a), _stream()), "attention_weighed",
                2 if slots else 1)
         return
-    ml = empty((q.shape[0], num_heads, 2), torch.float32, q.device)
-    if f32:
-        a = _SpanF32Args(q.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), seq_qstart.data_ptr(), seq_qlen.data_ptr(),
-                         seq_ctx.data_ptr(), pages.data_ptr(), None, None, None, None, ml.data_ptr(), None, weights.data_ptr(),
-                         B, num_heads, num_kv_heads, pages.shape[1], n_pages, 0, 1, 1, 1, max_len, head_dim, last)
-        _check(_launch(lib.gl_attention_weighed_runs_f32, byref(a), c_int(max_qlen), _stream()), "attention_weighed", 2)
-        return
-    tensor = USE_TCGEN05 and head_dim <= TC_ATTENTION_MAX_HEAD_DIM
-    parts, sums = 1, None
+    ml = empty((num_heads, q.shape[0], 2), torch.float32, q.device)
+    group, counted = num_heads // num_kv_heads, min(last, max_qlen) if last else max_qlen
+    tensor = not f32 and USE_TCGEN05 and head_dim <= TC_ATTENTION_MAX_HEAD_DIM
     if tensor:
         # the attention leaves its rows' statistics behind
         t = _attn_args(q, out, k_cache, v_cache, seq_qstart, seq_qlen, seq_ctx, pages, num_heads, num_kv_heads, head_dim, 0, max_qlen, 1.0)
         st = _AttnStats(ml.data_ptr(), q.shape[0])
         fn = _lib("attention_prefill_tc.cu", (f"GL_HEAD_DIM={head_dim}",)).gl_attention_prefill_tc_stats
         _check(_launch(fn, byref(t), byref(st), c_int(q.shape[0]), c_int(n_pages), _stream()), "attention_prefill_tc")
-        # few keys and heads: their queries are shared out, to even out what the SMs have to do
-        group, counted = num_heads // num_kv_heads, min(last, max_qlen) if last else max_qlen
-        blocks = -(-max_len // 128) * num_kv_heads * B
-        parts = max(1, min(2 * sm_count(q.device) // blocks, group * -(-counted // 128)))
+    else:
+        run = attention_generic if f32 else attention_prefill
+        run(q, out, k_cache, v_cache, seq_qstart, seq_qlen, seq_ctx, pages, num_heads, num_kv_heads, head_dim, max_qlen)
+    # few keys and heads: their queries are shared out, to even out what the SMs have to do
+    parts, sums = 1, None
+    if tensor or f32:
+        keys, rows = (128, 128) if tensor else (64, 64 // group if group < 64 else 1)
+        blocks = -(-max_len // keys) * num_kv_heads * B
+        parts = max(1, min((2 if tensor else 6) * sm_count(q.device) // blocks, (group if tensor else 1) * -(-counted // rows)))
         if parts > 1:
             sums = empty((parts, B, num_kv_heads, max_len), torch.float32, q.device)
+    fields = (q.data_ptr(), k_cache.data_ptr(), seq_qstart.data_ptr(), seq_qlen.data_ptr(), seq_ctx.data_ptr(), pages.data_ptr(),
+              ml.data_ptr(), weights.data_ptr(), _addr(sums), B, num_heads, num_kv_heads, pages.shape[1], n_pages, max_len, last, parts, q.shape[0])
+    if f32:
+        _check(_launch(lib.gl_attention_weigh_runs_f32, byref(_RunF32Args(*fields, head_dim)), c_int(max_qlen), _stream()), "attention_weighed", 3 if parts > 1 else 2)
     else:
-        attention_prefill(q, out, k_cache, v_cache, seq_qstart, seq_qlen, seq_ctx, pages, num_heads, num_kv_heads, head_dim, max_qlen)
-    a = _RunArgs(q.data_ptr(), k_cache.data_ptr(), seq_qstart.data_ptr(), seq_qlen.data_ptr(), seq_ctx.data_ptr(), pages.data_ptr(),
-                 ml.data_ptr(), weights.data_ptr(), _addr(sums), B, num_heads, num_kv_heads, pages.shape[1], n_pages, max_len, last, parts, q.shape[0])
-    _check(_launch(lib.gl_attention_weigh_runs, byref(a), c_int(max_qlen), c_int(q.shape[0]), c_int(tensor), c_int(sm_count(q.device) if tensor else 0), _stream()),
-           "attention_weighed", 2 if not tensor or parts > 1 else 1)
+        _check(_launch(lib.gl_attention_weigh_runs, byref(_RunArgs(*fields)), c_int(max_qlen), c_int(q.shape[0]), c_int(tensor),
+                       c_int(sm_count(q.device) if tensor else 0), _stream()), "attention_weighed", 2 if not tensor or parts > 1 else 1)
 
 
 class _AttnStats(Structure):
