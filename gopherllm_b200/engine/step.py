@@ -54,6 +54,10 @@ class StepContext:
         self.side_stream = None          # a second stream blocks may fork onto (decode steps only)
 
 
+# Bytes that reading shared pages once must spare a layer's decode step before it takes kernels of its own, in place of attention that takes
+# the projection's rows itself or of the whole layer as one kernel.  Measured with 32 heads of 64 and 80: two sequences gain from some 1,900
+# shared positions on (16 to 20 MB), eight from between 256 and 1,024 (18 loses, 59 gains), 32 from between 256 and 300 (65 loses 12 %, 81 gains).
+SHARED_BYTES, SHARED_BYTES_A_SEQUENCE = 16 << 20, 2 << 20
 GRAPH_F32_RUN_BYTES = 128 << 20      # weights of a model for each run of its schedule, up to which 32-bit decode steps are captured
 
 
@@ -251,7 +255,7 @@ class Engine:
         # (sized for a bucket of lengths, as captured steps are)
         own = self._length_bucket(max(c + 1 - s for c, s in zip(ctxs, shared)))
         layouts = (ops.PrefixLayout(groups, len(slots), *heads, self.act_dtype, own, ops.sm_count(self.device)) for heads in self.shared_heads)
-        return tuple(x for x in layouts if x.n_items)
+        return tuple(x for x in layouts if x.n_items and x.spared >= SHARED_BYTES + len(slots) * SHARED_BYTES_A_SEQUENCE)
 
     def _stage(self, buf: np.ndarray) -> torch.Tensor:
         """The descriptor in pinned host memory, ready for an asynchronous copy."""

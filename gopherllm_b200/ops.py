@@ -871,8 +871,8 @@ class PrefixLayout:
         self.rows = (128 if most <= 128 else 256) if tensor else min(most, span_rows(dtype, head_dim))      # rows of an item
         tiles = [-(-len(m) * group // self.rows) for m, _ in checked]
         # Where reading the shared pages once spares little, every sequence reads them with its own: a kernel less.
-        spared = sum((len(m) - 1) * p for m, p in checked) * 2 * PAGE * num_kv_heads * head_dim * (4 if dtype == torch.float32 else 2)
-        if spared < PREFIX_SPARED_BYTES:
+        self.spared = sum((len(m) - 1) * p for m, p in checked) * 2 * PAGE * num_kv_heads * head_dim * (4 if dtype == torch.float32 else 2)
+        if self.spared < PREFIX_SPARED_BYTES:
             own, checked, tiles = own + PAGE * max((p for _, p in checked), default=0), [], []
         # Blocks walk equal stretches of pages, as few rounds of them as the tiles allow: on the tensor cores a block an SM at a time, else
         # what the registers and shared memory hold.
@@ -917,7 +917,7 @@ class PrefixLayout:
                 self.items_at, self.shared_at)
 
 
-PREFIX_SPARED_BYTES = 12 << 20       # (see PrefixLayout)
+PREFIX_SPARED_BYTES = 12 << 20       # bytes that are worth a kernel for the shared pages: a launch and its partial results, some 4 us
 SPAN_FACTOR_BYTES, SPAN_HELD_BYTES = 24 * 1024, 56 * 1024      # shared memory for the factors of a row's parts, for a block's scores
 
 

@@ -13,7 +13,9 @@ pytestmark = pytest.mark.gpu
 def load(monkeypatch):
     import gopherllm_b200 as gl
     from gopherllm_b200 import ops
-    monkeypatch.setattr(ops, "PREFIX_SPARED_BYTES", 0)             # (tiny models would never be worth it)
+    from gopherllm_b200.engine import step
+    for where, name in ((ops, "PREFIX_SPARED_BYTES"), (step, "SHARED_BYTES"), (step, "SHARED_BYTES_A_SEQUENCE")):
+        monkeypatch.setattr(where, name, 0)                        # (tiny models would never be worth it)
     models = []
 
     def make(name, dtype, **kw):
@@ -103,6 +105,82 @@ def test_decode_loop_on_shared_pages(load):
             m.close_sequence(x)
         return out
     assert run(True) == run(False)
+
+
+def test_heads_with_a_gate_and_values_that_are_keys(load):
+    """The mixer that has both, without a window, on shared pages and in a cache that is weighed: as without either."""
+    import gopherllm_b200 as gl
+    import dibedra_models
+    cfg = dict(dibedra_models.BETA)
+    for dtype in ("float32", "bfloat16"):
+        rng = np.random.default_rng(4)
+        m = gl.load_random(cfg, seed=1, dtype=dtype, max_tokens=64 * 30)
+        V = m.spec.vocab
+        base, tails = tiny.prompt(rng, 70, V), [tiny.prompt(rng, 4, V) for _ in range(3)]
+
+        def run(shared):
+            s = m.open_sequence()
+            m.step([(s, base)], [[]])
+            slots = [s]
+            for _ in tails[1:]:
+                if shared:
+                    slots.append(m.fork_sequence(s))
+                else:
+                    slots.append(m.open_sequence())
+                    m.step([(slots[-1], base)], [[]])
+            out = [m.step([(x, [t[i]]) for x, t in zip(slots, tails)]).cpu().numpy() for i in range(4)]
+            for x in slots:
+                m.close_sequence(x)
+            return np.stack(out)
+        err, bound = tiny.close(run(True), run(False), dtype)
+        assert err <= bound, (dtype, err, bound)
+        m.engine.cache.check()
+        m.close()
+
+
+def test_gated_heads_are_weighed(load):
+    """Weighing changes no logits, with a gate on the result and values that are keys either; and all layers without a window can be cut."""
+    import gopherllm_b200 as gl
+    import dibedra_models
+    cfg = dict(dibedra_models.BETA)
+    cfg["layers"] = [dict(cfg["layers"][0], weights_of=None, mixer=dibedra_models._B1, mlp=None) for _ in range(2)]
+    cfg["layers"] = [{k: v for k, v in x.items() if v is not None or k == "mlp"} for x in cfg["layers"]]
+    rng = np.random.default_rng(6)
+    text = tiny.prompt(rng, 100, 257)
+    out = {}
+    for weigh in (False, True):
+        m = gl.load_random(cfg, seed=1, dtype="float32", max_tokens=64 * 10, weigh=weigh)
+        s = m.open_sequence()
+        got = [m.step([(s, text[:90])])] + [m.step([(s, [t])]) for t in text[90:]]
+        out[weigh] = torch.cat(got).cpu().numpy()
+        if weigh:
+            m.evict([s], 64, recent=64)
+            assert m.engine.cache.length(s) == 64 and np.isfinite(m.step([(s, [5])]).cpu().numpy()).all()
+        m.close()
+    err, bound = tiny.close(out[True], out[False], "float32")
+    assert err <= bound, (err, bound)
+
+
+@pytest.mark.parametrize("module,name", [("vopedra_models", "ALPHA"), ("gozolix_models", "ALPHA"), ("lilupel_models", "ALPHA"), ("nakurax_models", "ALPHA"), ("darusun_models", "ALPHA")])
+def test_designs_with_state_and_windows_can_be_forked_whole(load, module, name):
+    """State rows are copied, begun pages too, pages behind a window shared or given back: a forked sequence goes on as the one it was forked from."""
+    import importlib
+    import gopherllm_b200 as gl
+    m = gl.load_random(dict(getattr(importlib.import_module(module), name)), seed=2, dtype="float32", max_tokens=64 * 30)
+    rng = np.random.default_rng(5)
+    V = m.spec.vocab
+    s = m.open_sequence()
+    m.step([(s, tiny.prompt(rng, 75, V))], [[]])
+    for n in (1, 1, 3, 1):
+        f = m.fork_sequence(s)
+        new = tiny.prompt(rng, n, V)
+        a = m.step([(s, new), (f, new)]).cpu().numpy()
+        assert np.isfinite(a).all() and np.abs(a[0] - a[1]).max() <= 1e-5 * max(1.0, np.abs(a).max())
+        m.close_sequence(f)
+        m.engine.cache.check()
+    m.close_sequence(s)
+    m.engine.cache.check()
+    m.close()
 
 
 class Forgetful:
