@@ -471,7 +471,7 @@ attn_span_join_kernel(SpanArgs a) {
 
 
 // ---------------------------------------------------------------------------
-// One or two query heads on a key/value head: a sequence's own pages go from the cache straight to registers, as in
+// One or two query heads on a key/value head, larger than 64: a sequence's own pages go from the cache straight to registers, as in
 // attention_spans_f32.cu.  Eight lanes take a key, a warp four keys at a time with 2 UN of their rows under way; no barrier stands between
 // two keys, and the weights stay in 32 bits.  Eight columns of a tensor-core product would be empty but for one or two; what
 // bounds it is memory.
@@ -684,12 +684,16 @@ static int launch_stream(const SpanArgs& a, dim3 grid, int cluster, cudaStream_t
 
 template <int MODE>
 static int launch_spans(const SpanArgs& a, int rows, dim3 grid, int cluster, cudaStream_t stream) {
-    if constexpr (MODE != SP_ITEM) {
+    // One or two rows a block: the products on CUDA cores, where a row of the cache is long enough that the tensor cores' eight columns,
+    // most of them empty, cost more than the sums over eight lanes.  us, streamed against tensor cores, 8 sequences of 300 to 2,047
+    // positions, 16 query heads, with weights: one row, heads of 32: 13.0 / 12.3, of 64: 19.0 / 16.6, of 128: 21.1 / 28.5, of
+    // 256: 39.5 / 60.9; two rows, of 64: 11.3 / 11.0, of 128: 17.2 / 21.5, of 256: 33.8 / 52.7.
+    if constexpr (MODE != SP_ITEM && SP_HD > 64) {
         if (a.nH == a.nKV) return launch_stream<1, MODE>(a, grid, cluster, stream);
         if (a.nH == 2 * a.nKV) return launch_stream<2, MODE>(a, grid, cluster, stream);
     }
     // Pages in flight: two; one, and more blocks an SM, where a block has one page or two to walk (behind shared pages: 1,024 blocks
-    // of a page each, heads of 128, 59 us against 64 with what the shared pages take).
+    // of a page each, heads of 128: 5 us less).
     if constexpr (MODE == SP_JOIN)
         if (rows <= 8 && a.short_spans) return launch_span<1, MODE, 1>(a, grid, cluster, stream);
     if (rows <= 8) return launch_span<1, MODE>(a, grid, cluster, stream);
@@ -846,6 +850,7 @@ shared_tc_kernel(SpanArgs a, const __grid_constant__ StMaps maps) {
     // tile t: score buffers at columns 256 t and 256 t + 64 (a page's weights overwrite the first 32 columns of its scores, two a
     // column), output at 256 t + 128.  A second tile without rows takes no part.
     const int tiles = rows_all > ST_BM ? 2 : 1;
+    int issued = 0;
 
     if (warp == PRODUCER) {
         if (lane == 0) {
@@ -862,6 +867,7 @@ shared_tc_kernel(SpanArgs a, const __grid_constant__ StMaps maps) {
 #pragma unroll
                 for (int c = 0; c < ST_VATOMS; ++c)
                     tma_load_2d(sV + st * ST_V_BYTES + c * ST_VATOM_BYTES, &maps.v, 64 * c, row, bar_f + 8 * st);
+                issued = j + 1;
             }
         }
     } else if (warp > PRODUCER) {
@@ -1023,10 +1029,11 @@ shared_tc_kernel(SpanArgs a, const __grid_constant__ StMaps maps) {
                 for (int c = 0; c < SP_HD; c += 16) {
                     unsigned t16[16];
                     tmem_ld16(tO + c, t16);
-                    if (real)
+                    if (real)                              // (a row a thread: whole 32-byte sectors)
 #pragma unroll
-                        for (int i = 0; i < 16; i += 4)
-                            *(uint4*)(a.part_o + at * SP_HD + c + i) = make_uint4(t16[i], t16[i + 1], t16[i + 2], t16[i + 3]);
+                        for (int i = 0; i < 16; i += 8)
+                            asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(a.part_o + at * SP_HD + c + i), "r"(t16[i]), "r"(t16[i + 1]),
+                                         "r"(t16[i + 2]), "r"(t16[i + 3]), "r"(t16[i + 4]), "r"(t16[i + 5]), "r"(t16[i + 6]), "r"(t16[i + 7]) : "memory");
                 }
                 if (real) { a.part_ml[at * 2] = m_run; a.part_ml[at * 2 + 1] = l_run; }
             } else {
@@ -1039,6 +1046,8 @@ shared_tc_kernel(SpanArgs a, const __grid_constant__ StMaps maps) {
     if (warp == PRODUCER) {
         tc_fence_after();
         tmem_dealloc(tmem, ST_TMEM_COLS(NT));
+        if (failed && lane == 0)                           // a wait ran out: nothing is left on its way into this block's memory
+            for (int j = max(0, issued - STAGES); j < issued; ++j) (void)mbar_wait(bar_f + 8 * (j % STAGES), (j / STAGES) & 1);
     }
     if (threadIdx.x == 0 && failed) atomicExch(&gl_wait_failed, 1);
 }
@@ -1060,6 +1069,7 @@ static int launch_shared_tc(const SpanArgs& a, const StMaps& maps, cudaStream_t 
 }
 static int shared_tc(const SpanArgs& a, int rows, cudaStream_t stream) {
     if (rows > 2 * ST_BM) return GL_ERR_SHAPE;
+    if ((uintptr_t)a.part_o & 31) return GL_ERR_ALIGN;
     StMaps maps;
     const uint64_t kv_rows = (uint64_t)a.n_pages * a.nKV * GL_PAGE;
     if (kv_rows > 0x7fffffffULL) return GL_ERR_SHAPE;      // (a row's number is a coordinate)

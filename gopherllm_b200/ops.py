@@ -960,7 +960,7 @@ def span_splits(batch: int, heads: int, pages: int, sms: int, dtype, head_dim: i
     blocks an SM or have no more than eight pages each.  Clusters have 1, 2, 4 or 8 blocks: six, 6 x 64 blocks of heads of 128, took
     23.5 us where four took 18.0."""
     blocks = max(1, batch * heads)
-    if dtype == torch.float32 or group <= 2:
+    if dtype == torch.float32 or (group <= 2 and head_dim > 64):
         per_sm = 4                                         # (registers; the others shared memory)
     else:
         per_sm = max(1, min(8, 227 * 1024 // (4 * PAGE * (2 * head_dim + 16) + 4096)))
