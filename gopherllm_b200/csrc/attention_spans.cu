@@ -20,6 +20,7 @@
 #include "decode_common.cuh"
 #include "tma.cuh"
 #include "tcgen05.cuh"
+#include "span_weights.cuh"
 #include <cooperative_groups.h>
 namespace cg = cooperative_groups;
 
@@ -53,6 +54,7 @@ struct SpanArgs {
     float* part_ml;               // [B, nH, slots, 2]
     float* scores;                // [B, nH, reach] or null
     float* weights;               // [pages, nKV, GL_PAGE] or null
+    float* given;                 // [B, nKV, reach]: where sequences may hold a page together, what each gives its positions; or null
     int B, nH, nKV, max_pages, n_pages, n_items, splits, slots, chunks, reach;
     int short_spans;              // a block has a page or two to walk
     int early, held;              // set by the launchers: see the kernel
@@ -158,8 +160,12 @@ __device__ __forceinline__ void span_join(const SpanArgs& a, const SpanEnd& e, c
             float given = 0.f;
             for (int r = 0; r < rows; ++r) given = fmaf(sp_exp2(fmaf(held[r * a.held + i], scale, -stat[2 * r])), stat[2 * r + 1], given);
             const int j = e.p_begin * GL_PAGE + i;
+            if (a.given) {
+                if (j < a.reach) a.given[((size_t)b * a.nKV + e.g) * a.reach + j] = given;
+                continue;
+            }
             float* w = a.weights + ((size_t)gl_checked(pg[j / GL_PAGE], a.n_pages, GL_BAD_PAGE) * a.nKV + e.g) * GL_PAGE + j % GL_PAGE;
-            // (an addition that nobody waits for; one a position, so their order is no matter)
+            // (an addition that nobody waits for; one a position, as no two sequences share it: their order is no matter)
             if (j < e.total - 1) atomicAdd(w, given);
             else *w = given;
         }
@@ -463,8 +469,12 @@ attn_span_join_kernel(SpanArgs a) {
         float given = 0.f;
 #pragma unroll 4
         for (int i = 0; i < G; ++i) given = fmaf(sp_exp2(fmaf(sc[(size_t)i * a.reach], SP_LOG2E, -ml_all[2 * i])), ml_all[2 * i + 1], given);
+        if (a.given) {
+            a.given[((size_t)b * a.nKV + g) * a.reach + j] = given;
+            continue;
+        }
         float* w = a.weights + ((size_t)gl_checked(a.pages[(size_t)b * a.max_pages + j / GL_PAGE], a.n_pages, GL_BAD_PAGE) * a.nKV + g) * GL_PAGE + j % GL_PAGE;
-        if (j < pos) atomicAdd(w, given);                  // (one addition a position)
+        if (j < pos) atomicAdd(w, given);                  // (one addition a position: no two sequences share it)
         else *w = given;
     }
 }
@@ -756,11 +766,13 @@ GL_API int gl_attention_weighed(const SpanArgs* args, cudaStream_t stream) {
         // (a pitch of 4 more than whole pages: the eight keys of four rows that a warp stores lie in different banks)
         a.held = ((a.reach + GL_PAGE - 1) / GL_PAGE + a.splits - 1) / a.splits * GL_PAGE + 4;
         if (a.chunks > 1 || a.splits > 8 || a.slots > 0 || (long long)a.held * G * (int)sizeof(float) > SP_HELD_BYTES) return GL_ERR_SHAPE;
-        return launch_spans<SP_JOIN>(a, G, grid, a.splits, stream);
+        rc = launch_spans<SP_JOIN>(a, G, grid, a.splits, stream);
+    } else {
+        if (a.slots < a.splits) return GL_ERR_SHAPE;
+        if ((rc = launch_spans<SP_SPLIT>(a, (G + a.chunks - 1) / a.chunks, grid, 1, stream)) != GL_OK) return rc;
+        rc = launch_join(a, stream);
     }
-    if (a.slots < a.splits) return GL_ERR_SHAPE;
-    if ((rc = launch_spans<SP_SPLIT>(a, (G + a.chunks - 1) / a.chunks, grid, 1, stream)) != GL_OK) return rc;
-    return launch_join(a, stream);
+    return rc != GL_OK || !a.given ? rc : launch_given_join(a, a.given, 1, 1, stream);
 }
 
 // ---------------------------------------------------------------------------
@@ -1100,8 +1112,8 @@ struct RunArgs {
     const int* pages;             // [B, max_pages]
     float* ml;                    // [nH, rows, 2]: maximum, sum
     float* weights;               // [pages, nKV, GL_PAGE]
-    float* sums;                  // [parts, B, nKV, reach], where parts > 1
-    int B, nH, nKV, max_pages, n_pages, reach, last, parts, rows;
+    float* sums;                  // [parts, B, nKV, reach], where parts > 1 or sequences may hold a page together (shared)
+    int B, nH, nKV, max_pages, n_pages, reach, last, parts, rows, shared;
 };
 #define RW_ROWS 64                                  // rows of q of a tile
 
@@ -1284,7 +1296,8 @@ run_weigh_kernel(RunArgs a) {
         const int j = j_lo + 8 * i;
         if (t == 0 && j < total) {
             float* w = a.weights + ((size_t)gl_checked(pg[p], a.n_pages, GL_BAD_PAGE) * a.nKV + g) * GL_PAGE + (j % GL_PAGE);
-            *w = j < ctx ? *w + given[i] : given[i];
+            if (!a.sums) *w = j < ctx ? *w + given[i] : given[i];
+            else if (j < a.reach) a.sums[((size_t)b * a.nKV + g) * a.reach + j] = given[i];
         }
     }
     sp_wait<0>();
@@ -1446,7 +1459,7 @@ run_weigh_tc_kernel(RunArgs a, int n_items, const __grid_constant__ RtMaps maps)
         const unsigned tS = tmem + ((unsigned)((warp & 3) * 32) << 16) + col;
         // What an item needs of global memory is asked for while the one before is under way, and its sums leave by additions that nobody
         // waits for: every stall here would be the tensor core's too.  (One addition a position: their order is no matter.)
-        auto skipped = [&](const RtItem& x) { return x.n == 0 && (a.parts == 1 || x.k0 >= x.ctx + x.qlen || x.qlen <= 0); };
+        auto skipped = [&](const RtItem& x) { return x.n == 0 && (!a.sums || x.k0 >= x.ctx + x.qlen || x.qlen <= 0); };
         auto item_from = [&](int& round) {                 // the next item with something to do, from ``round`` on
             RtItem x = {};
             for (; round < rounds; ++round) {
@@ -1541,7 +1554,7 @@ run_weigh_tc_kernel(RunArgs a, int n_items, const __grid_constant__ RtMaps maps)
                 const float (*f)[RT_COLS] = &sums[done & 1][threadIdx.x / RT_COLS * 4];
                 const int c = threadIdx.x % RT_COLS;
                 const float given = (f[0][c] + f[1][c]) + (f[2][c] + f[3][c]);
-                if (a.parts > 1) {
+                if (a.sums) {
                     if (key < a.reach) a.sums[(((size_t)x.part * a.B + x.b) * a.nKV + x.g) * a.reach + key] = given;
                 } else {
                     float* w = a.weights + ((size_t)mine * a.nKV + x.g) * GL_PAGE + key % GL_PAGE;
@@ -1561,19 +1574,6 @@ run_weigh_tc_kernel(RunArgs a, int n_items, const __grid_constant__ RtMaps maps)
         tmem_dealloc(tmem, 256);
     }
     if (threadIdx.x == 0 && failed) atomicExch(&gl_wait_failed, 1);
-}
-
-// the parts' sums, in order: blockIdx = (stretch of the positions, key/value head, sequence)
-__global__ void run_weigh_join_kernel(RunArgs a) {
-    gl_grid_wait();
-    gl_grid_launch_dependents();
-    const int b = blockIdx.z, g = blockIdx.y, j = blockIdx.x * blockDim.x + threadIdx.x;
-    const int ctx = a.seq_ctx[b], qlen = a.seq_qlen[b];
-    if (qlen <= 0 || j >= min(ctx + qlen, a.reach)) return;
-    float given = 0.f;
-    for (int p = 0; p < a.parts; ++p) given += a.sums[(((size_t)p * a.B + b) * a.nKV + g) * a.reach + j];
-    float* w = a.weights + ((size_t)gl_checked(a.pages[(size_t)b * a.max_pages + j / GL_PAGE], a.n_pages, GL_BAD_PAGE) * a.nKV + g) * GL_PAGE + j % GL_PAGE;
-    *w = j < ctx ? *w + given : given;
 }
 
 static int launch_run_tc(const RunArgs& a, int n_tokens, int sms, cudaStream_t stream) {
@@ -1599,8 +1599,7 @@ static int launch_run_tc(const RunArgs& a, int n_tokens, int sms, cudaStream_t s
     const long long items = (long long)((a.reach + ST_BM - 1) / ST_BM) * a.nKV * a.B * a.parts;
     if (items > 0x3fffffffLL || sms < 1) return GL_ERR_SHAPE;
     const int rc = gl_launch(run_weigh_tc_kernel, dim3((unsigned)(items < sms ? items : sms)), dim3(RT_THREADS), smem, stream, 1, a, (int)items, maps);
-    if (rc != GL_OK || a.parts == 1) return rc;
-    return gl_launch(run_weigh_join_kernel, dim3((a.reach + 255) / 256, a.nKV, a.B), dim3(256), 0, stream, 1, a);
+    return rc != GL_OK || !a.sums ? rc : launch_given_join(a, a.sums, a.parts, a.shared, stream);
 }
 #else
 static int launch_run_tc(const RunArgs&, int, int, cudaStream_t) { return GL_ERR_SHAPE; }
@@ -1613,6 +1612,7 @@ GL_API int gl_attention_weigh_runs(const RunArgs* args, int max_qlen, int n_toke
     const RunArgs& a = *args;
     if (a.B <= 0 || max_qlen <= 0) return GL_OK;
     if (a.nH <= 0 || a.nKV <= 0 || a.nH % a.nKV || a.B > 65535 || a.nKV > 65535 || a.reach <= 0 || a.last < 0 || !a.ml || !a.weights) return GL_ERR_SHAPE;
+    if ((a.parts > 1 || a.shared) && !a.sums) return GL_ERR_SHAPE;
     if (((uintptr_t)a.q | (uintptr_t)a.k_cache) & 15 || (uintptr_t)a.ml & 7) return GL_ERR_ALIGN;
     if (tensor) return known ? launch_run_tc(a, n_tokens, tensor, stream) : GL_ERR_SHAPE;
     static bool allowed[64] = {};
@@ -1633,5 +1633,6 @@ GL_API int gl_attention_weigh_runs(const RunArgs* args, int max_qlen, int n_toke
         const int rc = gl_launch(run_stats_kernel, dim3((unsigned)tiles, a.nKV, a.B), dim3(SP_THREADS), (size_t)RW_SMEM, stream, 1, a);
         if (rc != GL_OK) return rc;
     }
-    return gl_launch(run_weigh_kernel, dim3((a.reach + GL_PAGE - 1) / GL_PAGE, a.nKV, a.B), dim3(SP_THREADS), (size_t)RW_SMEM, stream, 1, a);
+    const int rc = gl_launch(run_weigh_kernel, dim3((a.reach + GL_PAGE - 1) / GL_PAGE, a.nKV, a.B), dim3(SP_THREADS), (size_t)RW_SMEM, stream, 1, a);
+    return rc != GL_OK || !a.sums ? rc : launch_given_join(a, a.sums, 1, a.shared, stream);
 }

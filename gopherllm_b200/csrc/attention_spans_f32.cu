@@ -6,6 +6,7 @@
 // banks; the rows' pieces are broadcasts), a warp takes the softmax of a row, and a thread adds up one or two dims of the
 // values for all rows.  So it is for heads that are no whole 16-byte pieces; all others stream (below).
 #include "common.cuh"
+#include "span_weights.cuh"
 #include <cooperative_groups.h>
 namespace cg = cooperative_groups;
 
@@ -28,6 +29,7 @@ struct SpanF32Args {
     float* part_ml;               // [B, nH, slots, 2]
     float* scores;                // [B, nH, reach] or null
     float* weights;               // [pages, nKV, GL_PAGE] or null
+    float* given;                 // [B, nKV, reach]: where sequences may hold a page together, what each gives its positions; or null
     int B, nH, nKV, max_pages, n_pages, n_items, splits, slots, chunks, reach, hd;
     int early, held, joined;      // set by the launchers
 };
@@ -285,8 +287,12 @@ span_f32_join_kernel(SpanF32Args a) {
         float given = 0.f;
 #pragma unroll 4
         for (int i = 0; i < G; ++i) given += expf(sc[(size_t)i * a.reach] - sf[2 * i]) / sf[2 * i + 1];
+        if (a.given) {
+            a.given[((size_t)b * a.nKV + g) * a.reach + j] = given;
+            continue;
+        }
         float* w = a.weights + ((size_t)gl_checked(a.pages[(size_t)b * a.max_pages + j / GL_PAGE], a.n_pages, GL_BAD_PAGE) * a.nKV + g) * GL_PAGE + j % GL_PAGE;
-        if (j < pos) atomicAdd(w, given);                          // (one addition a position)
+        if (j < pos) atomicAdd(w, given);                          // (one addition a position: no two sequences share it)
         else *w = given;
     }
 }
@@ -561,8 +567,12 @@ stream_f32_kernel(SpanF32Args a) {
             float given = 0.f;
             for (int r = 0; r < rows; ++r) given += expf(held[r * a.held + i] - stat[2 * r]) / stat[2 * r + 1];
             const int j = p_begin * GL_PAGE + i;
+            if (a.given) {
+                if (j < a.reach) a.given[((size_t)b * a.nKV + g) * a.reach + j] = given;
+                continue;
+            }
             float* w = a.weights + ((size_t)gl_checked(pg[j / GL_PAGE], a.n_pages, GL_BAD_PAGE) * a.nKV + g) * GL_PAGE + j % GL_PAGE;
-            if (j < total - 1) atomicAdd(w, given);               // (nobody waits for it; one a position, so their order is no matter)
+            if (j < total - 1) atomicAdd(w, given);               // (nobody waits for it; one a position, as no two sequences share it: their order is no matter)
             else *w = given;
         }
     }
@@ -585,8 +595,8 @@ struct RunF32Args {
     const int* pages;             // [B, max_pages]
     float* ml;                    // [nH, rows, 2]: maximum, sum
     float* weights;               // [pages, nKV, GL_PAGE]
-    float* sums;                  // [parts, B, nKV, reach], where parts > 1
-    int B, nH, nKV, max_pages, n_pages, reach, last, parts, rows, hd;
+    float* sums;                  // [parts, B, nKV, reach], where parts > 1 or sequences may hold a page together (shared)
+    int B, nH, nKV, max_pages, n_pages, reach, last, parts, rows, shared, hd;
 };
 #define RF_ROWS 64
 // rows [r0, r0 + 64) of a run to the pitch of shared memory; what lies behind ``end`` or the head size is zero
@@ -738,27 +748,13 @@ run_f32_weigh_kernel(RunF32Args a) {
     float x = 0.f;
 #pragma unroll
     for (int k = 0; k < 8; ++k) x += sums[k * GL_PAGE + tid];
-    if (a.parts > 1) {
+    if (a.sums) {
         if (key < a.reach) a.sums[(((size_t)part * a.B + b) * a.nKV + g) * a.reach + key] = x;
     } else {
         float* w = a.weights + ((size_t)gl_checked(a.pages[(size_t)b * a.max_pages + p], a.n_pages, GL_BAD_PAGE) * a.nKV + g) * GL_PAGE + tid;
-        if (key < ctx) atomicAdd(w, x);                            // (one addition a position)
+        if (key < ctx) atomicAdd(w, x);                            // (one addition a position: no two sequences share it)
         else *w = x;
     }
-}
-
-// the parts' sums, in order: blockIdx = (stretch of the positions, key/value head, sequence)
-__global__ void run_f32_join_kernel(RunF32Args a) {
-    gl_grid_wait();
-    gl_grid_launch_dependents();
-    const int b = blockIdx.z, g = blockIdx.y, j = blockIdx.x * blockDim.x + threadIdx.x;
-    const int ctx = a.seq_ctx[b], qlen = a.seq_qlen[b];
-    if (qlen <= 0 || j >= min(ctx + qlen, a.reach)) return;
-    float x = 0.f;
-    for (int p = 0; p < a.parts; ++p) x += a.sums[(((size_t)p * a.B + b) * a.nKV + g) * a.reach + j];
-    float* w = a.weights + ((size_t)gl_checked(a.pages[(size_t)b * a.max_pages + j / GL_PAGE], a.n_pages, GL_BAD_PAGE) * a.nKV + g) * GL_PAGE + j % GL_PAGE;
-    if (j < ctx) atomicAdd(w, x);
-    else *w = x;
 }
 
 template <typename F>
@@ -873,7 +869,8 @@ GL_API int gl_attention_weighed_f32(const SpanF32Args* args, cudaStream_t stream
         return GL_ERR_SHAPE;
     }
     rc = launch_f32_rows<SF_OWN>(a, (G + a.chunks - 1) / a.chunks, dim3(a.splits, a.nKV * a.chunks, a.B), a.joined ? a.splits : 1, stream);
-    return rc != GL_OK || a.joined ? rc : launch_join(a, stream);
+    if (rc == GL_OK && !a.joined) rc = launch_join(a, stream);
+    return rc != GL_OK || !a.given ? rc : launch_given_join(a, a.given, 1, 1, stream);
 }
 
 // The weights of runs of up to max_qlen tokens.
@@ -881,7 +878,7 @@ GL_API int gl_attention_weigh_runs_f32(const RunF32Args* args, int max_qlen, cud
     const RunF32Args& a = *args;
     if (a.B <= 0 || max_qlen <= 0) return GL_OK;
     if (a.nH <= 0 || a.nKV <= 0 || a.nH % a.nKV || a.nKV > 65535 || a.B > 65535 || a.hd <= 0 || a.hd > SF_MAX_HD || a.max_pages <= 0 || a.reach <= 0 || a.last < 0) return GL_ERR_SHAPE;
-    if (!a.ml || !a.weights || !a.seq_row || !a.seq_qlen || a.parts < 1 || (a.parts > 1 && !a.sums)) return GL_ERR_SHAPE;
+    if (!a.ml || !a.weights || !a.seq_row || !a.seq_qlen || a.parts < 1 || ((a.parts > 1 || a.shared) && !a.sums)) return GL_ERR_SHAPE;
     if (((((uintptr_t)a.q | (uintptr_t)a.k_cache) & 15) && a.hd % 4 == 0) || ((uintptr_t)a.ml & 7)) return GL_ERR_ALIGN;
     const int G = a.nH / a.nKV, counted = a.last > 0 && a.last < max_qlen ? a.last : max_qlen;
     const long long tiles = ((long long)counted * G + RF_ROWS - 1) / RF_ROWS, pages = (long long)((a.reach + GL_PAGE - 1) / GL_PAGE) * a.parts;
@@ -896,6 +893,5 @@ GL_API int gl_attention_weigh_runs_f32(const RunF32Args* args, int max_qlen, cud
     }
     int rc = gl_launch(run_f32_stats_kernel, dim3((unsigned)tiles, a.nKV, a.B), dim3(SF_THREADS), need(a.hd), stream, 1, a);
     if (rc == GL_OK) rc = gl_launch(run_f32_weigh_kernel, dim3((unsigned)pages, a.nKV, a.B), dim3(SF_THREADS), need(a.hd), stream, 1, a);
-    if (rc != GL_OK || a.parts == 1) return rc;
-    return gl_launch(run_f32_join_kernel, dim3((a.reach + 255) / 256, a.nKV, a.B), dim3(256), 0, stream, 1, a);
+    return rc != GL_OK || !a.sums ? rc : launch_given_join(a, a.sums, a.parts, a.shared, stream);
 }

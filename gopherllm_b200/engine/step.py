@@ -36,6 +36,7 @@ class StepContext:
     tok_place[T]: where the token's key and value lie among the sequence's cached ones; tok_pos unless the sequence has been cut.
     prefix: plans for pages that the step's sequences share, by heads (query heads, key/value heads, head size); empty if they
     share none or too little.
+    weights_shared: sequences of the step may lie on common pages of a cache that is weighed.
     """
 
     def __init__(self, device, act_dtype):
@@ -50,6 +51,7 @@ class StepContext:
         self.is_decode = False
         self.tok_place = None
         self.prefix: Dict[tuple, object] = {}
+        self.weights_shared = False
         self.next_block = None           # the block of the run behind the current one (models of several residual streams)
         self.side_stream = None          # a second stream blocks may fork onto (decode steps only)
 
@@ -68,8 +70,10 @@ def _pad4(n: int) -> int:
 class _Layout:
     """Offsets of the step's arrays inside one int32 buffer (each 16-byte aligned)."""
 
-    def __init__(self, T: int, B: int, M: int, groups: int, max_pages: int, places: bool = False, prefix: Sequence = ()):
+    def __init__(self, T: int, B: int, M: int, groups: int, max_pages: int, places: bool = False, prefix: Sequence = (),
+                 weights_shared: bool = False):
         self.T, self.B, self.M, self.groups, self.max_pages = T, B, M, groups, max_pages
+        self.weights_shared = weights_shared
         self.places, self.prefix = places, tuple(prefix)       # a place for every token; plans (ops.PrefixLayout) for shared pages
         o = 0
         self.off: Dict[str, Tuple[int, int]] = {}
@@ -89,7 +93,7 @@ class _Layout:
         self.size = max(o, 4)
 
     def key(self):
-        return (self.T, self.B, self.M, self.groups, self.max_pages, *(p.key() for p in self.prefix))
+        return (self.T, self.B, self.M, self.groups, self.max_pages, self.weights_shared, *(p.key() for p in self.prefix))
 
 
 class Engine:
@@ -211,7 +215,8 @@ class Engine:
         # every check that can refuse the step comes before this line: a refused step holds nothing
         cache.reserve([(s, c + q) for s, c, q in zip(slots, ctxs, qlens)])
         prefix = self._prefix_layouts(slots, ctxs) if max(qlens) == 1 else ()
-        lay = _Layout(T, B, len(rows), len(cache.groups), cache.max_pages_per_seq, firsts != ctxs and max(qlens) > 1, prefix)
+        lay = _Layout(T, B, len(rows), len(cache.groups), cache.max_pages_per_seq, firsts != ctxs and max(qlens) > 1, prefix,
+                      cache.weigh and B > 1 and any(g.more for g in cache.groups))
         buf = np.zeros(lay.size, dtype=np.int32)
 
         def put(name, values):
@@ -287,6 +292,7 @@ class Engine:
             o, n = lay.off[f"pages{g}"]
             ctx.pages.append(dev[o:o + n].view(lay.B, lay.max_pages))
         # (one token a sequence: its place is what the sequence held before; captured steps move that along themselves)
+        ctx.weights_shared = lay.weights_shared
         ctx.tok_place = ctx.seq_ctx if meta["is_decode"] else ctx.tok_pos
         if lay.places:
             o, n = lay.off["tok_place"]

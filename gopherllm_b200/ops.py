@@ -990,7 +990,7 @@ def prefix_plan(groups, batch: int, num_heads: int, num_kv_heads: int, head_dim:
 
 class _SpanArgs(Structure):
     _fields_ = [(n, c_void_p) for n in ("q", "out", "k_cache", "v_cache", "seq_row", "seq_qlen", "seq_ctx", "pages", "order", "items",
-                                        "seq_shared", "part_o", "part_ml", "scores", "weights")] + \
+                                        "seq_shared", "part_o", "part_ml", "scores", "weights", "given")] + \
                [(n, c_int) for n in ("B", "nH", "nKV", "max_pages", "n_pages", "n_items", "splits", "slots", "chunks", "reach", "short", "early", "held")]
 
 
@@ -1000,7 +1000,7 @@ class _SpanF32Args(Structure):
 
 class _RunArgs(Structure):
     _fields_ = [(n, c_void_p) for n in ("q", "k_cache", "seq_row", "seq_qlen", "seq_ctx", "pages", "ml", "weights", "sums")] + \
-               [(n, c_int) for n in ("B", "nH", "nKV", "max_pages", "n_pages", "reach", "last", "parts", "rows")]
+               [(n, c_int) for n in ("B", "nH", "nKV", "max_pages", "n_pages", "reach", "last", "parts", "rows", "shared")]
 
 
 class _RunF32Args(Structure):
@@ -1077,7 +1077,7 @@ def attention_prefix(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, 
     f32 = q.dtype is torch.float32
     a = (_SpanF32Args if f32 else _SpanArgs)(
         q.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), None, None, seq_ctx.data_ptr(), pages.data_ptr(),
-        base, base + 4 * lay.items_at, base + 4 * lay.shared_at, at, ml, None, None,
+        base, base + 4 * lay.items_at, base + 4 * lay.shared_at, at, ml, None, None, None,
         B, num_heads, num_kv_heads, pages.shape[1], k_cache.shape[0], lay.n_items, lay.splits, lay.slots, lay.chunks, 0, head_dim if f32 else lay.short)
     fn = _lib("attention_spans_f32.cu").gl_attention_prefix_f32 if f32 else _lib("attention_spans.cu", (f"GL_HEAD_DIM={head_dim}",)).gl_attention_prefix
     _check(_launch(fn, byref(a), c_int(lay.rows), c_int(lay.joined), _stream()), "attention_prefix", lay.launches)
@@ -1085,14 +1085,16 @@ def attention_prefix(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, 
 
 def attention_weighed(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, weights: torch.Tensor,
                       seq_qstart: torch.Tensor, seq_qlen: torch.Tensor, seq_ctx: torch.Tensor, pages: torch.Tensor, num_heads: int,
-                      num_kv_heads: int, head_dim: int, max_qlen: int, max_len: int, last: int = 0) -> None:
+                      num_kv_heads: int, head_dim: int, max_qlen: int, max_len: int, last: int = 0, shared: bool = False) -> None:
     """Causal attention of this step's runs of tokens over the cache (their own keys included), keeping the weight that every
     cached position has been given.  ``weights`` [pages, key/value heads, PAGE] float32 lies beside the cache under the same page
     ids; with p the softmax weights of query i and head h,
     weights[j] <- (weights[j] if j < seq_ctx[b] else 0) + sum of p[i, h, j] over the run's queries i and the query heads h
     of the key/value head: a position that is new in this step starts from nothing.  ``last`` n > 0: only a run's last n
     queries are counted.  Places behind a sequence's last position stay as they are, a sequence without tokens leaves everything
-    as it is.  ``max_qlen``, ``max_len``: the longest run, and the longest sequence after the step."""
+    as it is.  ``max_qlen``, ``max_len``: the longest run, and the longest sequence after the step.  ``shared``: sequences of the step
+    may have pages in common, at the same places of their tables and full before the step; a position there is given the sum
+    of theirs, in the sequences' order.  Without it no two of the step's sequences hold the same page."""
     B = _need_span("attention_weighed", q, out, k_cache, v_cache, seq_ctx, pages, num_heads, num_kv_heads, head_dim)
     here, n_pages, dtype = q.get_device(), k_cache.shape[0], q.dtype
     if not (isinstance(weights, torch.Tensor) and _fit(here, torch.float32, weights) and weights.shape == k_cache.shape[:3]
@@ -1110,7 +1112,10 @@ def attention_weighed(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor,
     lib = _lib("attention_spans_f32.cu") if f32 else _lib("attention_spans.cu", (f"GL_HEAD_DIM={head_dim}",))
     if max_qlen == 1:
         chunks, splits, joined = _weigh_shape(B, num_heads, num_kv_heads, head_dim, dtype, max_len, sm_count(q.device))
-        slots, at, ml, scores = 0, None, None, None
+        slots, at, ml, scores, given = 0, None, None, None, None
+        if shared:
+            each = empty((B, num_kv_heads, max_len), torch.float32, q.device)      # (held until the launch)
+            given = each.data_ptr()
         if not joined:
             slots, n = splits, B * num_heads * splits * head_dim
             part = empty((n + B * num_heads * (2 * splits + max_len),), torch.float32, q.device)
@@ -1119,9 +1124,9 @@ def attention_weighed(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor,
         a = (_SpanF32Args if f32 else _SpanArgs)(
             q.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), seq_qstart.data_ptr(), seq_qlen.data_ptr(),
             seq_ctx.data_ptr(), pages.data_ptr(), None, None, None, at, ml, scores,
-            weights.data_ptr(), B, num_heads, num_kv_heads, pages.shape[1], n_pages, 0, splits, slots, chunks, max_len, head_dim if f32 else 0)
+            weights.data_ptr(), given, B, num_heads, num_kv_heads, pages.shape[1], n_pages, 0, splits, slots, chunks, max_len, head_dim if f32 else 0)
         _check(_launch(lib.gl_attention_weighed_f32 if f32 else lib.gl_attention_weighed, byref(a), _stream()), "attention_weighed",
-               2 if slots else 1)
+               (2 if slots else 1) + (1 if shared else 0))
         return
     ml = empty((num_heads, q.shape[0], 2), torch.float32, q.device)
     group, counted = num_heads // num_kv_heads, min(last, max_qlen) if last else max_qlen
@@ -1141,15 +1146,15 @@ def attention_weighed(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor,
         keys, rows = (128, 128) if tensor else (64, 64 // group if group < 64 else 1)
         blocks = -(-max_len // keys) * num_kv_heads * B
         parts = max(1, min((2 if tensor else 6) * sm_count(q.device) // blocks, (group if tensor else 1) * -(-counted // rows)))
-        if parts > 1:
-            sums = empty((parts, B, num_kv_heads, max_len), torch.float32, q.device)
+    if parts > 1 or shared:
+        sums = empty((parts, B, num_kv_heads, max_len), torch.float32, q.device)
     fields = (q.data_ptr(), k_cache.data_ptr(), seq_qstart.data_ptr(), seq_qlen.data_ptr(), seq_ctx.data_ptr(), pages.data_ptr(),
-              ml.data_ptr(), weights.data_ptr(), _addr(sums), B, num_heads, num_kv_heads, pages.shape[1], n_pages, max_len, last, parts, q.shape[0])
+              ml.data_ptr(), weights.data_ptr(), _addr(sums), B, num_heads, num_kv_heads, pages.shape[1], n_pages, max_len, last, parts, q.shape[0], int(bool(shared)))
     if f32:
-        _check(_launch(lib.gl_attention_weigh_runs_f32, byref(_RunF32Args(*fields, head_dim)), c_int(max_qlen), _stream()), "attention_weighed", 3 if parts > 1 else 2)
+        _check(_launch(lib.gl_attention_weigh_runs_f32, byref(_RunF32Args(*fields, head_dim)), c_int(max_qlen), _stream()), "attention_weighed", 2 if sums is None else 3)
     else:
         _check(_launch(lib.gl_attention_weigh_runs, byref(_RunArgs(*fields)), c_int(max_qlen), c_int(q.shape[0]), c_int(tensor),
-                       c_int(sm_count(q.device) if tensor else 0), _stream()), "attention_weighed", 2 if not tensor or parts > 1 else 1)
+                       c_int(sm_count(q.device) if tensor else 0), _stream()), "attention_weighed", (1 if tensor else 2) + (0 if sums is None else 1))
 
 
 class _AttnStats(Structure):

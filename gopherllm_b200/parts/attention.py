@@ -182,7 +182,7 @@ class Attention(Mixer):
         if not alone:
             if cache.weights is not None:
                 ops.attention_weighed(q, o, cache.k, cache.v, cache.weights, ctx.seq_qstart, ctx.seq_qlen, ctx.seq_ctx, pages,
-                                      s.num_heads, s.num_kv_heads, s.head_dim, ctx.max_qlen, ctx.max_len)
+                                      s.num_heads, s.num_kv_heads, s.head_dim, ctx.max_qlen, ctx.max_len, shared=ctx.weights_shared)
             else:
                 ops.attention_prefix(q, o, cache.k, cache.v, ctx.seq_ctx, pages, prefix, s.num_heads, s.num_kv_heads, s.head_dim)
             if self.gate:

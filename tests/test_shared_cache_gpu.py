@@ -296,6 +296,41 @@ def test_a_forked_sequence_is_cut_onto_pages_of_its_own(load):
             assert err <= bound, (err, bound)
 
 
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_positions_of_forked_sequences_are_given_what_all_give(load, dtype):
+    """Two forks of one sequence, token by token (captured) and with a run, twice: the same weights to the last bit, and on
+    the common pages what each step gave from both: every step gives a layer's positions one for each token and query head."""
+    m = load("B", dtype, weigh=True)
+    V = tiny.TINY_B["vocab_size"]
+    rng = np.random.default_rng(12)
+    base, runs = tiny.prompt(rng, 128, V), [tiny.prompt(rng, 12, V) for _ in range(3)]
+
+    def run():
+        s = m.open_sequence()
+        m.step([(s, base)], [[]])
+        slots = [s, m.fork_sequence(s), m.fork_sequence(s)]
+        for i in range(8):
+            m.step(list(zip(slots, [[r[i]] for r in runs])))
+        m.step([(x, r[8:]) for x, r in zip(slots, runs)])
+        g = m.engine.cache.groups[0]
+        lists = [m.engine.cache._pages[x][0] for x in slots]
+        assert all(p[:2] == lists[0][:2] and p[2] != lists[0][2] for p in lists[1:])
+        got = torch.cat([g.weights[:, lists[0][:2]], *(g.weights[:, p[2:3]] for p in lists)], 1)      # [layers, 5 pages, heads, PAGE]
+        got[:, 2:, :, 12:] = 0.0                                   # (nothing is there)
+        for x in slots:
+            m.close_sequence(x)
+        return got
+
+    run()                                                          # (the first steps of the first time are not captured: they divide sequences otherwise)
+    one, two = run(), run()
+    assert torch.equal(one, two)
+    spec = m.engine.model.blocks[0].mixer.spec
+    total = one.double().sum((1, 2, 3))
+    want = (128 + 3 * 12) * spec.num_heads                         # every query and head gives one altogether
+    # each weight is off by a few 2^-20 of itself at most, a sum of fewer than 200 of them by that and 200 roundings of 2^-24
+    assert ((total - want).abs() <= want * (2 ** -14)).all(), total
+
+
 def test_generate_in_a_bounded_cache(load):
     """Six pages serve prompts of 100 tokens and 120 more each, two at a time, where 220 positions would take four pages a sequence;
     the tokens are those of stepping and cutting by hand."""

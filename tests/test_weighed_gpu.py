@@ -136,3 +136,45 @@ def test_refusals():
                  (7, ctx.cpu()), (8, table.t()), (9, 3), (10, 3), (11, 32), (12, -1), (13, 0), (13, 65), (14, -1), (4, sums.cpu())):
         with pytest.raises(ops.KernelError):
             ops.attention_weighed(*good[:i], x, *good[i + 1:])
+
+
+@pytest.mark.parametrize("dtype,H,G,D", [(BF, 4, 2, 64), (BF, 2, 2, 128), (BF, 40, 1, 32), (BF, 4, 2, 256), (F, 4, 4, 64), (F, 4, 1, 50), (F, 20, 2, 36)])
+@pytest.mark.parametrize("ctx,qlen,last", [([200, 150, 128, 190, 700], [1] * 5, 0), ([128, 131, 300, 192, 129], [1, 140, 0, 40, 3], 0), ([128, 131, 300, 192, 129], [1, 140, 70, 40, 3], 2),
+                                           ([5000, 5100], [1, 1], 0)])
+def test_sequences_on_common_pages(dtype, H, G, D, ctx, qlen, last):
+    """Every other sequence lies on the same first two pages: a position there is given what all of them give it, the same in every run."""
+    from gopherllm_b200 import ops
+    s = build(ctx, qlen, H, G, D, dtype, 7)
+    q, k, v, sums, start, qlens, ctxs, table = s
+    for b in range(2, len(ctx)):
+        table[b, :2] = table[b % 2, :2]
+    if len(ctx) == 2:
+        table[1, :2] = table[0, :2]
+    outs = []
+    for _ in range(3):
+        out, now = torch.full_like(q, float("nan")), sums.clone()
+        ops.attention_weighed(q, out, k, v, now, start, qlens, ctxs, table, H, G, D, max(qlen), max(c + n for c, n in zip(ctx, qlen)), last, shared=True)
+        outs.append((out, now))
+    assert all(torch.equal(x, outs[0][0]) and torch.equal(y.nan_to_num(-1.0), outs[0][1].nan_to_num(-1.0)) for x, y in outs)
+    out, now = outs[0]
+    given, terms, most = torch.zeros_like(sums, dtype=torch.float64), torch.zeros_like(sums, dtype=torch.float64), 0.0
+    had, touched = sums.double().clone(), torch.zeros_like(sums, dtype=torch.bool)
+    for b in range(len(ctx)):
+        if not qlen[b]:
+            continue
+        at, T, n = sum(qlen[:b]), qlen[b], ctx[b] + qlen[b]
+        want, p, A, S = plain.attention(q[at:at + T].double().view(T, H, D), plain.rows(k, table[b], n), plain.rows(v, table[b], n), ctx[b])
+        assert ((out[at:at + T].double().view(T, H, D) - want).abs() <= plain.out_bound(dtype, want, A, D, n, S)).all()
+        j = torch.arange(n, device="cuda")
+        page, slot = table[b].long()[j // PAGE], j % PAGE
+        p = p[-last:] if last else p
+        given[page, :, slot] += p.sum(0).view(G, H // G, n).sum(1).T
+        terms[page, :, slot] += p.shape[0] * H // G
+        new = j >= ctx[b]
+        had[page[new], :, slot[new]] = 0.0
+        touched[page, :, slot] = True
+        most = max(most, S)
+    off = (now.double() - had - given).abs()
+    assert (off <= plain.sums_bound(had, given, terms + len(ctx), D, most))[touched].all(), float(off[touched].max())
+    same = (now == sums) | (torch.isnan(now) & torch.isnan(sums))
+    assert (same | touched).all()
