@@ -1171,7 +1171,7 @@ def cache_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, weights: torch.Ten
     """Cuts sequences longer than ``keep`` positions down to that many, layer by layer and key/value head by head: the ``first``
     and the ``recent`` last positions stay and, of those between, the ones with the largest ``weights`` (equal ones: the lower
     position; a NaN counts as less than any number).  What stays moves, in order, to positions 0..keep - 1 of the
-    sequence's own pages, or with ``to_pages`` [B, n] of those (none of which any of ``pages`` may be; the sequence's own
+    sequence's own pages, or with ``to_pages`` [B, n] of those (each once, none of them among ``pages``; the sequence's own
     pages then stay as they are, and a sequence of up to ``keep`` positions is copied whole).  Keys, values
     [(layers,) pages, key/value heads, PAGE, head size] and weights [(layers,) pages, key/value heads, PAGE] move together;
     places behind the ones that are kept stay as they are.  ``seq_len`` [B]: positions cached.  In place no two sequences may share a page.
