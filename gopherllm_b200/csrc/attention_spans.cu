@@ -430,19 +430,27 @@ attn_span_kernel(SpanArgs a) {
     span_join(a, e, fin_o, fin_ml, held, ml_w, pg, SP_LOG2E);
 }
 
-// The spans of a sequence put together: blockIdx = (share of the positions, key/value head, sequence).  The blocks of a head share its
-// output out by query heads; with scores written down each turns the scores of its positions into weights, added up over the
-// query heads.  A position new in this step starts from nothing, whatever its place held.
+// The spans of a sequence put together: blockIdx = (x, key/value head, sequence).  The first ``shares`` blocks of a head turn the scores
+// of a thousand positions each into weights, added up over the query heads, four positions a thread so that their scores and
+// page numbers are under way together; a position new in this step starts from nothing, whatever its place held.  The G blocks
+// behind them put a query head's output together, the spans dealt out to as many threads a number as there are.
+// Latency bounds it: two reads that depend on one another, and a write.
 #define SP_JOIN_THREADS 256
+#define SP_JOIN_KEYS 4
+template <bool GIVEN>
 __global__ void __launch_bounds__(SP_JOIN_THREADS)
-attn_span_join_kernel(SpanArgs a) {
+attn_span_join_kernel(SpanArgs a, int shares) {
     extern __shared__ float ml_all[];                      // [G][2]: maximum, 1 / sum
+    constexpr int PER = SP_JOIN_THREADS / SP_HD > 0 ? SP_JOIN_THREADS / SP_HD : 1;          // threads that share a number of the output
+    __shared__ float sums[PER][SP_HD];
     const int b = blockIdx.z, g = blockIdx.y, G = a.nH / a.nKV, tid = threadIdx.x, lane = tid & 31;
     gl_grid_wait();
     gl_grid_launch_dependents();
     if (a.seq_qlen && a.seq_qlen[b] <= 0) return;
-    const int n = (a.seq_shared ? a.seq_shared[2 * b + 1] : 0) + a.splits;
-    for (int i = tid >> 5; i < G; i += SP_JOIN_THREADS / 32) {
+    const int n = (a.seq_shared ? a.seq_shared[2 * b + 1] : 0) + a.splits, own = (int)blockIdx.x - shares;
+    const int pos = a.seq_ctx[b], most = min(pos + 1, a.reach), j0 = (int)blockIdx.x * SP_JOIN_THREADS * SP_JOIN_KEYS + tid;
+    if (own < 0 && j0 - tid >= most) return;
+    for (int i = own < 0 ? tid >> 5 : own + (tid >> 5) * G; i < G; i += SP_JOIN_THREADS / 32) {      // (all heads, or the block's)
         const float* ml = a.part_ml + ((size_t)b * a.nH + g * G + i) * a.slots * 2;
         float m = -INFINITY, l = 0.f;
         for (int s = lane; s < n; s += 32) m = fmaxf(m, ml[2 * s]);
@@ -452,30 +460,51 @@ attn_span_join_kernel(SpanArgs a) {
         if (lane == 0) { ml_all[2 * i] = m; ml_all[2 * i + 1] = 1.0f / l; }
     }
     __syncthreads();
-    for (int i = blockIdx.x; i < G; i += gridDim.x) {
-        const size_t at = ((size_t)b * a.nH + g * G + i) * a.slots;
-        const float m = ml_all[2 * i], inv = ml_all[2 * i + 1];
-        for (int d = tid; d < SP_HD; d += SP_JOIN_THREADS) {
+    if (own >= 0) {
+        const size_t row = (size_t)b * a.nH + g * G + own, at = row * a.slots;
+        const float m = ml_all[2 * own], inv = ml_all[2 * own + 1];
+        if (tid < PER * SP_HD) {
+            const int d = tid % SP_HD, first = tid / SP_HD;
             float o = 0.f;
+#pragma unroll 8
+            for (int s = first; s < n; s += PER) o = fmaf(sp_factor(a.part_ml[(at + s) * 2], m), a.part_o[(at + s) * SP_HD + d], o);
+            sums[first][d] = o;
+        }
+        __syncthreads();
+        if (tid < SP_HD) {
+            float o = 0.f;
+#pragma unroll
+            for (int k = 0; k < PER; ++k) o += sums[k][tid];
+            a.out[((size_t)(a.seq_row ? a.seq_row[b] : b) * a.nH + g * G + own) * SP_HD + tid] = __float2bfloat16_rn(inv == INFINITY ? 0.f : o * inv);
+        }
+        return;
+    }
+    float given[SP_JOIN_KEYS];
+    int page[SP_JOIN_KEYS];
+#pragma unroll
+    for (int u = 0; u < SP_JOIN_KEYS; ++u) {
+        const int j = j0 + u * SP_JOIN_THREADS;
+        given[u] = 0.f;
+        page[u] = !GIVEN && j < most ? a.pages[(size_t)b * a.max_pages + j / GL_PAGE] : 0;
+    }
+    const float* sc = a.scores + ((size_t)b * a.nH + g * G) * a.reach + j0;
 #pragma unroll 4
-            for (int s = 0; s < n; ++s) o = fmaf(sp_factor(a.part_ml[(at + s) * 2], m), a.part_o[(at + s) * SP_HD + d], o);
-            a.out[((size_t)(a.seq_row ? a.seq_row[b] : b) * a.nH + g * G + i) * SP_HD + d] = __float2bfloat16_rn(inv == INFINITY ? 0.f : o * inv);
+    for (int i = 0; i < G; ++i) {
+        const float m = ml_all[2 * i], inv = ml_all[2 * i + 1];
+#pragma unroll
+        for (int u = 0; u < SP_JOIN_KEYS; ++u) {
+            const float x = j0 + u * SP_JOIN_THREADS < most ? sc[(size_t)i * a.reach + u * SP_JOIN_THREADS] : 0.f;
+            given[u] = fmaf(sp_exp2(fmaf(x, SP_LOG2E, -m)), inv, given[u]);
         }
     }
-    if (!a.weights) return;
-    const int pos = a.seq_ctx[b], most = min(pos + 1, a.reach);
-    for (int j = blockIdx.x * SP_JOIN_THREADS + tid; j < most; j += gridDim.x * SP_JOIN_THREADS) {
-        const float* sc = a.scores + ((size_t)b * a.nH + g * G) * a.reach + j;
-        float given = 0.f;
-#pragma unroll 4
-        for (int i = 0; i < G; ++i) given = fmaf(sp_exp2(fmaf(sc[(size_t)i * a.reach], SP_LOG2E, -ml_all[2 * i])), ml_all[2 * i + 1], given);
-        if (a.given) {
-            a.given[((size_t)b * a.nKV + g) * a.reach + j] = given;
-            continue;
-        }
-        float* w = a.weights + ((size_t)gl_checked(a.pages[(size_t)b * a.max_pages + j / GL_PAGE], a.n_pages, GL_BAD_PAGE) * a.nKV + g) * GL_PAGE + j % GL_PAGE;
-        if (j < pos) atomicAdd(w, given);                  // (one addition a position: no two sequences share it)
-        else *w = given;
+#pragma unroll
+    for (int u = 0; u < SP_JOIN_KEYS; ++u) {
+        const int j = j0 + u * SP_JOIN_THREADS;
+        if (j >= most) return;
+        float* w = GIVEN ? a.given + ((size_t)b * a.nKV + g) * a.reach + j
+                         : a.weights + ((size_t)gl_checked(page[u], a.n_pages, GL_BAD_PAGE) * a.nKV + g) * GL_PAGE + j % GL_PAGE;
+        if (!GIVEN && j < pos) atomicAdd(w, given[u]);     // (one addition a position: no two sequences share it)
+        else *w = given[u];
     }
 }
 
@@ -722,9 +751,10 @@ static int span_checked(const SpanArgs& a) {
 
 static int launch_join(const SpanArgs& a, cudaStream_t stream) {
     const int G = a.nH / a.nKV;
-    // with weights: a block for a thousand positions, one for each query head at least
-    const int shares = a.weights ? (a.reach + 4 * SP_JOIN_THREADS - 1) / (4 * SP_JOIN_THREADS) : 1;
-    return gl_launch(attn_span_join_kernel, dim3(shares > G ? shares : G, a.nKV, a.B), dim3(SP_JOIN_THREADS), 2 * G * sizeof(float), stream, 1, a);
+    const int shares = a.weights ? (a.reach + SP_JOIN_KEYS * SP_JOIN_THREADS - 1) / (SP_JOIN_KEYS * SP_JOIN_THREADS) : 0;
+    const dim3 grid(shares + G, a.nKV, a.B);
+    if (a.given) return gl_launch(attn_span_join_kernel<true>, grid, dim3(SP_JOIN_THREADS), 2 * G * sizeof(float), stream, 1, a, shares);
+    return gl_launch(attn_span_join_kernel<false>, grid, dim3(SP_JOIN_THREADS), 2 * G * sizeof(float), stream, 1, a, shares);
 }
 
 static int shared_tc(const SpanArgs& a, int rows, cudaStream_t stream);

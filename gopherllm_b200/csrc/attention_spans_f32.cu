@@ -250,17 +250,23 @@ span_f32_kernel(SpanF32Args a) {
     }
 }
 
-// The spans of a sequence put together, as in attention_spans.cu: blockIdx = (share of the positions, key/value head, sequence).
+// The spans of a sequence put together, as in attention_spans.cu: blockIdx = (x, key/value head, sequence), first the blocks of a thousand
+// positions each, then a block a query head for its output.
 #define SF_JOIN_THREADS 256
+#define SF_JOIN_KEYS 4
+template <bool GIVEN>
 __global__ void __launch_bounds__(SF_JOIN_THREADS)
-span_f32_join_kernel(SpanF32Args a) {
+span_f32_join_kernel(SpanF32Args a, int shares) {
     extern __shared__ __align__(16) float sf[];                    // [G][2]: maximum, sum
+    __shared__ float sums[SF_JOIN_THREADS];
     const int b = blockIdx.z, g = blockIdx.y, G = a.nH / a.nKV, tid = threadIdx.x, lane = tid & 31;
     gl_grid_wait();
     gl_grid_launch_dependents();
     if (a.seq_qlen && a.seq_qlen[b] <= 0) return;
-    const int n = (a.seq_shared ? a.seq_shared[2 * b + 1] : 0) + a.splits;
-    for (int i = tid >> 5; i < G; i += SF_JOIN_THREADS / 32) {
+    const int n = (a.seq_shared ? a.seq_shared[2 * b + 1] : 0) + a.splits, own = (int)blockIdx.x - shares;
+    const int pos = a.seq_ctx[b], most = min(pos + 1, a.reach), j0 = (int)blockIdx.x * SF_JOIN_THREADS * SF_JOIN_KEYS + tid;
+    if (own < 0 && j0 - tid >= most) return;
+    for (int i = own < 0 ? tid >> 5 : own + (tid >> 5) * G; i < G; i += SF_JOIN_THREADS / 32) {      // (all heads, or the block's)
         const float* ml = a.part_ml + ((size_t)b * a.nH + g * G + i) * a.slots * 2;
         float m = -INFINITY, l = 0.f;
         for (int s = lane; s < n; s += 32) m = fmaxf(m, ml[2 * s]);
@@ -270,30 +276,47 @@ span_f32_join_kernel(SpanF32Args a) {
         if (lane == 0) { sf[2 * i] = m; sf[2 * i + 1] = l; }
     }
     __syncthreads();
-    for (int i = blockIdx.x; i < G; i += gridDim.x) {
-        const size_t at = ((size_t)b * a.nH + g * G + i) * a.slots;
-        const float m = sf[2 * i], l = sf[2 * i + 1];
-        for (int d = tid; d < a.hd; d += SF_JOIN_THREADS) {
-            float o = 0.f;
-#pragma unroll 4
-            for (int s = 0; s < n; ++s) o = fmaf(sf_factor(a.part_ml[(at + s) * 2], m), a.part_o[(at + s) * a.hd + d], o);
-            a.out[((size_t)(a.seq_row ? a.seq_row[b] : b) * a.nH + g * G + i) * a.hd + d] = l == 0.f ? 0.f : o / l;
+    if (own >= 0) {
+        const size_t at = ((size_t)b * a.nH + g * G + own) * a.slots;
+        const float m = sf[2 * own], l = sf[2 * own + 1];
+        const int per = SF_JOIN_THREADS / a.hd, first = tid / a.hd, d = tid - first * a.hd;          // (heads of up to 256)
+        float o = 0.f;
+        if (first < per) {
+#pragma unroll 8
+            for (int s = first; s < n; s += per) o = fmaf(sf_factor(a.part_ml[(at + s) * 2], m), a.part_o[(at + s) * a.hd + d], o);
         }
+        sums[tid] = o;
+        __syncthreads();
+        if (tid < a.hd) {
+            for (int k = 1; k < per; ++k) o += sums[k * a.hd + tid];
+            a.out[((size_t)(a.seq_row ? a.seq_row[b] : b) * a.nH + g * G + own) * a.hd + tid] = l == 0.f ? 0.f : o / l;
+        }
+        return;
     }
-    if (!a.weights) return;
-    const int pos = a.seq_ctx[b], most = min(pos + 1, a.reach);
-    for (int j = blockIdx.x * SF_JOIN_THREADS + tid; j < most; j += gridDim.x * SF_JOIN_THREADS) {
-        const float* sc = a.scores + ((size_t)b * a.nH + g * G) * a.reach + j;
-        float given = 0.f;
+    float given[SF_JOIN_KEYS];
+    int page[SF_JOIN_KEYS];
+#pragma unroll
+    for (int u = 0; u < SF_JOIN_KEYS; ++u) {
+        const int j = j0 + u * SF_JOIN_THREADS;
+        given[u] = 0.f;
+        page[u] = !GIVEN && j < most ? a.pages[(size_t)b * a.max_pages + j / GL_PAGE] : 0;
+    }
+    const float* sc = a.scores + ((size_t)b * a.nH + g * G) * a.reach + j0;
 #pragma unroll 4
-        for (int i = 0; i < G; ++i) given += expf(sc[(size_t)i * a.reach] - sf[2 * i]) / sf[2 * i + 1];
-        if (a.given) {
-            a.given[((size_t)b * a.nKV + g) * a.reach + j] = given;
-            continue;
-        }
-        float* w = a.weights + ((size_t)gl_checked(a.pages[(size_t)b * a.max_pages + j / GL_PAGE], a.n_pages, GL_BAD_PAGE) * a.nKV + g) * GL_PAGE + j % GL_PAGE;
-        if (j < pos) atomicAdd(w, given);                          // (one addition a position: no two sequences share it)
-        else *w = given;
+    for (int i = 0; i < G; ++i) {
+        const float m = sf[2 * i], l = sf[2 * i + 1];
+#pragma unroll
+        for (int u = 0; u < SF_JOIN_KEYS; ++u)
+            if (j0 + u * SF_JOIN_THREADS < most) given[u] += expf(sc[(size_t)i * a.reach + u * SF_JOIN_THREADS] - m) / l;
+    }
+#pragma unroll
+    for (int u = 0; u < SF_JOIN_KEYS; ++u) {
+        const int j = j0 + u * SF_JOIN_THREADS;
+        if (j >= most) return;
+        float* w = GIVEN ? a.given + ((size_t)b * a.nKV + g) * a.reach + j
+                         : a.weights + ((size_t)gl_checked(page[u], a.n_pages, GL_BAD_PAGE) * a.nKV + g) * GL_PAGE + j % GL_PAGE;
+        if (!GIVEN && j < pos) atomicAdd(w, given[u]);             // (one addition a position: no two sequences share it)
+        else *w = given[u];
     }
 }
 
@@ -830,8 +853,10 @@ static int f32_spans_checked(const SpanF32Args& a) {
     return (a.chunks - 1) * ((G + a.chunks - 1) / a.chunks) >= G ? GL_ERR_SHAPE : GL_OK;
 }
 static int launch_join(const SpanF32Args& a, cudaStream_t stream) {
-    const int G = a.nH / a.nKV, shares = a.weights ? (a.reach + 4 * SF_JOIN_THREADS - 1) / (4 * SF_JOIN_THREADS) : 1;
-    return gl_launch(span_f32_join_kernel, dim3(shares > G ? shares : G, a.nKV, a.B), dim3(SF_JOIN_THREADS), 2 * G * sizeof(float), stream, 1, a);
+    const int G = a.nH / a.nKV, shares = a.weights ? (a.reach + SF_JOIN_KEYS * SF_JOIN_THREADS - 1) / (SF_JOIN_KEYS * SF_JOIN_THREADS) : 0;
+    const dim3 grid(shares + G, a.nKV, a.B);
+    if (a.given) return gl_launch(span_f32_join_kernel<true>, grid, dim3(SF_JOIN_THREADS), 2 * G * sizeof(float), stream, 1, a, shares);
+    return gl_launch(span_f32_join_kernel<false>, grid, dim3(SF_JOIN_THREADS), 2 * G * sizeof(float), stream, 1, a, shares);
 }
 
 // rows, joined: as for gl_attention_prefix (joined: heads of whole 16-byte pieces only)
