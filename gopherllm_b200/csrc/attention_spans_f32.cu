@@ -325,7 +325,8 @@ span_f32_join_kernel(SpanF32Args a, int shares) {
 // so a warp takes four at a time and has 2 UN of their pieces' rows under way; no barrier stands between two keys.  With R rows
 // the eight lanes' shares of R products are added up and dealt out in one exchange, so that a lane ends with the whole score of
 // row ``lane mod R`` and takes its power alone.  Each of a warp's four groups of lanes has a softmax of its own; they meet at the end of
-// the span, then the warps, then the blocks of a cluster (as in attention_spans.cu).
+// the span, then the warps, then the blocks of a cluster (as in attention_spans.cu).  Bound by latency at the sizes that 32 bits serve:
+// twelve sequences on two texts of 1,024 tokens, 32 heads of 64, 19 us; four of 50 to 700 positions with weights, 11 us.
 // ---------------------------------------------------------------------------
 #define ST_WARPS 4
 // loads that stay behind the wait before them (what another kernel wrote meanwhile)

@@ -12,7 +12,9 @@
 // Moving: a row is its key's and its value's pieces of 16 bytes side by side.  What stays at place i came from place kept[i] >= i,
 // and kept grows, so in place a block walks forward: the places it has written lie before everything it has still to read.  The
 // blocks of a cluster share out the columns of all rows, so no two touch the same bytes, and begin when all have selected; rows
-// that stay where they are are not touched.  Into other pages they share out the rows.  Memory bounds it.
+// that stay where they are are not touched.  Into other pages they share out the rows.  Memory bounds it where heads are many (24 layers
+// of four sequences, 32 heads of 64: 295 us, 5.6 TB/s); of two sequences of 32,700 positions and four layers of 8 heads of 128 (72 us, 43 for the
+// bytes) the first 25 us go to the three rounds of counting, before which nothing can move.
 #include "common.cuh"
 #include <cooperative_groups.h>
 namespace cg = cooperative_groups;
