@@ -819,9 +819,9 @@ GL_API int gl_attention_weighed(const SpanArgs* args, cudaStream_t stream) {
 // them).  Four warps a tile own a row a thread: no shuffles for the sum, and a maximum only where a page needs one.  All
 // pages are seen whole, so there is no mask but for a caller whose sequences end inside.
 // Bound by the issue of the products (12 a page of 64 keys at a head size of 128) beside the powers, and by memory where one tile holds
-// all rows.  32 heads of 128 on 8: 128 sequences on one document of 16,384 tokens, 48 us, 0.72 PFLOP/s, a page of two tiles some 1,980 clocks, of
+// all rows.  32 heads of 128 on 8: 128 sequences on one document of 16,384 tokens, 46 us, 0.75 PFLOP/s, a page of two tiles some 1,850 clocks, of
 // which the powers need 1,024; 64 sequences on four texts of 8,192, 24 us.  Scores of two pages at once (N 128) leave no room in tensor
-// memory for a second buffer and took 61 us in all against 55.  Waits are bounded; a block whose wait runs out records it, frees its tensor memory and returns.
+// memory for a second buffer and took 6 us more in all.  Waits are bounded; a block whose wait runs out records it, frees its tensor memory and returns.
 // ---------------------------------------------------------------------------
 #if SP_HD <= 128
 #define ST_BM 128
@@ -855,6 +855,13 @@ __host__ __device__ constexpr int st_stages(int nt) {
 }
 static_assert(st_stages(2) >= 3 && st_stages(1) >= 3, "shared memory holds too few pages");
 struct StMaps { CUtensorMap k[4], v; };
+
+// the one lane of a whole warp that issues: the same one every time
+__device__ __forceinline__ bool elect_one() {
+    unsigned p;
+    asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.b32 %0, 1, 0, p;\n}" : "=r"(p));
+    return p != 0;
+}
 
 template <int NT>
 __global__ void __launch_bounds__(ST_THREADS(NT), 1)
@@ -919,13 +926,16 @@ shared_tc_kernel(SpanArgs a, const __grid_constant__ StMaps maps) {
             }
         }
     } else if (warp > PRODUCER) {
-        if (lane == 0) {
-            constexpr uint32_t idesc_s = umma_idesc_bf16(GL_PAGE, 0);
-            constexpr uint32_t idesc_o = umma_idesc_bf16(SP_HD, 1);
-            const int t = warp - PRODUCER - 1, nt = t < tiles ? n : 0;
-            auto issue_scores = [&](int j) {
-                const int st = j % STAGES;
-                bool begin = true;
+        // (the whole warp goes through the waits and addresses, which are the same for all its lanes, and one lane issues: where one lane
+        // went through all of it alone, 128 sequences on a document of 16,384 tokens took 55 us against 52)
+        constexpr uint32_t idesc_s = umma_idesc_bf16(GL_PAGE, 0);
+        constexpr uint32_t idesc_o = umma_idesc_bf16(SP_HD, 1);
+        const int t = warp - PRODUCER - 1, nt = t < tiles ? n : 0;
+        auto wait = [](unsigned bar, unsigned parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)) != 0; };
+        auto issue_scores = [&](int j) {
+            const int st = j % STAGES;
+            bool begin = true;
+            if (elect_one()) {
 #pragma unroll
                 for (int s = 0; s < ST_NSEG; ++s) {
                     const int rb = st_seg(s).width * 2;
@@ -938,43 +948,48 @@ shared_tc_kernel(SpanArgs a, const __grid_constant__ StMaps maps) {
                     }
                 }
                 umma_commit(ST_SF(t, j & 1));
-            };
-            // What this thread does a page is what the kernel waits for, and a wait costs it some 250 clocks even where there is nothing to wait
-            // for, a commit 40: so a page's keys and values arrive together (that page's wait was made before its scores), go back
-            // together behind the second product, and the products done are announced by the scores behind them (a commit
-            // speaks for all that its thread issued before) but for the last product that has none.
-            bool ok = nt == 0 || mbar_wait(ST_QF(t), 0);
-            for (int j = 0; ok && j < 2 && j < nt; ++j) {
-                ok = mbar_wait(bar_f + 8 * (j % STAGES), (j / STAGES) & 1);
-                if (ok) { tc_fence_after(); issue_scores(j); }
             }
-            for (int j = 0; ok && j < nt; ++j) {
-                const int st = j % STAGES;
-                ok = mbar_wait(ST_PF(t, j & 1), (j >> 1) & 1);
-                if (!ok) break;
-                tc_fence_after();
-                const uint64_t dv = umma_smem_desc(sV + st * ST_V_BYTES, ST_VATOM_BYTES, 1024, 2);
+            __syncwarp();
+        };
+        // What this thread does a page is what the kernel waits for, and a wait costs it some 250 clocks even where there is nothing to wait
+        // for, a commit 40: so a page's keys and values arrive together (that page's wait was made before its scores), go back
+        // together behind the second product, and the products done are announced by the scores behind them (a commit
+        // speaks for all that its thread issued before) but for the last product that has none.
+        bool ok = nt == 0 || wait(ST_QF(t), 0);
+        for (int j = 0; ok && j < 2 && j < nt; ++j) {
+            ok = wait(bar_f + 8 * (j % STAGES), (j / STAGES) & 1);
+            if (ok) { tc_fence_after(); issue_scores(j); }
+        }
+        for (int j = 0; ok && j < nt; ++j) {
+            const int st = j % STAGES;
+            if (NT > 1 && j + 2 < nt) ok = wait(bar_f + 8 * ((j + 2) % STAGES), ((j + 2) / STAGES) & 1);
+            ok = ok && wait(ST_PF(t, j & 1), (j >> 1) & 1);
+            if (!ok) break;
+            tc_fence_after();
+            const uint64_t dv = umma_smem_desc(sV + st * ST_V_BYTES, ST_VATOM_BYTES, 1024, 2);
+            if (elect_one()) {
 #pragma unroll
                 for (int k = 0; k < GL_PAGE / 16; ++k)
                     umma_bf16_tmem_a(tmem + 256 * t + 128, tmem + 256 * t + 64 * (j & 1) + 8 * k, dv + (uint64_t)((16 * 128) >> 4) * k, idesc_o, (j | k) ? 1u : 0u);
                 umma_commit(bar_e + 8 * st);
                 if (j == nt - 2) umma_commit(ST_PD(t));
                 if (j == nt - 1) umma_commit(ST_OF(t));
-                if (j + 2 < nt) {                          // over S_j and P_j, which the rows and the product above are done with
-                    ok = mbar_wait(bar_f + 8 * ((j + 2) % STAGES), ((j + 2) / STAGES) & 1);
-                    if (!ok) break;
-                    tc_fence_after();
-                    issue_scores(j + 2);
-                }
             }
-            // a tile without rows still hands every page back, once it has been loaded
-            for (int j = nt; ok && j < n && !failed; ++j) {
-                const int st = j % STAGES;
-                ok = mbar_wait(bar_f + 8 * st, (j / STAGES) & 1);
-                if (ok) mbar_arrive(bar_e + 8 * st);
+            __syncwarp();
+            if (j + 2 < nt) {                          // over S_j and P_j, which the rows and the product above are done with
+                if (NT == 1) ok = wait(bar_f + 8 * ((j + 2) % STAGES), ((j + 2) / STAGES) & 1);
+                if (!ok) break;
+                tc_fence_after();
+                issue_scores(j + 2);
             }
-            if (!ok) failed = 1;
         }
+        // a tile without rows still hands every page back, once it has been loaded
+        for (int j = nt; ok && j < n && !__any_sync(0xffffffffu, failed); ++j) {
+            const int st = j % STAGES;
+            ok = wait(bar_f + 8 * st, (j / STAGES) & 1);
+            if (ok && lane == 0) mbar_arrive(bar_e + 8 * st);
+        }
+        if (!ok) failed = 1;
     } else if ((warp >> 2) < tiles) {
         const int t = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane, row = t * ST_BM + r;
         const bool real = row < rows_all;
