@@ -382,3 +382,23 @@ def test_refusals(load):
     import vopedra_models
     with pytest.raises(ValueError, match="weigh=True"):
         gl.load_random(dict(vopedra_models.ALPHA), weigh=True, max_tokens=256)
+
+
+def test_a_cut_that_fails_holds_no_pages(load, monkeypatch):
+    from gopherllm_b200 import ops
+    m = load("B", "float32", weigh=True)
+    s = m.open_sequence()
+    m.step([(s, list(range(1, 131)))], [[]])
+    f = m.fork_sequence(s)
+    cache = m.engine.cache
+    free, length = cache.groups[0].pool.free_count, cache.length(f)
+
+    def refuse(*_):
+        raise ops.KernelError("no")
+    monkeypatch.setattr(ops, "cache_evict", refuse)
+    with pytest.raises(ops.KernelError):
+        m.evict([f], 40)
+    cache.check()
+    assert cache.groups[0].pool.free_count == free and cache.length(f) == length
+    m.close_sequence(s)
+    m.close_sequence(f)
