@@ -216,6 +216,7 @@ evict_kernel(EvictArgs a, int listed, int held) {
             if (i < n && listed) list[i] = i;
         }
         if (same) return;
+        if (SHARED && !listed) cg::this_cluster().sync();          // (the list is the output, which the first block has just written)
     } else {
         ev_select<T>(a, n, keys, SHARED ? kept : list, hists, warp_sum, warp_eq, found, rank, C, [&](int j) { return a.weights + place(pg, j); });
         if (SHARED) {

@@ -100,6 +100,23 @@ def test_long_sequences(lengths, keep):
         check(s, keep, keep // 4, 4, in_place)
 
 
+@pytest.mark.parametrize("lengths,keep", [([4500], 4544), ([5000, 0, 4999, 70], 6000), ([52000, 300, 51300], 51300)])
+@pytest.mark.parametrize("G", [1, 2])
+def test_short_sequences_of_long_tables_are_copied_whole(lengths, keep, G):
+    """Tables beyond 4,096 positions and a list of what stays that shared memory does not hold: several blocks copy a head's rows, and each
+    must know all of them.  Ten times, as what another block has not written yet shows only now and then."""
+    s = build(lengths, G, 16, BF, 1, -(-min(keep, max(lengths)) // PAGE), 7)
+    k, v, sums, length, pages, to = s
+    assert pages.shape[1] * PAGE > 4096 and (keep >= pages.shape[1] * PAGE or 4 * keep > 200 * 1024)
+    from gopherllm_b200 import ops
+    want = expected(k, v, sums, length, pages, to, keep, 5, 3)
+    for _ in range(10):
+        got = [t.clone() for t in (k, v, sums)]
+        kept = ops.cache_evict(*got, length, pages, keep, recent=5, first=3, to_pages=to)
+        assert torch.equal(kept.cpu(), want[0])
+        assert all(same(a, b) for a, b in zip(got, want[1:]))
+
+
 def test_rows_beside_one_another_do_not_matter_and_captured_it_runs_again():
     from gopherllm_b200 import ops
     k, v, sums, length, pages, to = build([300, 250, 400], 2, 32, BF, 2, 2, 5)
