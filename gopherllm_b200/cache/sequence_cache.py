@@ -175,22 +175,28 @@ class SequenceCache:
         return slot
 
     def state_snapshot(self, slots: Sequence[int]) -> List[torch.Tensor]:
-        """Copies of these sequences' rows of every state tensor (the reference saves and restores
-        such state around work that must leave no trace, qwen35.go:306-322)."""
-        states = [s for s in self._states if s is not None]
-        if not states:
-            return []
-        idx = torch.tensor([int(s) for s in slots], dtype=torch.int64).to(self.device)
-        return [s.index_select(0, idx) for s in states]
+        """Copies of what a step of these sequences changes other than by writing it anew: their rows of every state
+        tensor (the reference saves and restores such state around work that must leave no trace,
+        qwen35.go:306-322) and, in a cache that is weighed, the weights of all positions on their pages."""
+        return [t.index_select(dim, idx) for t, dim, idx in self._changed_by(slots)]
 
     def state_restore(self, slots: Sequence[int], rows: Sequence[torch.Tensor]) -> None:
-        """Put back what ``state_snapshot`` took for the same sequences."""
+        """Put back what ``state_snapshot`` took for the same sequences, which hold the same pages."""
+        for (t, dim, idx), r in zip(self._changed_by(slots), rows):
+            t.index_copy_(dim, idx, r)
+
+    def _changed_by(self, slots: Sequence[int]) -> List[Tuple[torch.Tensor, int, torch.Tensor]]:
+        """(tensor, dimension, indices) of the rows that a step of these sequences adds to."""
+        out = []
         states = [s for s in self._states if s is not None]
-        if not states:
-            return
-        idx = torch.tensor([int(s) for s in slots], dtype=torch.int64).to(self.device)
-        for s, r in zip(states, rows):
-            s.index_copy_(0, idx, r)
+        if states:
+            idx = torch.tensor([int(s) for s in slots], dtype=torch.int64).to(self.device)
+            out += [(s, 0, idx) for s in states]
+        for g in self.groups:
+            if g.weights is not None:
+                pages = sorted({p for s in slots for p in self._pages[s][g.gid] if p != RELEASED})
+                out.append((g.weights, 1, torch.tensor(pages, dtype=torch.int64).to(self.device)))
+        return out
 
     def length(self, slot: int) -> int:
         self._held(slot)

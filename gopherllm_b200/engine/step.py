@@ -515,8 +515,9 @@ class Engine:
             # Once kernel by kernel, which loads and warms everything, with a context of its own: what
             # the parts memoise per step (position tables) must be computed again inside the capture,
             # or the graph would go on reading the warm-up step's tables at every position.  The
-            # warm-up leaves no trace: the sampler's state and the sequences' state rows are put back,
-            # and the keys and values it wrote are written again, equal, by the first replay.
+            # warm-up leaves no trace: the sampler's state, the sequences' state rows and what the warm-up
+            # added to weighed positions are put back, and the keys and values it wrote are written
+            # again, equal, by the first replay.
             saved = [t.clone() for t in (sampler.rng, sampler.recent, sampler.recent_n)]
             states = cache.state_snapshot(slots)
             body(self.context(lay, g.desc, g.bound))

@@ -107,6 +107,69 @@ def test_decode_loop_on_shared_pages(load):
     assert run(True) == run(False)
 
 
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("shared", [False, True])
+def test_decode_loop_weighs_every_token_once(load, dtype, shared):
+    """A loop's first call of a shape, which warms up before it is captured, and a second: every query head gives a layer's positions one for
+    each token fed, whether sequences share pages or not; and the same sums as one token at a time."""
+    from gopherllm_b200.sampling.sampler import DeviceSampler, SamplerConfig
+    m = load("B", dtype, weigh=True)
+    rng = np.random.default_rng(21)
+    V = tiny.TINY_B["vocab_size"]
+    base = tiny.prompt(rng, 128, V)
+    g, cache = m.engine.cache.groups[0], m.engine.cache
+    heads = m.engine.model.blocks[0].mixer.spec.num_heads
+    cfg = SamplerConfig(temperature=0.0, top_k=0, top_p=1.0, repeat_penalty=1.0)
+
+    def begin():
+        slots = [m.open_sequence()]
+        m.step([(slots[0], base)], [[]])
+        for _ in range(2):
+            if shared:
+                slots.append(m.fork_sequence(slots[0]))
+            else:
+                slots.append(m.open_sequence())
+                m.step([(slots[-1], base)], [[]])
+        return slots
+
+    def sums(slots):
+        """Weights on the pages held, each page once, places without a position left out: [pages, layers, heads, PAGE]."""
+        out, seen = [], set()
+        for s in slots:
+            for i, p in enumerate(cache._pages[s][0]):
+                n = min(64, cache.length(s) - 64 * i)
+                if p not in seen and n > 0:
+                    seen.add(p)
+                    page = g.weights[:, p].double().clone()
+                    page[:, :, n:] = 0.0
+                    out.append(page)
+        return torch.stack(out)
+
+    prompts = 128 if shared else 3 * 128
+    slots = begin()
+    sampler = DeviceSampler(cfg, [1, 2, 3], [base] * 3, V, m.engine.device)
+    fed, tokens = 0, [5, 6, 7]
+    text = [[], [], []]
+    for steps in (4, 3):
+        chosen = m.engine.decode_loop(slots, tokens, steps, sampler).cpu().tolist()
+        for t, x, column in zip(text, tokens, zip(*chosen)):
+            t += [x, *column[:-1]]
+        tokens = chosen[-1]
+        fed += steps
+        got = sums(slots)
+        want = (prompts + 3 * fed) * heads
+        # a weight is off by a few 2^-20 of itself at most, a position's sum of fewer than 500 of them by as many roundings of 2^-24
+        assert ((got.sum((0, 2, 3)) - want).abs() <= want * 2 ** -14).all(), (steps, got.sum((0, 2, 3)), want)
+    for s in slots:
+        m.close_sequence(s)
+    slots = begin()
+    for i in range(fed):
+        m.step([(s, [t[i]]) for s, t in zip(slots, text)], [[]] * 3)
+    err, bound = tiny.close(got.cpu().numpy(), sums(slots).cpu().numpy(), dtype)
+    assert err <= bound, (err, bound)
+    cache.check()
+
+
 def test_heads_with_a_gate_and_values_that_are_keys(load):
     """The mixer that has both, without a window, on shared pages and in a cache that is weighed: as without either."""
     import gopherllm_b200 as gl
