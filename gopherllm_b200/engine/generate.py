@@ -242,7 +242,9 @@ def generate(engine, prompts: Sequence[Sequence[int]], options: GenerationOption
                 # sampler's output and starts that step at once, before the host has seen the tokens, so
                 # the device does not wait for the host between steps; should a sequence then end with
                 # a stop token, the step has merely fed one token too many to a sequence that is closed,
-                # and the rows of the others stand (a row does not depend on its neighbours).
+                # and the rows of the others stand (a row does not depend on its neighbours).  Where sequences are
+                # cut by the weight of their positions and share pages, that token would leave its weights on
+                # pages that others are cut by: with a stop token about, such a step waits for the tokens.
                 ahead, ahead_logits, sampled = None, None, None
                 # (a sequence that has grown a page beyond what it may keep is cut before its next step)
                 due = options.cache_keep and [slots[r] for r in live if cache.length(slots[r]) >= options.cache_keep + PAGE]
@@ -250,7 +252,8 @@ def generate(engine, prompts: Sequence[Sequence[int]], options: GenerationOption
                     engine.evict(due, options.cache_keep, options.cache_recent, options.cache_first)
                 if prepare is not None and all(states[r].may_continue() for r in live):
                     ahead = prepare([slots[r] for r in live])
-                    if fetch is not None:
+                    waits = options.cache_keep and options.stop_tokens and any(cache.shares_pages(slots[r]) for r in live)
+                    if fetch is not None and not waits:
                         sampled = torch.cuda.Event()
                         sampled.record()
                         ahead_logits = engine.finish_decode(ahead, chosen)

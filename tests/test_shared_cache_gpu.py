@@ -423,6 +423,60 @@ def test_generate_in_a_bounded_cache(load):
     m.engine.cache.check()
 
 
+def test_a_stop_token_leaves_no_weights_on_shared_pages(load):
+    """Three sequences on two common pages, of which one ends with a stop token before the first cut: the token that ends it is never fed,
+    so the others are cut by the weights, and say the tokens, of stepping and cutting by hand."""
+    from gopherllm_b200.sampling.sampler import DeviceSampler, SamplerConfig
+    m = load("B", "float32", weigh=True)
+    V = tiny.TINY_B["vocab_size"]
+    rng = np.random.default_rng(30)
+    base = tiny.prompt(rng, 128, V)
+    prompts = [base + tiny.prompt(rng, n, V) for n in (3, 2, 5)]
+    cut = dict(cache_keep=100, cache_recent=20, cache_first=2)
+    sampling = dict(temperature=0.0, top_k=0, top_p=1.0, repeat_penalty=1.5)
+    cache, g = m.engine.cache, m.engine.cache.groups[0]
+    evict, masses = m.engine.evict, []
+
+    def watched(slots, *a):
+        pages = sorted({p for s in cache.live_slots() for p in cache._pages[s][0][:2]})          # whole pages of all that goes on
+        masses.append(g.weights[:, pages].double().sum((1, 2, 3)).cpu())
+        evict(slots, *a)
+    m.engine.evict = watched
+    free = [r.tokens for r in m.generate(prompts, share_prefix=True, max_tokens=60, stop_tokens=(), **cut, **sampling)]
+    ends = next((r, t) for r in range(3) for i, t in enumerate(free[r][:25]) if i >= 3 and t not in free[r][:i]
+                and not any(t in o for k, o in enumerate(free) if k != r))
+    masses.clear()
+    got = m.generate(prompts, share_prefix=True, max_tokens=60, stop_tokens=(ends[1],), **cut, **sampling)
+    assert got[ends[0]].finish_reason == "stop" and [r.finish_reason for r in got].count("length") == 2
+    said, masses = masses[0], []
+    # by hand, as stepped; the stop token ends its sequence before anything else is done
+    slots = [m.open_sequence()]
+    m.step([(slots[0], base)], [[]])
+    slots += [m.fork_sequence(slots[0]) for _ in prompts[1:]]
+    logits = m.step([(s, p[128:]) for s, p in zip(slots, prompts)])
+    sampler = DeviceSampler(SamplerConfig(**sampling), [1, 2, 3], prompts, V, m.engine.device)
+    live, tokens = [0, 1, 2], [[], [], []]
+    while live:
+        chosen = sampler.sample(logits, torch.tensor(live, dtype=torch.int32, device=m.engine.device)).tolist()
+        for r, t in zip(list(live), chosen):
+            if t == ends[1] or len(tokens[r]) == 59:
+                if t != ends[1]:
+                    tokens[r].append(t)
+                m.close_sequence(slots[r])
+                live.remove(r)
+            else:
+                tokens[r].append(t)
+        due = [slots[r] for r in live if cache.length(slots[r]) >= 164]
+        if due:
+            watched(due, 100, 20, 2)
+        if live:
+            logits = m.step([(slots[r], [tokens[r][-1]]) for r in live])
+    # (weights are off by a few 2^-20 of themselves and a sum's roundings; one token too many is 4 heads' worth among some 900)
+    assert ((said - masses[0]).abs() <= masses[0] * 2 ** -14).all(), (said, masses[0])
+    assert [r.tokens for r in got] == tokens
+    cache.check()
+
+
 def test_refusals(load):
     import gopherllm_b200 as gl
     m = load("A", "bfloat16")
