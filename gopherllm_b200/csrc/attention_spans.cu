@@ -749,7 +749,7 @@ static int span_checked(const SpanArgs& a) {
     const int G = a.nH / a.nKV;
     if (a.chunks < 1 || a.chunks > G || (long long)a.nKV * a.chunks > 65535 || (G + a.chunks - 1) / a.chunks > 8 * SP_MAX_NT) return GL_ERR_SHAPE;
     if ((a.chunks - 1) * ((G + a.chunks - 1) / a.chunks) >= G) return GL_ERR_SHAPE;        // every share of the heads has one
-    if (((uintptr_t)a.q | (uintptr_t)a.k_cache | (uintptr_t)a.v_cache) & 15) return GL_ERR_ALIGN;
+    if (((uintptr_t)a.q | (uintptr_t)a.k_cache | (uintptr_t)a.v_cache) & 15 || (uintptr_t)a.out & 7) return GL_ERR_ALIGN;      // (results leave in pieces of 8 bytes)
     return a.slots > 0 && (!a.part_o || !a.part_ml) ? GL_ERR_SHAPE : GL_OK;
 }
 

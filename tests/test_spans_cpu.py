@@ -113,3 +113,20 @@ def test_no_launch_behind_a_refusal(monkeypatch):
         with pytest.raises(ops.KernelError):
             ops.attention_prefix(*good[:i], x, *good[i + 1:])
     assert len(launched) == 2
+
+
+ALIGN = -3                                                         # GL_ERR_ALIGN (csrc/common.cuh)
+
+
+@pytest.mark.parametrize("name,off", [("out", 2), ("out", 4), ("q", 2), ("q", 8), ("k_cache", 2), ("v_cache", 4)])
+def test_tensors_at_odd_places_are_refused_by_the_launchers(name, off):
+    """A contiguous view into a larger buffer may begin anywhere; the kernels read and write in wider pieces.  The launchers look at addresses
+    before they do anything else, so no device is needed (and none is reached: every call here is refused)."""
+    lib = ops._lib("attention_spans.cu", ("GL_HEAD_DIM=64",))
+    at = dict(q=1 << 20, out=2 << 20, k_cache=3 << 20, v_cache=4 << 20)
+    at[name] += off
+    sizes = dict(B=2, nH=4, nKV=2, max_pages=3, n_pages=6, splits=1, chunks=1, reach=100)
+    one = ops._SpanArgs(**at, **sizes, seq_row=5 << 20, seq_qlen=5 << 20, seq_ctx=5 << 20, pages=5 << 20, weights=6 << 20)
+    assert lib.gl_attention_weighed(ops.byref(one), None) == ALIGN
+    two = ops._SpanArgs(**at, **sizes, seq_ctx=5 << 20, pages=5 << 20, seq_shared=5 << 20)
+    assert lib.gl_attention_prefix(ops.byref(two), ops.c_int(8), ops.c_int(1), None) == ALIGN
