@@ -255,6 +255,7 @@ GL_API int gl_attention_prefill(const AttnArgs* args, cudaStream_t stream) {
     if (a.B <= 0 || a.max_qlen <= 0) return GL_OK;
     if (a.hd != AP_HD || a.nH <= 0 || a.nKV <= 0 || a.nH % a.nKV) return GL_ERR_SHAPE;
     if (a.B > 65535 || a.nH > 65535 || a.score_scale != 1.0f) return GL_ERR_SHAPE;
+    if (((uintptr_t)a.q | (uintptr_t)a.k_cache | (uintptr_t)a.v_cache) & 15 || (uintptr_t)a.out & 3) return GL_ERR_ALIGN;
     const size_t smem = 5 * (size_t)AP_TILE;
     static bool configured = false;
     if (!configured) {

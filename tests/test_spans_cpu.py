@@ -130,3 +130,13 @@ def test_tensors_at_odd_places_are_refused_by_the_launchers(name, off):
     assert lib.gl_attention_weighed(ops.byref(one), None) == ALIGN
     two = ops._SpanArgs(**at, **sizes, seq_ctx=5 << 20, pages=5 << 20, seq_shared=5 << 20)
     assert lib.gl_attention_prefix(ops.byref(two), ops.c_int(8), ops.c_int(1), None) == ALIGN
+
+
+@pytest.mark.parametrize("name,off", [("out", 2), ("q", 2), ("q", 8), ("k_cache", 2), ("v_cache", 4)])
+def test_the_attention_behind_weighed_runs_of_wide_heads_refuses_odd_places(name, off):
+    """Runs of several tokens with heads above 128 reach this launcher before any of attention over spans."""
+    lib = ops._lib("attention_prefill.cu", ("GL_HEAD_DIM=256",))
+    at = dict(q=1 << 20, out=2 << 20, k_cache=3 << 20, v_cache=4 << 20)
+    at[name] += off
+    a = ops._AttnArgs(**at, seq_qstart=5 << 20, seq_qlen=5 << 20, seq_ctx=5 << 20, pages=5 << 20, B=1, nH=4, nKV=2, hd=256, max_pages=3, max_qlen=5, score_scale=1.0)
+    assert lib.gl_attention_prefill(ops.byref(a), None) == ALIGN
