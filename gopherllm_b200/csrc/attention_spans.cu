@@ -1435,10 +1435,10 @@ run_weigh_tc_kernel(RunArgs a, int n_items, const __grid_constant__ RtMaps maps)
     const int G = a.nH / a.nKV;
     auto item_of = [&](int round) { return round * (int)gridDim.x + (round & 1 ? (int)gridDim.x - 1 - (int)blockIdx.x : (int)blockIdx.x); };
     const int rounds = (n_items + gridDim.x - 1) / gridDim.x;
+    int j = 0, k = 0;                                      // tiles and items so far
 
     if (warp == PRODUCER) {
         if (lane == 0) {
-            int j = 0, k = 0;                              // tiles and items so far
             bool ok = true;
             for (int round = 0; round < rounds && ok && !failed; ++round) {
                 if (item_of(round) >= n_items) continue;
@@ -1474,7 +1474,6 @@ run_weigh_tc_kernel(RunArgs a, int n_items, const __grid_constant__ RtMaps maps)
     } else if (warp == PRODUCER + 1) {
         if (lane == 0) {
             constexpr uint32_t idesc = umma_idesc_bf16(ST_BM, 0);
-            int j = 0, k = 0;
             bool ok = true;
             for (int round = 0; round < rounds && ok && !failed; ++round) {
                 if (item_of(round) >= n_items) continue;
@@ -1505,6 +1504,7 @@ run_weigh_tc_kernel(RunArgs a, int n_items, const __grid_constant__ RtMaps maps)
                 ++k;
             }
             if (!ok) failed = 1;
+            if (failed && j > 0) (void)mbar_wait(bar_sf + 8 * ((j - 1) & 1), ((j - 1) >> 1) & 1);      // (its last product writes to tensor memory)
         }
     } else {
         const int r = (warp & 3) * 32 + lane, col = (warp >> 2) * RT_COLS;      // the row of each tile, the first of its keys
@@ -1521,7 +1521,7 @@ run_weigh_tc_kernel(RunArgs a, int n_items, const __grid_constant__ RtMaps maps)
             }
             return x;
         };
-        int j = 0, round = 0, done = 0;
+        int round = 0, done = 0;
         bool ok = true;
         RtItem x = item_from(round);
         // the rows' statistics, a tile ahead of the scores: where the next tile's lie, and how many tiles its head has left
@@ -1624,6 +1624,10 @@ run_weigh_tc_kernel(RunArgs a, int n_items, const __grid_constant__ RtMaps maps)
     if (warp == PRODUCER) {
         tc_fence_after();
         tmem_dealloc(tmem, 256);
+        if (failed && lane == 0) {                         // a wait ran out: nothing is left on its way into this block's memory
+            for (int i = max(0, j - STAGES); i < j; ++i) (void)mbar_wait(bar_qf + 8 * (i % STAGES), (i / STAGES) & 1);
+            for (int i = max(0, k - 2); i < k; ++i) (void)mbar_wait(bar_kf + 8 * (i & 1), (i >> 1) & 1);
+        }
     }
     if (threadIdx.x == 0 && failed) atomicExch(&gl_wait_failed, 1);
 }
