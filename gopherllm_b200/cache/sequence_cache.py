@@ -133,6 +133,7 @@ class SequenceCache:
         # per-slot bookkeeping
         self._length = [0] * self.max_slots
         self._forgotten = [0] * self.max_slots                 # positions a sequence has lost to ``shrink``
+        self._spoiled: set = set()                             # slots that ``spoil`` was called for
         self._pages: List[List[List[int]]] = [[[] for _ in self.groups] for _ in range(self.max_slots)]
         # per slot and group: pages before this index have been released (groups with a window or chunks only)
         self._first_page: List[List[int]] = [[0 for _ in self.groups] for _ in range(self.max_slots)]
@@ -210,6 +211,13 @@ class SequenceCache:
     def _held(self, slot: int) -> None:
         if not self.slots.is_held(slot):
             raise ValueError(f"slot {slot} is not in use")
+        if slot in self._spoiled:
+            raise ValueError(f"slot {slot}: a change of what it holds failed midway; it can only be closed")
+
+    def spoil(self, slot: int) -> None:
+        """Record that what the sequence holds is no longer one: all that is left is to close it."""
+        self._held(slot)
+        self._spoiled.add(slot)
 
     def pages_needed(self, slot: int, new_len: int) -> int:
         have = len(self._pages[slot][0]) if self.groups else 0
@@ -262,6 +270,7 @@ class SequenceCache:
 
     def close(self, slot: int) -> None:
         """Give back a sequence's pages and slot."""
+        self._spoiled.discard(slot)
         self._held(slot)
         for g in self.groups:
             for p in self._pages[slot][g.gid]:

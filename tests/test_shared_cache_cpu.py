@@ -198,3 +198,69 @@ def test_pages_and_options_of_a_sequence_that_is_cut():
     for kw in (dict(cache_keep=-1), dict(cache_keep=10, cache_recent=11), dict(cache_recent=1), dict(cache_keep=4, cache_first=-1), dict(cache_keep=4.0)):
         with pytest.raises(ValueError):
             GenerationOptions(**kw).validate()
+
+
+class _Net:
+    class spec:
+        vocab = 100
+        max_positions = 640
+
+
+def cutting_engine(monkeypatch, fail_at=0, pages=40, slots=6):
+    """An engine on the CPU whose cuts are written down and of which the ``fail_at``-th fails; its cache has two groups of entries."""
+    import contextlib
+    from gopherllm_b200 import ops
+    from gopherllm_b200.engine.step import Engine
+    c = make(pages=pages, slots=slots, reqs=(KVRequest(1, 8), KVRequest(1, 16), KVRequest(1, 8)), allocate=True, weigh=True, last=5000)
+    assert len(c.groups) == 2
+    calls = []
+
+    def cut(keys, values, weights, length, table, keep, recent, first, to=None):
+        calls.append((keys.shape[-1], length.tolist(), to is None))
+        if len(calls) == fail_at:
+            raise ops.KernelError("no")
+    monkeypatch.setattr(ops, "cache_evict", cut)
+    monkeypatch.setattr(torch.cuda, "device", lambda d: contextlib.nullcontext())
+    return Engine(_Net(), c, torch.float32, "cpu"), c, calls
+
+
+@pytest.mark.parametrize("fail_at", [0, 1, 2, 3, 4])
+def test_a_cut_that_fails_midway(monkeypatch, fail_at):
+    """Cuts onto fresh pages come first, as they can be taken back.  One that fails leaves every sequence as it was; where a sequence's own pages
+    have been cut in one group of layers and not in the next, it can only be closed."""
+    eng, c, calls = cutting_engine(monkeypatch, fail_at)
+    a, short = c.open(), c.open()
+    grow(c, a, 300)
+    grow(c, short, 50)
+    b = c.fork(a, 200)
+    alone = c.open()
+    grow(c, alone, 130)
+    free = [g.pool.free_count for g in c.groups]
+    held = {s: [list(p) for p in c._pages[s]] for s in (a, b, alone)}
+    if fail_at:
+        with pytest.raises(Exception, match="no"):
+            eng.evict([a, alone, short, b], 64)
+    else:
+        eng.evict([a, alone, short, b], 64)
+    assert [x[1:] for x in calls] == [([300, 200], False), ([300, 200], False), ([130], True), ([130], True)][:fail_at or 4]
+    if fail_at:
+        assert [g.pool.free_count for g in c.groups] == free and c.length(a) == 300 and c.length(b) == 200
+        assert all([list(p) for p in c._pages[s]] == held[s] for s in held)
+        if fail_at == 4:
+            for use in (lambda: c.length(alone), lambda: c.position(alone), lambda: c.fork(alone), lambda: c.reserve([(alone, 140)]),
+                        lambda: eng.plan([(alone, [1])], None), lambda: eng.evict([alone], 64)):
+                with pytest.raises(ValueError, match="closed"):
+                    use()
+        else:
+            assert c.length(alone) == 130
+    else:
+        assert [c.length(s) for s in (a, b, alone, short)] == [64, 64, 64, 50]
+    c.check()
+    for s in (a, b, alone, short):
+        c.close(s)
+    c.check()
+    assert all(g.pool.held_count == 0 for g in c.groups)
+    s = c.open()
+    while s != alone:                                              # the slot serves another sequence
+        s = c.open()
+    assert c.length(s) == 0
