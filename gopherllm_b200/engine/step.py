@@ -160,27 +160,26 @@ class Engine:
         alone = [s for s in long if s not in set(shared)]
         fresh = cache.fresh_pages([(s, keep) for s in shared])
         i32 = lambda v: torch.from_numpy(np.ascontiguousarray(v, dtype=np.int32)).to(self.device)  # noqa: E731
-        begun: List[int] = []                              # sequences whose own pages are being cut
+        begun: set = set()                                 # sequences whose own pages are being cut
+        most = max(1, ops.EVICT_MOST // max((g.keys.shape[0] for g in cache.groups), default=1))      # sequences of a launch
         try:
             with torch.cuda.device(self.device):
                 # Onto fresh pages first: until the books are changed below, that can be taken back.
-                for part in (shared, alone):
-                    if not part:
-                        continue
+                for part, moved in [(p[i:i + most], p is shared) for p in (shared, alone) for i in range(0, len(p), most)]:
                     length = i32([cache.length(s) for s in part])
                     used = max(-(-cache.length(s) // PAGE) for s in part)
-                    tables = [(i32(cache.page_rows(g.gid, part)[:, :used]), i32([fresh[s][g.gid] for s in part]) if part is shared else None)
+                    tables = [(i32(cache.page_rows(g.gid, part)[:, :used]), i32([fresh[s][g.gid] for s in part]) if moved else None)
                               for g in cache.groups]
                     for g, (pages, to) in zip(cache.groups, tables):
                         ops.cache_evict(g.keys, g.values, g.weights, length, pages, keep, recent, first, to)
-                        if part is alone:
-                            begun = part
+                        if not moved:
+                            begun.update(part)
         except BaseException:
             for s in fresh:                                # (nothing was recorded: what was taken goes back)
                 for g, pages in zip(cache.groups, fresh[s]):
                     for p in pages:
                         g.pool.give(p)
-            for s in begun:                                # (cut in some layers and not in others)
+            for s in begun:                                # (cut in some layers at least, and not recorded)
                 cache.spoil(s)
             raise
         for s in long:

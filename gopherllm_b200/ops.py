@@ -1166,6 +1166,9 @@ class _EvictArgs(Structure):
                [(n, c_int) for n in ("layers", "B", "nKV", "n_pages", "max_pages", "to_pages", "keep", "recent", "first", "k_bytes", "v_bytes")]
 
 
+EVICT_MOST = 65535                   # sequences times layers of one call
+
+
 def cache_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, weights: torch.Tensor, seq_len: torch.Tensor, pages: torch.Tensor, keep: int,
                 recent: int = 0, first: int = 0, to_pages: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Cuts sequences longer than ``keep`` positions down to that many, layer by layer and key/value head by head: the ``first``
@@ -1201,7 +1204,7 @@ def cache_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, weights: torch.Ten
     es = k_cache.element_size()
     if max(k_cache.shape[-1], v_cache.shape[-1]) * es > 4096 or min(k_cache.shape[-1], v_cache.shape[-1]) < 1:
         raise KernelError(f"cache_evict: heads of {k_cache.shape[-1]} and {v_cache.shape[-1]} are outside 1..{4096 // es}")
-    if heads > 65535 or B * layers > 65535:
+    if heads > 65535 or B * layers > EVICT_MOST:
         raise KernelError(f"cache_evict: {layers} layers of {B} sequences, {heads} heads are more than a launch takes")
     kept = empty((*k_cache.shape[:-4], B, heads, keep), torch.int32, k_cache.device)
     to = pages if to_pages is None else to_pages

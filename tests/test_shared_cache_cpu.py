@@ -264,3 +264,24 @@ def test_a_cut_that_fails_midway(monkeypatch, fail_at):
     while s != alone:                                              # the slot serves another sequence
         s = c.open()
     assert c.length(s) == 0
+
+
+def test_more_layers_and_sequences_than_a_launch_takes_are_cut_in_parts(monkeypatch):
+    from gopherllm_b200 import ops
+    eng, c, calls = cutting_engine(monkeypatch)
+    slots = [c.open() for _ in range(3)]
+    for i, s in enumerate(slots):
+        grow(c, s, 130 + i)
+    slots.append(c.fork(slots[0]))
+    monkeypatch.setattr(ops, "EVICT_MOST", 3)                      # (one group has two layers, the other one)
+    eng.evict(slots, 64)
+    # the group of two layers decides: one sequence a launch
+    assert [x[1:] for x in calls] == [([130], False)] * 4 + [([131], True)] * 2 + [([132], True)] * 2
+    assert [c.length(s) for s in slots] == [64] * 4
+    c.check()
+    monkeypatch.setattr(ops, "EVICT_MOST", 65535)
+    calls.clear()
+    for s in slots:
+        grow(c, s, 70)
+    eng.evict(slots, 64)
+    assert [x[1:] for x in calls] == [([70] * 4, True)] * 2
