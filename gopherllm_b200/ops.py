@@ -1068,6 +1068,8 @@ def attention_prefix(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, 
         raise KernelError(f"attention_prefix: {lay.max_shared} shared pages in a table of {pages.shape[1]}")
     if ints.get_device() != q.get_device():
         raise KernelError(f"attention_prefix: the plan is on {ints.device}")
+    if k_cache.shape[0] == 0:
+        raise KernelError(f"attention_prefix: {B} sequences in a cache of no pages")
     base, at, ml = ints.data_ptr(), None, None
     if lay.slots:
         n = B * num_heads * lay.slots * head_dim
@@ -1108,6 +1110,8 @@ def attention_weighed(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor,
                           f"{pages.shape[1]} pages, the last {last} queries counted")
     if B == 0 or max_qlen == 0:
         return
+    if n_pages == 0:
+        raise KernelError(f"attention_weighed: {B} sequences in a cache of no pages")
     f32 = dtype is torch.float32
     lib = _lib("attention_spans_f32.cu") if f32 else _lib("attention_spans.cu", (f"GL_HEAD_DIM={head_dim}",))
     if max_qlen == 1:

@@ -115,6 +115,23 @@ def test_no_launch_behind_a_refusal(monkeypatch):
     assert len(launched) == 2
 
 
+def test_a_cache_of_no_pages_is_refused(monkeypatch):
+    """Whatever a table says, nothing lies there: no launcher is reached."""
+    monkeypatch.setattr(ops, "_launch_device", lambda t: t.get_device())
+    monkeypatch.setattr(ops, "sm_count", lambda d: 148)
+    monkeypatch.setattr(ops, "_lib", lambda *a: pytest.fail("a launcher was asked for"))
+    i32 = lambda *s: torch.zeros(*s, dtype=torch.int32)  # noqa: E731
+    for dtype in (BF, F):
+        q, k = torch.zeros(2, 256, dtype=dtype), torch.zeros(0, 2, 64, 64, dtype=dtype)
+        for run in (1, 3):
+            with pytest.raises(ops.KernelError, match="no pages"):
+                ops.attention_weighed(q, q.clone(), k, k.clone(), torch.zeros(0, 2, 64), i32(2), i32(2), i32(2), i32(2, 3), 4, 2, 64, run, 100)
+        ops.attention_weighed(q, q.clone(), k, k.clone(), torch.zeros(0, 2, 64), i32(2), i32(2), i32(2), i32(2, 3), 4, 2, 64, 0, 0)      # (no tokens: nothing to do)
+        plan = ops.PrefixPlan(ops.PrefixLayout([([0, 1], 128)], 2, 4, 2, 64, dtype, 5, 148), i32(9))
+        with pytest.raises(ops.KernelError, match="no pages"):
+            ops.attention_prefix(q, q.clone(), k, k.clone(), i32(2), i32(2, 3), plan, 4, 2, 64)
+
+
 ALIGN = -3                                                         # GL_ERR_ALIGN (csrc/common.cuh)
 
 
