@@ -108,50 +108,84 @@ def pages_for(prompt_len: int, max_tokens: int, max_positions: int, keep: int = 
     """Pages a request can come to hold: its prompt plus every token it may feed; with ``keep`` its prompt, and later no
     more than a page beyond that many positions.  What is kept of a sequence that ``shares`` pages moves to others."""
     most = min(prompt_len + max_tokens, max_positions)
+    moves = shares and 0 < keep and keep + PAGE <= most            # (a shorter one is never cut)
     if keep > 0:
-        most = min(most, max(prompt_len, keep + PAGE)) + (keep if shares else 0)
-    return -(-most // PAGE) + (1 if keep > 0 and shares else 0)
+        most = min(most, max(prompt_len, keep + PAGE)) + (keep if moves else 0)
+    return -(-most // PAGE) + (1 if moves else 0)
+
+
+class _Alike:
+    """Prompts that begin with the same page of tokens: their numbers and the tokens that all of them have in common, short of any
+    one's last token (which is run by each, for its logits)."""
+
+    def __init__(self, members: List[int], first: Sequence[int], common: int):
+        self.members, self.first, self.common = members, first, common
+
+    @staticmethod
+    def key(prompt: Sequence[int]):
+        """The same for prompts of a group; None for a prompt that is in none."""
+        return tuple(prompt[:PAGE]) if len(prompt) > PAGE else None
+
+    @classmethod
+    def joined(cls, group: Optional["_Alike"], i: int, prompt: Sequence[int]) -> "_Alike":
+        """The group with one more prompt (None: a group of it alone)."""
+        if group is None:
+            return cls([i], prompt, len(prompt) - 1)
+        first, common = group.first, min(group.common, len(prompt) - 1)
+        if first[:common] != prompt[:common]:
+            common = next((n for n in range(common) if first[n] != prompt[n]), common)
+        return cls(group.members + [i], first, common)
+
+    @property
+    def pages(self) -> int:
+        return self.common // PAGE
 
 
 def begin_alike(prompts: Sequence[Sequence[int]]) -> List[Tuple[List[int], int]]:
     """(members, tokens) for prompts that share their first page of tokens or more: how many whole pages of tokens all members
     have in common, short of any member's last token (which is run by each, for its logits)."""
-    by_first: dict = {}
+    groups: dict = {}
     for i, p in enumerate(prompts):
-        if len(p) > PAGE:
-            by_first.setdefault(tuple(p[:PAGE]), []).append(i)
-    out = []
-    for members in by_first.values():
-        if len(members) < 2:
-            continue
-        least, most = min(prompts[i] for i in members), max(prompts[i] for i in members)      # (all others lie between them)
-        n, end = 0, min(len(prompts[i]) for i in members) - 1
-        while n < end and least[n] == most[n]:
-            n += 1
-        out.append((members, n // PAGE * PAGE))
-    return out
+        key = _Alike.key(p)
+        if key is not None:
+            groups[key] = _Alike.joined(groups.get(key), i, p)
+    return [(g.members, g.pages * PAGE) for g in groups.values() if len(g.members) > 1]
 
 
 def plan_batches(prompt_lens: Sequence[int], max_tokens: int, max_positions: int,
-                 page_budget: int, slot_budget: int, keep: int = 0, shares: bool = False) -> List[List[int]]:
-    """Cut requests, in order, into batches whose worst-case page need fits the cache."""
+                 page_budget: int, slot_budget: int, keep: int = 0, alike: Optional[Sequence[List[int]]] = None) -> List[List[int]]:
+    """Cut requests, in order, into batches whose worst-case page need fits the cache.  ``alike``: the prompts, where those of a batch that
+    begin alike hold their common pages once."""
     batches: List[List[int]] = []
     cur: List[int] = []
     used = 0
+    groups: dict = {}                                              # of the current batch: (prompts, pages of each beside the others, pages of all)
     for i, n in enumerate(prompt_lens):
         if n < 1:
             raise ValueError(f"request {i}: the prompt is empty")
         if n >= max_positions:
             # the reference rejects len(tokens) >= MaxSeqLen before any forward (runtime.go:866-868)
             raise ValueError(f"request {i}: prompt of {n} tokens does not fit {max_positions} positions")
-        need = pages_for(n, max_tokens, max_positions, keep, shares)
-        if need > page_budget:
-            raise ValueError(f"request {i} needs {need * PAGE} cached positions, the cache holds {page_budget * PAGE}")
+        need = alone = pages_for(n, max_tokens, max_positions, keep)
+        if alone > page_budget:
+            raise ValueError(f"request {i} needs {alone * PAGE} cached positions, the cache holds {page_budget * PAGE}")
+        key = None if alike is None else _Alike.key(alike[i])
+        if key is not None:
+            group, each, held = groups.get(key, (None, 0, 0))
+            grown = _Alike.joined(group, i, alike[i])
+            each += pages_for(n, max_tokens, max_positions, keep, True)
+            need = alone if group is None else each - (len(grown.members) - 1) * grown.pages - held
         if cur and (used + need > page_budget or len(cur) >= slot_budget):
             batches.append(cur)
-            cur, used = [], 0
+            cur, used, groups = [], 0, {}
+            need = alone
+            if key is not None:
+                held = 0
+                grown, each = _Alike.joined(None, i, alike[i]), pages_for(n, max_tokens, max_positions, keep, True)
         cur.append(i)
         used += need
+        if key is not None:
+            groups[key] = (grown, each, held + need)
     if cur:
         batches.append(cur)
     return batches
@@ -195,7 +229,7 @@ def generate(engine, prompts: Sequence[Sequence[int]], options: GenerationOption
     cache = engine.cache
     seed = options.seed if options.seed != 0 else time.time_ns()
     batches = plan_batches([len(p) for p in prompts], options.max_tokens, spec.max_positions,
-                           cache.n_pages, cache.max_slots, options.cache_keep, options.share_prefix)
+                           cache.n_pages, cache.max_slots, options.cache_keep, [list(p) for p in prompts] if options.share_prefix else None)
     if options.cache_keep and not getattr(cache, "weigh", False):
         raise ValueError("cache_keep needs a cache that keeps the weight of its positions (load the model with weigh=True)")
     results: List[Optional[GenerationResult]] = [None] * len(prompts)

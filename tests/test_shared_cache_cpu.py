@@ -285,3 +285,72 @@ def test_more_layers_and_sequences_than_a_launch_takes_are_cut_in_parts(monkeypa
         grow(c, s, 70)
     eng.evict(slots, 64)
     assert [x[1:] for x in calls] == [([70] * 4, True)] * 2
+
+
+def host_generate(monkeypatch, engine, prompts, options, vocab=100):
+    """generate() on an engine without a device: every sequence ends with the stop token 9 when ``engine.ends`` says, and says 5 until then."""
+    from gopherllm_b200.engine import generate as gen
+
+    class Sampler:
+        def __init__(self, *a, **k):
+            pass
+
+        def sample(self, logits, rows=None):
+            return logits.argmax(-1).to(torch.int32)
+    monkeypatch.setattr(gen, "DeviceSampler", Sampler)
+    return gen.generate(engine, prompts, options)
+
+
+class _HostEngine:
+    """The cache's side of an engine; ``most``: the most sequences of a step."""
+    device, prepare_decode = "cpu", None
+
+    def __init__(self, cache, evict, ends):
+        self.model, self.cache, self.evict, self.ends, self.most = _Net(), cache, evict, ends, 0
+        self.open, self.close, self.fork = cache.open, cache.close, cache.fork
+
+    def step(self, runs, want=None):
+        self.most = max(self.most, len(runs))
+        self.cache.reserve([(s, self.cache.length(s) + len(t)) for s, t in runs])
+        out = torch.zeros(len(runs), 100)
+        for i, (s, t) in enumerate(runs):
+            self.cache.commit(s, self.cache.length(s) + len(t))
+            out[i, 9 if self.ends(self.cache.position(s)) else 5] = 1.0
+        return out
+
+
+def test_requests_behind_one_text_share_its_pages_when_they_are_counted(monkeypatch):
+    """Four requests behind a text of 640 tokens: ten common pages and one more each, where four sequences of their own take 44."""
+    text = list(range(640))
+    prompts = [[t % 100 for t in text] + [k] * 5 for k in range(4)]
+    for pages, most in ((14, 4), (13, 3), (11, 1)):
+        eng, c, _ = cutting_engine(monkeypatch, pages=pages)
+        host = _HostEngine(c, eng.evict, lambda n: False)
+        host.model = type("N", (), dict(spec=type("S", (), dict(vocab=100, max_positions=2000, stop_tokens=()))))
+        c.max_positions = 2000
+        out = host_generate(monkeypatch, host, prompts, GenerationOptions(max_tokens=20, seed=1, share_prefix=True))
+        assert [len(r.tokens) for r in out] == [20] * 4 and host.most == most
+        c.check()
+        assert all(g.pool.held_count == 0 for g in c.groups)
+    assert plan_batches([645] * 4, 20, 2000, 14, 8, alike=prompts) == [[0, 1, 2, 3]]
+    assert plan_batches([645] * 4, 20, 2000, 14, 8) == [[0], [1], [2], [3]]
+    # a request that shares nothing, or is never cut, needs no second place
+    assert plan_batches([100], 5000, 20480, 9, 8, keep=512, alike=[[1] * 100]) == [[0]]
+    assert plan_batches([100, 100], 20, 20480, 3, 8, keep=512, alike=[[1] * 100, [1] * 100]) == [[0, 1]]
+
+
+@pytest.mark.parametrize("seed", range(30))
+def test_a_batch_fits_whenever_its_sequences_end_or_are_cut(monkeypatch, seed):
+    """Families of prompts with random ends, cut or not, in a cache of just the pages that the batches were planned for."""
+    rng = random.Random(seed)
+    texts = [[rng.randrange(10, 100) for _ in range(400)] for _ in range(3)]
+    prompts = [rng.choice(texts)[:rng.randint(1, 399)] + [rng.randrange(10, 100) for _ in range(rng.randint(1, 80))] for _ in range(8)]
+    keep = rng.choice((0, 70, 130, 200))
+    pages = rng.randint(10, 40)
+    eng, c, _ = cutting_engine(monkeypatch, pages=pages, slots=5)
+    host = _HostEngine(c, eng.evict, lambda n: rng.random() < 0.01)
+    options = GenerationOptions(max_tokens=rng.randint(1, 150), seed=1, stop_tokens=(9,), share_prefix=True, cache_keep=keep, cache_recent=keep // 3)
+    out = host_generate(monkeypatch, host, prompts, options)
+    assert all(r.finish_reason in ("stop", "length") for r in out)
+    c.check()
+    assert all(g.pool.held_count == 0 for g in c.groups)
