@@ -133,6 +133,7 @@ class SequenceCache:
         # per-slot bookkeeping
         self._length = [0] * self.max_slots
         self._forgotten = [0] * self.max_slots                 # positions a sequence has lost to ``shrink``
+        self.sharing = 0               # goes up with every call after which other sequences may share other pages
         self._spoiled: set = set()                             # slots that ``spoil`` was called for
         self._pages: List[List[List[int]]] = [[[] for _ in self.groups] for _ in range(self.max_slots)]
         # per slot and group: pages before this index have been released (groups with a window or chunks only)
@@ -280,6 +281,7 @@ class SequenceCache:
             self._first_page[slot][g.gid] = 0
         self._length[slot] = self._forgotten[slot] = 0
         self.slots.give(slot)
+        self.sharing += 1
 
     @staticmethod
     def _give(g: _Group, page: int) -> None:
@@ -326,6 +328,7 @@ class SequenceCache:
             self._pages[new][g.gid] = pages
             self._first_page[new][g.gid] = self._first_page[slot][g.gid]
         self._length[new], self._forgotten[new] = n, self._forgotten[slot]
+        self.sharing += 1
         return new
 
     def shares_pages(self, slot: int) -> bool:
@@ -383,6 +386,7 @@ class SequenceCache:
                 self._give(g, p)
         self._forgotten[slot] += self._length[slot] - keep
         self._length[slot] = keep
+        self.sharing += 1
 
     def page_rows(self, group: int, slots: Sequence[int], out: Optional[np.ndarray] = None) -> np.ndarray:
         """[len(slots), max_pages_per_seq] int32 page ids (the unused tail and pages released before a

@@ -119,6 +119,8 @@ class Engine:
         heads = {b.mixer.shared_heads for b in getattr(model, "blocks", ()) if getattr(getattr(b, "mixer", None), "shared_heads", None)}
         self.shared_heads = sorted(h for h in heads if span_heads_fit(act_dtype, h[2]))
         self.share_prefixes = True
+        # plans for shared pages, by batch of sequences, as of cache.sharing: (groups, shared positions, layouts by bucket of lengths)
+        self._prefix_at, self._prefixes = 0, {}
         self.overlap_branches = True                         # decode steps run parallel branches on two streams
         self._side_stream = None
         self._copy_stream = None
@@ -258,20 +260,29 @@ class Engine:
 
     def _prefix_layouts(self, slots, ctxs):
         """Plans for the pages that these sequences share, one for each kind of heads; none where reading them once spares too
-        little: a step's attention then takes the sequences one by one, from the same pages."""
-        if not self.shared_heads or not self.share_prefixes or self.cache.weigh:
+        little: a step's attention then takes the sequences one by one, from the same pages.  Made once for a batch of sequences and
+        kept for its steps: until some sequence is forked, closed or cut, or a bucket of lengths is full."""
+        if not self.shared_heads or not self.share_prefixes or self.cache.weigh or not any(g.more for g in self.cache.groups):
             return ()
         from .. import ops
-        groups = self.cache.shared_prefixes(slots)
+        if self._prefix_at != self.cache.sharing or len(self._prefixes) > 256:
+            self._prefix_at, self._prefixes = self.cache.sharing, {}
+        batch = tuple(slots)
+        known = self._prefixes.get(batch)
+        if known is None:
+            groups, shared = self.cache.shared_prefixes(slots), [0] * len(slots)
+            for members, n in groups:
+                for b in members:
+                    shared[b] = n
+            known = self._prefixes[batch] = (groups, shared, {})
+        groups, shared, plans = known
         if not groups:
             return ()
-        shared = [0] * len(slots)
-        for members, n in groups:
-            for b in members:
-                shared[b] = n
         # (sized for a bucket of lengths, as captured steps are)
         own = self._length_bucket(max(c + 1 - s for c, s in zip(ctxs, shared)))
-        layouts = (ops.PrefixLayout(groups, len(slots), *heads, self.act_dtype, own, ops.sm_count(self.device)) for heads in self.shared_heads)
+        layouts = plans.get(own)
+        if layouts is None:
+            layouts = plans[own] = [ops.PrefixLayout(groups, len(slots), *heads, self.act_dtype, own, ops.sm_count(self.device)) for heads in self.shared_heads]
         return tuple(x for x in layouts if x.n_items and x.spared >= SHARED_BYTES + len(slots) * SHARED_BYTES_A_SEQUENCE)
 
     def _stage(self, buf: np.ndarray) -> torch.Tensor:

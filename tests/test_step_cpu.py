@@ -129,3 +129,102 @@ def test_generate_reads_the_failure_word_after_the_prompts_and_at_the_end(monkey
             generate(bad, [[1, 2, 3], [4]], opts)
         assert bad.cache.slots.held_count == 0          # the batch's slots went back all the same
         bad.cache.check()
+
+
+def sharing_engine(monkeypatch, max_tokens=64 * 60, heads=((4, 2, 64), (8, 8, 16))):
+    from gopherllm_b200 import ops
+    from gopherllm_b200.engine import step
+    for where, name in ((ops, "PREFIX_SPARED_BYTES"), (step, "SHARED_BYTES"), (step, "SHARED_BYTES_A_SEQUENCE")):
+        monkeypatch.setattr(where, name, 0)
+    monkeypatch.setattr(ops, "sm_count", lambda d: 148)
+    cache = SequenceCache([KVRequest(2, 16)], max_tokens, 2048, torch.float32, "cpu", allocate=False, max_slots=12)
+    cache.groups[0].keys = torch.zeros(1, 60, 2, 64, 16)           # (what a fork copies)
+    cache.groups[0].values = torch.zeros(1, 60, 2, 64, 16)
+    eng = Engine(_Net(), cache, torch.float32, "cpu")
+    eng.shared_heads = sorted(heads)
+    return eng, cache
+
+
+def test_plans_for_shared_pages_are_made_once_for_a_batch(monkeypatch):
+    """Steps of the same sequences make no plan anew until a bucket of lengths is full or some sequence is forked, closed or cut."""
+    from gopherllm_b200 import ops
+    eng, cache = sharing_engine(monkeypatch)
+    made, looked = [], []
+    layout, look = ops.PrefixLayout, cache.shared_prefixes
+    monkeypatch.setattr(ops, "PrefixLayout", lambda *a: (made.append(a), layout(*a))[1])
+    monkeypatch.setattr(cache, "shared_prefixes", lambda s: (looked.append(tuple(s)), look(s))[1])
+    a = cache.open()
+    cache.reserve([(a, 200)])
+    cache.commit(a, 200)
+    slots = [a, cache.fork(a), cache.fork(a, 64)]
+
+    def step(batch):
+        lay, buf, meta = eng.plan([(s, [1]) for s in batch], None)
+        for s, n in zip(batch, meta["new_lens"]):
+            cache.commit(s, n)
+        for i, plan in enumerate(lay.prefix):
+            o, n = lay.off[f"prefix{i}"]
+            assert list(buf[o:o + n]) == plan.ints.tolist()
+        return lay.prefix
+    first = step(slots)
+    assert len(first) == 2 and len(made) == 2 and len(looked) == 1
+    for _ in range(40):
+        assert all(x is y for x, y in zip(step(slots), first))
+    step(slots[:2])                                                # another batch, and back
+    assert len(made) == 4 and len(looked) == 2
+    step(slots)
+    step(slots[:2])
+    assert len(made) == 4 and len(looked) == 2
+    for _ in range(150):                                           # 64 + 192 own positions of the longest: the next bucket
+        step(slots)
+    assert len(made) == 6 and len(looked) == 2
+    more = cache.fork(slots[2])
+    step(slots)
+    assert len(made) == 8 and len(looked) == 3
+    cache.close(slots[2])
+    assert step(slots[:2])[0].max_shared == 3 and len(looked) == 4
+    cache.shrink(slots[1], 10, cache.fresh_pages([(slots[1], 10)])[slots[1]])
+    assert step(slots[:2]) == () and len(looked) == 5              # (what it shared, it no longer does)
+    cache.close(more)
+
+
+def test_kept_plans_are_those_made_anew(monkeypatch):
+    """Random forks, closes, growth and batches: what is kept is never stale."""
+    import random
+    from gopherllm_b200 import ops
+    from gopherllm_b200.cache.pool import CacheFull
+    rng = random.Random(5)
+    eng, cache = sharing_engine(monkeypatch)
+    seen = 0
+    for _ in range(600):
+        live = cache.live_slots()
+        try:
+            what = rng.random()
+            if not live or what < 0.1:
+                s = cache.open()
+                cache.reserve([(s, 150)])
+                cache.commit(s, 150)
+            elif what < 0.25:
+                s = rng.choice(live)
+                cache.fork(s, rng.randint(0, cache.length(s)))
+            elif what < 0.4:
+                cache.close(rng.choice(live))
+            else:
+                batch = rng.sample(live, rng.randint(1, len(live)))
+                ctxs = [cache.length(s) for s in batch]
+                got = eng._prefix_layouts(batch, ctxs)
+                groups = cache.shared_prefixes(batch)
+                assert (len(got) > 0) == (len(groups) > 0)
+                if groups:
+                    seen += 1
+                    shared = {b: n for members, n in groups for b in members}
+                    own = eng._length_bucket(max(c + 1 - shared.get(b, 0) for b, c in enumerate(ctxs)))
+                    want = [ops.PrefixLayout(groups, len(batch), *h, torch.float32, own, 148) for h in eng.shared_heads]
+                    assert [x.ints.tolist() for x in got] == [x.ints.tolist() for x in want] and [x.key() for x in got] == [x.key() for x in want]
+                cache.reserve([(s, cache.length(s) + 30) for s in batch])
+                for s in batch:
+                    cache.commit(s, cache.length(s) + 30)
+        except CacheFull:
+            if live:
+                cache.close(rng.choice(live))
+    assert seen > 50
