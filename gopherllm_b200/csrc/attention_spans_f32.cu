@@ -801,7 +801,6 @@ static int launch_f32(const SpanF32Args& a, dim3 grid, cudaStream_t stream) {
 }
 // rows a block takes of heads of a given size, streaming: what the registers hold
 static int stream_rows(int hd) { return hd % 4 ? 8 : hd <= 64 ? 8 : hd <= 128 ? 4 : 2; }
-GL_API int gl_attention_span_rows_f32(int hd) { return stream_rows(hd); }
 
 #define ST_HELD_BYTES (56 * 1024)
 #define ST_FACTOR_BYTES (24 * 1024)
