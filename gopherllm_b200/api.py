@@ -74,8 +74,9 @@ class Model:
         self.engine.close(slot)
 
     def fork_sequence(self, slot: int, positions: Optional[int] = None) -> int:
-        """A new sequence that begins as the first ``positions`` (default: all) of an open one.  Their whole pages are shared, held
-        once and, in steps of one token a sequence, read once for all sequences of the batch that share them."""
+        """A new sequence that begins as the first ``positions`` (default: all) of an open one.  Their whole pages are shared and
+        held once.  Steps of one token a sequence also read them once for all sequences of the batch that share them, where that spares
+        enough (some 16 MB a layer and 2 MB a sequence) and the cache is not weighed; other steps read them sequence by sequence."""
         return self.engine.fork(slot, positions)
 
     def evict(self, slots, keep: int, recent: int = 0, first: int = 0) -> None:

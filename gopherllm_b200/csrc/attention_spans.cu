@@ -1033,7 +1033,8 @@ shared_tc_kernel(SpanArgs a, const __grid_constant__ StMaps maps) {
                     if (j0 + i > last) sc[i] = -INFINITY;
             }
             // The powers' reference is a maximum of an earlier page, whichever: what lies above it by less than 2^60 loses nothing, in the
-            // weights (bfloat16 has the range of 32 bits) or in the sums, and takes no search for the maximum.  The first page,
+            // weights (bfloat16 has the range of 32 bits) or in the sums (of values below 2^50: 16,384 pages of them stay in range), and takes no
+            // search for the maximum.  The first page,
             // and one whose sum says that a score lay higher, is done with its own maximum, the output rescaled.
             float mu = m_run == -INFINITY ? 0.f : m_run, sum;
             unsigned pk[32];
@@ -1566,6 +1567,7 @@ run_weigh_tc_kernel(RunArgs a, int n_items, const __grid_constant__ RtMaps maps)
 #pragma unroll
             for (int i = 0; i < RT_COLS; ++i) acc[i] = 0.f;
             for (int i = 0; i < x.n; ++i, ++j) {
+                // (an approximate quotient, off by 2 steps of 2^-23 at most: less than the power beside it)
                 const float m = next.x, inv = __fdividef(1.0f, next.y);
                 if (i + 1 < x.n) next = fetch(x);
                 // (a warp whose wait ran out goes on through the motions: the others meet it at the barrier)

@@ -59,6 +59,7 @@ class StepContext:
 # Bytes that reading shared pages once must spare a layer's decode step before it takes kernels of its own, in place of attention that takes
 # the projection's rows itself or of the whole layer as one kernel.  Measured with 32 heads of 64 and 80: two sequences gain from some 1,900
 # shared positions on (16 to 20 MB), eight from between 256 and 1,024 (18 loses, 59 gains), 32 from between 256 and 300 (65 loses 12 %, 81 gains).
+# Heads of other sizes and numbers go by the same bytes; where their border lies was not measured.
 SHARED_BYTES, SHARED_BYTES_A_SEQUENCE = 16 << 20, 2 << 20
 GRAPH_F32_RUN_BYTES = 128 << 20      # weights of a model for each run of its schedule, up to which 32-bit decode steps are captured
 

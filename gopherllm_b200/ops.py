@@ -837,7 +837,7 @@ def attention(q, out, k_cache, v_cache, ctx, pages, num_heads: int, num_kv_heads
 # A cache that sequences share, and that forgets.
 class PrefixPlan:
     """Which sequences of a batch have their first pages in common, and how their attention is shared out among blocks:
-    made by ``prefix_plan`` for the batch's composition and kept as long as that stays (the sequences' own positions
+    made by ``prefix_plan`` for the batch's composition and good as long as that stays (the sequences' own positions
     may grow).  ``ints`` on the device: the sequences group by group, the items of the shared pages, and for every sequence the
     pages it shares and the slots their results take."""
 
@@ -1057,8 +1057,9 @@ def attention_prefix(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, 
     """Attention of one token a sequence (row b of ``q``, scaled, is sequence b) over the paged cache, the keys and values on
     shared pages read once for all sequences that ``plan`` says share them:
     out[b, h] = sum_j softmax_j(q[b, h] . k[j]) v[j], j = 0..seq_ctx[b].  What ``plan`` says is what ``pages`` holds: a group's
-    members have the same ids in their first columns.  ``seq_ctx``, positions cached before this step, is read on the device:
-    one call captured in a graph serves later steps.  bfloat16 (heads of 16..256 in steps of 16) or float32 (heads up to 256)."""
+    members have the same ids in their first columns.  A member's newest position may lie inside the shared pages; the values behind
+    it there must then be finite, as one product serves all members, with weights of 0 for what one of them does not see.
+    ``seq_ctx``, positions cached before this step, is read on the device: one call captured in a graph serves later steps.  bfloat16 (heads of 16..256 in steps of 16) or float32 (heads up to 256)."""
     B = _need_span("attention_prefix", q, out, k_cache, v_cache, seq_ctx, pages, num_heads, num_kv_heads, head_dim)
     lay, ints = plan.layout, plan.ints
     if lay.call != (B, num_heads, num_kv_heads, head_dim, q.dtype) or q.shape[0] != B:
