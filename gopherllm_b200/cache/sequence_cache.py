@@ -332,7 +332,7 @@ class SequenceCache:
         return new
 
     def shares_pages(self, slot: int) -> bool:
-        return any(p in g.more for g in self.groups for p in self._pages[slot][g.gid])
+        return any(p in g.more for g in self.groups if g.more for p in self._pages[slot][g.gid])
 
     def shared_prefixes(self, slots: Sequence[int]) -> List[Tuple[List[int], int]]:
         """(members, positions) for the sequences among ``slots`` that begin on the same pages: indices into ``slots``, and how many
