@@ -182,6 +182,7 @@ attn_prefill_tc_kernel(AttnArgs a, AttnGate gate, AttnPlace place, AttnStats sta
     gl_grid_wait();                                       // comes after the kernel before
     // tile t: score buffers at columns 256 t and 256 t + 64 (the weights of a page overwrite the first
     // 32 columns of its scores, two a column), output at 256 t + 128
+    int keys = 0, values = 0;                              // pages asked for
 
     if (warp == PRODUCER) {
         // ---- TMA producer ------------------------------------------------------
@@ -203,11 +204,13 @@ attn_prefill_tc_kernel(AttnArgs a, AttnGate gate, AttnPlace place, AttnStats sta
 #pragma unroll
                 for (int s = 0; s < AT_NSEG; ++s)
                     tma_load_2d(sK + st * AT_K_BYTES + at_seg_base(s, GL_PAGE), &maps.k[s], col + at_seg(s).off, row, bar_kf + 8 * st);
+                keys = j + 1;
                 if (j >= AT_STAGES && !mbar_wait(bar_ve + 8 * st, par)) { failed = 1; break; }
                 mbar_expect_tx(bar_vf + 8 * st, AT_V_BYTES);                       // zero fill counts
 #pragma unroll
                 for (int c = 0; c < AT_VATOMS; ++c)
                     tma_load_2d(sV + st * AT_V_BYTES + c * AT_VATOM_BYTES, &maps.v, col + 64 * c, row, bar_vf + 8 * st);
+                values = j + 1;
             }
         }
     } else if (warp > PRODUCER) {
@@ -420,6 +423,11 @@ attn_prefill_tc_kernel(AttnArgs a, AttnGate gate, AttnPlace place, AttnStats sta
     if (warp == PRODUCER) {
         tc_fence_after();
         tmem_dealloc(tmem, AT_TMEM_COLS(NT));
+        if (failed && lane == 0) {                         // a wait ran out: nothing is left on its way into this block's memory
+            (void)mbar_wait(bar_q, 0);
+            for (int j = max(0, keys - AT_STAGES); j < keys; ++j) (void)mbar_wait(bar_kf + 8 * (j % AT_STAGES), (j / AT_STAGES) & 1);
+            for (int j = max(0, values - AT_STAGES); j < values; ++j) (void)mbar_wait(bar_vf + 8 * (j % AT_STAGES), (j / AT_STAGES) & 1);
+        }
     }
     if (threadIdx.x == 0 && failed) atomicExch(&gl_wait_failed, 1);
 }
